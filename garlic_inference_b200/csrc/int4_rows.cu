@@ -1,0 +1,205 @@
+// The key/value cache in 4 bits: new rows in, rows out.
+//
+// Pages are codes [pages, heads, page size, d / 2] bytes and meta [pages, heads, page size, d / 64] words (step, low as two
+// bfloat16): a row of d numbers takes d / 2 + d / 16 bytes, 4.5 bits a number.  A group of 64 numbers of a head has one step:
+//   low = min,  step = (max - min) / 15 rounded up to bfloat16,  q = round((x - low) / step) in 0 .. 15
+// so that a number comes back within half a step.  Every kernel gives a group to 16 lanes, 4 numbers each: 8 bytes
+// of a bfloat16 row, 2 bytes of codes.  All are bound by the 16-bit side (2 bytes a number against 0.56).
+#include "int4.cuh"
+
+#define I4R_THREADS 256
+
+struct Int4Pool { unsigned char* codes; uint32_t* meta; };
+
+// Where a token's rows of the cache are: the page's first row and the row in it, or false.  Bad indexes are reported.
+__device__ __forceinline__ bool i4r_place(int pos, int slot, const int* __restrict__ table, int n_slots, int max_pages, int page_size,
+                                          int n_pages, int* status, bool report, long long& page, int& row) {
+    if (slot < 0) return false;                                          // padding
+    const int lp = pos / page_size;
+    if (pos < 0 || lp >= max_pages || slot >= n_slots) { if (report) atomicExch(status, 1); return false; }
+    page = table[(size_t)slot * max_pages + lp];
+    if (page < 0 || page >= n_pages) { if (report) atomicExch(status, 2); return false; }
+    row = pos - lp * page_size;
+    return true;
+}
+
+// Keys and values of the step's tokens into their pages; k and v: a token's heads k_hs (v_hs) numbers apart, tokens k_ts (v_ts) apart.
+template <typename T>
+__global__ void __launch_bounds__(I4R_THREADS)
+int4_append_kernel(const T* __restrict__ k, long long k_ts, long long k_hs, const T* __restrict__ v, long long v_ts, long long v_hs,
+                   Int4Pool kp, Int4Pool vp, const int* __restrict__ table, const int* __restrict__ tok_pos,
+                   const int* __restrict__ tok_slot, int n_kv, int groups, int n_slots, int max_pages, int page_size, int n_pages,
+                   int vec, long long items, int* __restrict__ status) {
+    gi_pdl_launch_dependents();
+    const long long item = ((long long)blockIdx.x * I4R_THREADS + threadIdx.x) >> 4;
+    const int l = threadIdx.x & 15;
+    const bool live = item < items;                                      // 16 lanes alike; the other half of the warp may differ
+    const int grp = (int)(item % groups), head = (int)(item / groups % n_kv);
+    const bool values = (int)(item / groups / n_kv % 2);
+    const int tok = live ? (int)(item / groups / n_kv / 2) : 0;
+    // positions, slots and the block table are set before the step's first kernel: read before the wait
+    long long page = 0;
+    int row = 0;
+    const int pos = tok_pos[tok], slot = tok_slot[tok];
+    gi_pdl_wait();
+    const bool there = i4r_place(pos, slot, table, n_slots, max_pages, page_size, n_pages, status, live && l == 0, page, row) && live;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (there) {
+        const T* src = (values ? v + tok * v_ts + head * v_hs : k + tok * k_ts + head * k_hs) + grp * I4_GROUP_KV + l * 4;
+        if (vec) {
+            const float4 f = load4_act(src);
+            x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = to_f32(src[i]);
+        }
+    }
+    float mn = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    int odd = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd |= !(fabsf(x[i]) <= 3.402823466e38f);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        odd |= __shfl_xor_sync(0xffffffffu, odd, o);
+    }
+    if (!there) return;
+    float step, low;
+    i4_step_low(mn, mx, !odd, step, low);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits |= i4_code(x[i], step, low) << (4 * i);
+    const Int4Pool pool = values ? vp : kp;
+    const size_t at = (((size_t)page * n_kv + head) * page_size + row) * groups + grp;
+    reinterpret_cast<uint16_t*>(pool.codes)[at * 16 + l] = (uint16_t)bits;
+    if (l == 0) pool.meta[at] = i4_meta(step, low);
+}
+
+template <typename T>
+__device__ __forceinline__ void i4r_unpack4(T* dst, uint32_t bits, uint32_t meta) {
+    const float step = i4_bf16_low(meta), low = i4_bf16_high(meta);
+    store4_act(dst, make_float4(fmaf(step, (float)(bits & 15), low), fmaf(step, (float)((bits >> 4) & 15), low),
+                                fmaf(step, (float)((bits >> 8) & 15), low), fmaf(step, (float)((bits >> 12) & 15), low)));
+}
+
+// What the pages hold of the listed tokens: out [tokens, n_kv, d], zeros for padding and where no page is mapped.
+template <typename T>
+__global__ void __launch_bounds__(I4R_THREADS)
+int4_read_kernel(Int4Pool pool, T* __restrict__ out, const int* __restrict__ table, const int* __restrict__ tok_pos,
+                 const int* __restrict__ tok_slot, int n_kv, int groups, int n_slots, int max_pages, int page_size, int n_pages,
+                 long long items, int* __restrict__ status) {
+    gi_pdl_start();
+    const long long item = ((long long)blockIdx.x * I4R_THREADS + threadIdx.x) >> 4;
+    if (item >= items) return;
+    const int l = threadIdx.x & 15;
+    const int grp = (int)(item % groups), head = (int)(item / groups % n_kv), tok = (int)(item / groups / n_kv);
+    long long page;
+    int row;
+    uint32_t bits = 0, meta = 0;
+    if (i4r_place(tok_pos[tok], tok_slot[tok], table, n_slots, max_pages, page_size, n_pages, status, l == 0, page, row)) {
+        const size_t at = (((size_t)page * n_kv + head) * page_size + row) * groups + grp;
+        bits = reinterpret_cast<const uint16_t*>(pool.codes)[at * 16 + l];
+        meta = pool.meta[at];
+    }
+    i4r_unpack4(out + item * I4_GROUP_KV + l * 4, bits, meta);
+}
+
+// Blocks of 64 positions of the step's sequences as bfloat16 pages of their own, [blocks, n_kv, 64, d], for the prompt kernel on
+// tensor memory, and their block table [n_slots, max_blocks]: block i holds positions 64 b .. of the slot that blocks[i] =
+// {slot, b} names.  Positions without a page are zeros, as are those behind the table's last column.
+__global__ void __launch_bounds__(I4R_THREADS)
+int4_gather_kernel(Int4Pool kp, Int4Pool vp, bf16* __restrict__ k_out, bf16* __restrict__ v_out, int* __restrict__ out_table,
+                   const int2* __restrict__ blocks, const int* __restrict__ table, int n_kv, int groups, int n_slots, int max_pages,
+                   int max_blocks, int page_size, int n_pages, int* __restrict__ status) {
+    gi_pdl_start();
+    const int2 b = blocks[blockIdx.x];
+    const bool ok = b.x >= 0 && b.x < n_slots && b.y >= 0 && b.y < max_blocks;
+    if (blockIdx.y == 0 && threadIdx.x == 0) {
+        if (ok) out_table[(size_t)b.x * max_blocks + b.y] = blockIdx.x;
+        else atomicExch(status, 1);
+    }
+    const int head = blockIdx.y >> 1;
+    const Int4Pool pool = blockIdx.y & 1 ? vp : kp;
+    bf16* out = (blockIdx.y & 1 ? v_out : k_out) + ((size_t)blockIdx.x * n_kv + head) * 64 * groups * I4_GROUP_KV;
+    // 64 rows x groups x 16 lanes; groups is 1 or 2, so a thread's lane and group stay the same from row to row
+    for (int i = threadIdx.x; i < 64 * groups * 16; i += I4R_THREADS) {
+        const int l = i & 15, grp = (i >> 4) % groups, r = (i >> 4) / groups, pos = b.y * 64 + r, lp = pos / page_size;
+        uint32_t bits = 0, meta = 0;
+        if (ok && lp < max_pages) {
+            const int page = __ldg(table + (size_t)b.x * max_pages + lp);
+            if (page >= 0 && page < n_pages) {
+                const size_t at = (((size_t)page * n_kv + head) * page_size + (pos - lp * page_size)) * groups + grp;
+                bits = reinterpret_cast<const uint16_t*>(pool.codes)[at * 16 + l];
+                meta = pool.meta[at];
+            }
+        }
+        i4r_unpack4(out + (size_t)(r * groups + grp) * I4_GROUP_KV + l * 4, bits, meta);
+    }
+}
+
+static int check_pool(const char* who, const void* codes, const void* meta, int n_kv, int d, int page_size, int max_pages, int n_slots) {
+    GI_REQUIRE(n_kv > 0 && d > 0 && d % I4_GROUP_KV == 0 && d <= 1024, "%s: %d heads of %d; heads are multiples of 64 numbers", who, n_kv, d);
+    GI_REQUIRE(page_size > 0 && max_pages > 0 && n_slots > 0, "%s: page and table sizes must be positive", who);
+    GI_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)meta % 16 == 0, "%s: pages must start on 16 bytes", who);
+    return 0;
+}
+
+extern "C" int gi_int4_append(const void* k, long long k_ts, long long k_hs, const void* v, long long v_ts, long long v_hs, int dtype,
+                              void* k_codes, void* k_meta, void* v_codes, void* v_meta, const int* table, const int* tok_pos,
+                              const int* tok_slot, int n_tokens, int n_kv, int d, int n_slots, int max_pages, int page_size,
+                              int n_pages, int* status, void* stream) {
+    if (int rc = check_pool("gi_int4_append", k_codes, k_meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
+    if (int rc = check_pool("gi_int4_append", v_codes, v_meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
+    GI_REQUIRE(n_tokens >= 0, "gi_int4_append: %d tokens", n_tokens);
+    if (n_tokens == 0) return 0;
+    const int groups = d / I4_GROUP_KV;
+    const long long items = (long long)n_tokens * n_kv * 2 * groups, blocks = (items * 16 + I4R_THREADS - 1) / I4R_THREADS;
+    GI_REQUIRE(blocks < 2147483647LL, "gi_int4_append: too many (token, head) pairs");
+    const size_t four = dtype == GI_DTYPE_F32 ? 16 : 8;                  // bytes of four numbers
+    const int vec = (uintptr_t)k % four == 0 && (uintptr_t)v % four == 0 && k_ts % 4 == 0 && k_hs % 4 == 0 && v_ts % 4 == 0 && v_hs % 4 == 0;
+    const Int4Pool kp = {(unsigned char*)k_codes, (uint32_t*)k_meta}, vp = {(unsigned char*)v_codes, (uint32_t*)v_meta};
+    cudaStream_t s = (cudaStream_t)stream;
+#define GI_APPEND(T)                                                                                                                 \
+    gi_launch(int4_append_kernel<T>, dim3((unsigned)blocks), dim3(I4R_THREADS), 0, s, (const T*)k, k_ts, k_hs, (const T*)v, v_ts,    \
+              v_hs, kp, vp, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, vec, items, status)
+    if (dtype == GI_DTYPE_F32) GI_APPEND(float);
+    else if (dtype == GI_DTYPE_BF16) GI_APPEND(bf16);
+    else GI_REQUIRE(false, "gi_int4_append: dtype %d", dtype);
+#undef GI_APPEND
+    return gi_check_launch("gi_int4_append");
+}
+
+extern "C" int gi_int4_read(const void* codes, const void* meta, void* out, int dtype, const int* table, const int* tok_pos,
+                            const int* tok_slot, int n_tokens, int n_kv, int d, int n_slots, int max_pages, int page_size, int n_pages,
+                            int* status, void* stream) {
+    if (int rc = check_pool("gi_int4_read", codes, meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
+    GI_REQUIRE(n_tokens >= 0 && (uintptr_t)out % 16 == 0, "gi_int4_read: %d tokens, the output must start on 16 bytes", n_tokens);
+    if (n_tokens == 0) return 0;
+    const int groups = d / I4_GROUP_KV;
+    const long long items = (long long)n_tokens * n_kv * groups, blocks = (items * 16 + I4R_THREADS - 1) / I4R_THREADS;
+    GI_REQUIRE(blocks < 2147483647LL, "gi_int4_read: too many (token, head) pairs");
+    const Int4Pool pool = {(unsigned char*)codes, (uint32_t*)meta};
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == GI_DTYPE_F32)
+        gi_launch(int4_read_kernel<float>, dim3((unsigned)blocks), dim3(I4R_THREADS), 0, s, pool, (float*)out, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, items, status);
+    else if (dtype == GI_DTYPE_BF16)
+        gi_launch(int4_read_kernel<bf16>, dim3((unsigned)blocks), dim3(I4R_THREADS), 0, s, pool, (bf16*)out, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, items, status);
+    else GI_REQUIRE(false, "gi_int4_read: dtype %d", dtype);
+    return gi_check_launch("gi_int4_read");
+}
+
+extern "C" int gi_int4_gather(const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, void* k_out, void* v_out,
+                              int* out_table, const int* blocks, int n_blocks, const int* table, int n_kv, int d, int n_slots,
+                              int max_pages, int max_blocks, int page_size, int n_pages, int* status, void* stream) {
+    if (int rc = check_pool("gi_int4_gather", k_codes, k_meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
+    if (int rc = check_pool("gi_int4_gather", v_codes, v_meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
+    GI_REQUIRE(n_blocks >= 0 && max_blocks > 0 && n_kv <= 32767 && (uintptr_t)blocks % 8 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
+               "gi_int4_gather: %d blocks of %d heads; blocks must start on 8 bytes, the pages on 16", n_blocks, n_kv);
+    if (n_blocks == 0) return 0;
+    const Int4Pool kp = {(unsigned char*)k_codes, (uint32_t*)k_meta}, vp = {(unsigned char*)v_codes, (uint32_t*)v_meta};
+    gi_launch(int4_gather_kernel, dim3((unsigned)n_blocks, (unsigned)(2 * n_kv)), dim3(I4R_THREADS), 0, (cudaStream_t)stream, kp, vp, (bf16*)k_out,
+              (bf16*)v_out, out_table, (const int2*)blocks, table, n_kv, d / I4_GROUP_KV, n_slots, max_pages, max_blocks, page_size,
+              n_pages, status);
+    return gi_check_launch("gi_int4_gather");
+}

@@ -112,6 +112,13 @@ _SIGNATURES = {
     "gi_sample_chunks": ([I], I),
     "gi_sample_uniform": ([c_ulonglong, L, I, I], F),
     "gi_sample_uniform_from_hash": ([c_ulonglong], F),
+    "gi_int4_quantize_weight": ([P, I, L, P, I, I, P], I),
+    "gi_int4_dequantize_weight": ([P, P, I, I, I, I, I, P], I),
+    "gi_int4_linear": ([P, P, P, I, L, I, I, I, I, I, F, F, F, F, I, P], I),
+    "gi_int4_append": ([P, L, L, P, L, L, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, P], I),
+    "gi_int4_read": ([P, P, P, I, P, P, P, I, I, I, I, I, I, I, P, P], I),
+    "gi_int4_gather": ([P, P, P, P, P, P, P, P, I, P, I, I, I, I, I, I, I, P, P], I),
+    "gi_int4_attention": ([P, P, P, P, P, P, P, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, P], I),
     "gi_random_normal": ([P, I, L, c_ulonglong, F, F, P], I),
     "gi_random_sum12": ([c_ulonglong, c_ulonglong], I),
 }

@@ -15,6 +15,7 @@ Which product runs:
     `torch.mm`), float32 accumulation, or this package's tcgen05 kernel when
     `LARGE_GEMM` says so.  Upstream uses the same library for all
     its products (src/src-cuda/mat-ops/gemm/gemm.cu:22-41).
+  * weight in 4 bits (`int4.Int4Weight`): see `_int4`.
 `swiglu_product` is the gate/up product of a SwiGLU feed-forward with its activation: one
 tcgen05 kernel for prompts, product and SwiGLU kernel otherwise.
 """
@@ -25,7 +26,7 @@ from typing import Optional
 
 import torch
 
-from . import kernels
+from . import int4, kernels
 from .library import KernelError
 
 # Which product takes bfloat16 weights with more than SKINNY_MAX_ROWS rows of x: "library" (cuBLAS through
@@ -67,7 +68,55 @@ def _streamk_min_bytes(m: int) -> int:
     return STREAMK_MIN_BYTES_WIDE if SKINNY_MAX_ROWS < m <= STREAMK_WIDE_MAX_ROWS else STREAMK_MIN_BYTES
 
 
-def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+INT4_CODES_MAX_ROWS = 64          # up to here: the kernel that reads the codes; more rows: the weight made wide first
+INT4_WIDE_BYTES = 64 << 20        # of a weight made wide at a time: it stays in L2 between the two kernels
+
+
+def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Optional[tuple] = None,
+          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The product with a weight in 4 bits, or (`unit`) the gated unit of its halves.  Few rows of bfloat16: the kernel that
+    reads the codes.  More, or float32: the weight is made wide, some outputs at a time, for the products that `linear`
+    has for that type; bfloat16 rounds each of its numbers once on the way (by half a step of 2^-8, a hundredth
+    of what 4 bits leave of it)."""
+    if x.dim() != 2 or x.shape[1] != w.k:
+        raise KernelError(f"linear: x {tuple(x.shape)} does not fit a weight {w.shape} ([out, in])")
+    if unit is not None and w.n % 2:
+        raise KernelError(f"linear: {w.n} outputs cannot be a gate and an up half")
+    m, n = x.shape[0], w.n if unit is None else w.n // 2
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    if m == 0:
+        return out
+    if unit is not None and (x.dtype != torch.bfloat16 or n % 16):
+        return kernels.glu(_int4(x, w, torch.float32), unit, out=out) if out_dtype == torch.float32 else \
+            _narrow(kernels.glu(_int4(x, w, torch.float32), unit), out)
+    if x.dtype == torch.bfloat16 and (m <= INT4_CODES_MAX_ROWS or w.k % 8 or x.data_ptr() % 16):
+        for r in range(0, m, int4.LINEAR_MAX_ROWS):
+            int4.linear_rows(x[r:r + int4.LINEAR_MAX_ROWS], w, out_dtype, unit, out[r:r + int4.LINEAR_MAX_ROWS])
+        return out
+    if unit is not None:
+        return kernels.gemm_tcgen05_glu_bf16(x, int4.dequantize_weight(w), unit, out=out)
+    per = max(256, INT4_WIDE_BYTES // (w.k * x.element_size()) // 256 * 256)
+    for a in range(0, w.n, per):
+        b = min(per, w.n - a)
+        wide = int4.dequantize_weight(w, x.dtype, a, b)
+        if x.dtype == torch.float32:
+            out[:, a:a + b] = kernels.cast(kernels.sgemm_nt(x, wide), out_dtype)
+        elif b == w.n:
+            return kernels.gemm_tcgen05_bf16(x, wide, out_dtype)
+        else:
+            out[:, a:a + b] = kernels.gemm_tcgen05_bf16(x, wide, out_dtype)
+    return out
+
+
+def _narrow(y: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    out.copy_(kernels.cast(y, out.dtype))
+    return out
+
+
+def linear(x: torch.Tensor, w, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    if isinstance(w, int4.Int4Weight):
+        return _int4(x, w, out_dtype or x.dtype)
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise KernelError(f"linear: x {tuple(x.shape)} does not fit a weight {tuple(w.shape)} ([out, in])")
     out_dtype = out_dtype or x.dtype
@@ -100,6 +149,8 @@ def swiglu_product(x: torch.Tensor, w_gate_up: torch.Tensor) -> torch.Tensor:
     """silu(x . Wg^T) * (x . Wu^T) for the packed weight [Wg; Wu]: prompts in bfloat16 run it as one tcgen05
     kernel (product and activation), decode batches of 1 to 8 as one skinny (or gemv) kernel, everything else as the
     product of `linear` and the SwiGLU kernel."""
+    if isinstance(w_gate_up, int4.Int4Weight):
+        return _int4(x, w_gate_up, x.dtype, kernels.glu_shape("silu"))
     m, k = x.shape
     if (FUSED_SWIGLU_MIN_ROWS > 0 and m >= FUSED_SWIGLU_MIN_ROWS and x.dtype == torch.bfloat16
             and w_gate_up.dtype == torch.bfloat16 and k % 8 == 0 and w_gate_up.shape[0] % 2 == 0
@@ -120,6 +171,8 @@ def glu_product(x: torch.Tensor, w_gate_up: torch.Tensor, unit: tuple, out: Opti
     `kernels.glu_shape` tuple), into `out` (columns of a wider matrix) when given: the same choice of kernels as
     `swiglu_product` makes, with the unit in the product's epilogue for prompts and for decode batches of 1 to 8,
     and the product of `linear` followed by the row-wise kernel otherwise."""
+    if isinstance(w_gate_up, int4.Int4Weight):
+        return _int4(x, w_gate_up, x.dtype, unit, out)
     m, k = x.shape
     fits = (x.dtype == torch.bfloat16 and w_gate_up.dtype == torch.bfloat16 and k % 8 == 0 and w_gate_up.shape[0] % 2 == 0
             and x.data_ptr() % 16 == 0 and w_gate_up.data_ptr() % 16 == 0)

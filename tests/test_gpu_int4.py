@@ -1,0 +1,395 @@
+"""Weights and cache rows in 4 bits on the GPU: every entry point against the formulas in 64 bits (plain_int4.py)."""
+import random
+
+import pytest
+import torch
+
+import plain_int4 as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from garlic_inference_b200 import ops
+    return ops
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV)
+
+
+# ------------------------------------------------------------------------------------------------------------ weights
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,k", [(16, 128), (1, 1), (37, 300), (128, 4096), (5, 127)])
+def test_weights_are_quantised_by_the_formula(ops, n, k, dtype):
+    w = (randn(gen(n + k), n, k) * 0.02 + 0.003).to(dtype)
+    w[0, :min(k, 128)] = 0.25                                # a group of equal numbers has step 0
+    got = ops.int4.quantize_weight(w)
+    codes, step, low = plain.unpack_weight(got)
+    want = plain.quantise(w, 128)
+    assert torch.equal(step, want[1]) and torch.equal(low, want[2])
+    # float32 quotients may round to the other side of a half; half a step either way then
+    differ = codes != want[0]
+    assert int((codes - want[0]).abs().max()) <= 1
+    if bool(differ.any()):
+        x = ((w.double() - low.repeat_interleave(128, -1)[:, :k]) / step.repeat_interleave(128, -1)[:, :k])[differ]
+        assert float((x - x.floor() - 0.5).abs().max()) < 2 ** -18
+    back = plain.values(codes, step, low, 128)
+    assert float((back - w.double()).abs().sub(step.repeat_interleave(128, -1)[:, :k] * (0.5 + 2 ** -18)).max()) <= 0
+    for t in (torch.bfloat16, torch.float32):
+        assert torch.equal(ops.int4.dequantize_weight(got, t), back.float().to(t))
+    if n > 3:
+        assert torch.equal(ops.int4.dequantize_weight(got, torch.float32, 2, n - 3), back.float()[2:n - 1])
+
+
+def test_weights_whose_numbers_are_not_finite(ops):
+    w = randn(gen(3), 20, 256).to(torch.bfloat16)
+    w[2, 5], w[3, 200], w[4, 0] = NAN, INF, -INF
+    w[5, :128] = 3.3e38
+    w[5, :64] = -3.3e38
+    codes, step, low = plain.unpack_weight(ops.int4.quantize_weight(w))
+    bad = torch.zeros(20, 2, dtype=torch.bool, device=DEV)
+    bad[2, 0] = bad[3, 1] = bad[4, 0] = True
+    assert torch.equal(torch.isnan(step), bad) and torch.equal(torch.isnan(low), bad)
+    assert codes[5, :128].unique().tolist() == [0, 15]
+
+
+def linear_bound(x, w):
+    """How far the kernel that reads codes may be off: the result's rounding is the caller's.  Float32 roundings of sums whose numbers
+    add up to A = sum step code |x| + |low| |x|: 8 in a group, 2 a group, 8 blocks and 16 of the ends; and what the two parts
+    of x leave, 2^-21 of the row's largest number."""
+    codes, step, low = plain.unpack_weight(w)
+    zero = torch.zeros_like(low)
+    sq, lo = plain.values(codes, step, zero, 128), plain.values(torch.zeros_like(codes), zero, low.abs(), 128)
+    a = x.double().abs() @ (sq + lo).t()
+    return (32 + 2 * step.shape[1]) * 2 ** -24 * a + 2 ** -21 * x.double().abs().amax(1, keepdim=True) * sq.sum(1)[None]
+
+
+def random_weight(ops, g, n, k):
+    codes = torch.randint(0, 16, (n, k), generator=g, device=DEV)
+    groups = -(-k // 128)
+    step = (0.2 + torch.rand(n, groups, generator=g, device=DEV)) * 0.01
+    low = -step * (6 + 3 * torch.rand(n, groups, generator=g, device=DEV))
+    return ops.int4.Int4Weight(plain.pack_weight(codes, step, low), n, k)
+
+
+SHAPES = [(1, 16, 128), (1, 6144, 4096), (2, 1, 1), (3, 777, 1347), (5, 48, 640), (8, 4096, 1024), (8, 33, 9000), (9, 256, 256), (13, 100, 4100),
+          (16, 512, 12288), (17, 64, 384), (40, 130, 1000)]
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_linear(ops, m, n, k, out_dtype):
+    g = gen(m * 1000 + n + k)
+    w = random_weight(ops, g, n, k)
+    x = (randn(g, m, k) * torch.exp(randn(g, k))).to(torch.bfloat16)
+    got = ops.linear(x, w, out_dtype)
+    assert got.shape == (m, n) and got.dtype == out_dtype
+    want = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    bound = linear_bound(x, w) * 1.0 + (2 ** -8 if out_dtype == torch.bfloat16 else 2 ** -24) * want.abs()
+    worst = ((got.double() - want).abs() / bound).max()
+    assert float(worst) <= 1, float(worst)
+    assert torch.equal(got, ops.linear(x, w, out_dtype))
+
+
+@pytest.mark.parametrize("ranks", range(1, 9))
+def test_linear_with_any_number_of_blocks_to_share_the_inputs(ops, ranks):
+    g = gen(ranks)
+    w = random_weight(ops, g, 1500, 1152)                    # 9 groups: uneven shares, and none for some
+    x = randn(g, 7, 1152).to(torch.bfloat16)
+    want = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    got = ops.int4.linear_rows(x, w, torch.float32, ranks=ranks)
+    assert float(((got.double() - want).abs() / (linear_bound(x, w) + 2 ** -24 * want.abs())).max()) <= 1
+
+
+@pytest.mark.parametrize("m", [1, 7, 16, 33])
+@pytest.mark.parametrize("inter,k", [(16, 128), (768, 1024), (40, 200), (2000, 640)])
+def test_gated_units(ops, m, inter, k):
+    from garlic_inference_b200.ops import kernels
+    g = gen(m + inter + k)
+    w = random_weight(ops, g, 2 * inter, k)
+    x = randn(g, m, k).to(torch.bfloat16)
+    y = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    off = linear_bound(x, w)
+    gate, up = y[:, :inter], y[:, inter:]
+    # |silu'| <= 1.1, |gelu'| <= 1.13
+    for unit, act in ((kernels.glu_shape("silu"), lambda z: z * torch.sigmoid(z)),
+                      (kernels.glu_shape("gelu_tanh", gate_max=1.0, up_limit=0.5, up_shift=1.0),
+                       lambda z: torch.nn.functional.gelu(z, approximate="tanh"))):
+        gg, uu = (gate, up) if unit[0] == 0 else (gate.clamp(max=1.0), up.clamp(-0.5, 0.5) + 1.0)
+        want = act(gg) * uu
+        got = ops.swiglu_product(x, w) if unit[0] == 0 else ops.glu_product(x, w, unit)
+        # the function of a float32 is within 2^-20 of itself
+        bound = 2 ** -8 * want.abs() + 1.13 * off[:, :inter] * uu.abs() + act(gg).abs() * off[:, inter:] + 2 ** -19 * (gg * uu).abs() + 2 ** -30
+        assert got.dtype == torch.bfloat16 and got.shape == (m, inter)
+        assert float(((got.double() - want).abs() / bound).max()) <= 1
+    wide = torch.full((m, inter + 24), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.glu_product(x, w, kernels.glu_shape("silu"), out=wide[:, 8:8 + inter])
+    assert torch.equal(wide[:, 8:8 + inter], ops.swiglu_product(x, w))
+    assert bool((wide[:, :8] == 7).all()) and bool((wide[:, 8 + inter:] == 7).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(70, 96, 256), (130, 700, 1024), (100, 40, 333), (257, 512, 640)])
+def test_linear_of_many_rows_and_of_float32(ops, m, n, k):
+    g = gen(m + n + k)
+    w = random_weight(ops, g, n, k)
+    x = randn(g, m, k)
+    wide = plain.values(*plain.unpack_weight(w), 128)
+    # float32: numbers of the weight rounded once, then a float32 product of k numbers
+    want = x.double() @ wide.t()
+    a = x.double().abs() @ wide.abs().t()
+    assert float(((ops.linear(x, w).double() - want).abs() / (a * (k + 4) * 2 ** -24)).max()) <= 1
+    # bfloat16: numbers of the weight rounded to bfloat16 where the weight is made wide
+    xb = x.to(torch.bfloat16)
+    want = xb.double() @ wide.t()
+    a = xb.double().abs() @ wide.abs().t()
+    bound = a * (2 ** -8 + (k + 4) * 2 ** -24) + linear_bound(xb, w) + 2 ** -8 * want.abs()
+    assert float(((ops.linear(xb, w).double() - want).abs() / bound).max()) <= 1
+    if n % 2 == 0:
+        got = ops.swiglu_product(xb, w).double()
+        gate, up = want.chunk(2, 1)
+        off = bound
+        silu = gate * torch.sigmoid(gate)
+        # both factors rounded to bfloat16 first where the activation is the product's last step
+        tol = 2 ** -8 * (silu * up).abs() + (1.1 * (off[:, :n // 2] + 2 ** -8 * gate.abs())) * (up.abs() + off[:, n // 2:]) \
+            + (silu.abs() + 2 ** -8 * gate.abs()) * (off[:, n // 2:] + 2 ** -8 * up.abs()) + 2 ** -18 * (gate * up).abs() + 2 ** -30
+        assert float(((got - silu * up).abs() / tol).max()) <= 1
+
+
+def test_rows_of_x_that_are_not_finite_or_huge_or_tiny(ops):
+    g = gen(11)
+    w = random_weight(ops, g, 70, 700)
+    x = randn(g, 8, 700).to(torch.bfloat16)
+    x[1, 3], x[2, 300], x[3, 10], x[3, 11] = NAN, INF, INF, -INF
+    x[4] *= 1e36
+    x[5] *= 1e-37
+    x[6] = 0
+    x[7, 5] = 1e4                                            # one large number among ordinary ones
+    wide = plain.values(*plain.unpack_weight(w), 128)
+    want = x.double() @ wide.t()
+    got = ops.linear(x, w, torch.float32).double()
+    assert bool(torch.isnan(got[1]).all()) and bool(torch.isnan(got[3]).sum() == torch.isnan(want[3]).sum())
+    assert torch.equal(torch.isinf(got[2]), torch.isinf(want[2])) and torch.equal(got[2] > 0, want[2] > 0)
+    for r in (0, 4, 5, 6, 7):
+        bound = linear_bound(x[r:r + 1], w)[0] * 1.0 + (700 * 2 ** -24) * (x[r].double().abs() @ wide.abs().t()) + 2 ** -140
+        assert float(((got[r] - want[r]).abs() / bound).max()) <= 1, r
+    clean = x.clone()
+    clean[1:4] = 1.0
+    assert torch.equal(ops.linear(clean, w, torch.float32)[[0, 5, 6, 7]].double(), got[[0, 5, 6, 7]])      # neighbours see nothing of it
+
+
+# -------------------------------------------------------------------------------------------------------------- cache
+def make_cache(ops, g, sequences, heads, d, page, spare=2, scale=1.0):
+    """Pages of sequences of the given lengths, in random order, filled by `append`; (k_rows, v_rows, table, status, k, v)."""
+    need = [-(-n // page) for n in sequences]
+    n_pages, width = sum(need) + spare, max(need) + 1
+    order = torch.randperm(n_pages, generator=torch.Generator().manual_seed(7)).tolist()
+    table = torch.full((len(sequences), width), -1, dtype=torch.int32)
+    at = 0
+    for s, c in enumerate(need):
+        table[s, :c] = torch.tensor(order[at:at + c], dtype=torch.int32)
+        at += c
+    table = table.to(DEV)
+    rows = [ops.int4.Int4Rows.zeros(n_pages, heads, page, d, DEV) for _ in range(2)]
+    for r in rows:                                           # what pages held before is garbage, NaN among it
+        r.codes.fill_(0xA5)
+        r.meta.fill_(NAN)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    pos = torch.cat([torch.arange(n) for n in sequences]).to(torch.int32).to(DEV)
+    slot = torch.cat([torch.full((n,), s) for s, n in enumerate(sequences)]).to(torch.int32).to(DEV)
+    k = (randn(g, len(pos), heads, d) * scale + 0.5 * randn(g, heads, d)).to(torch.bfloat16)
+    v = (randn(g, len(pos), heads, d) + 0.3).to(torch.bfloat16)
+    ops.int4.append(k, v, *rows, table, pos, slot, status)
+    assert int(status) == 0
+    return rows[0], rows[1], table, status, k, v, pos, slot
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,d,page", [(1, 64, 16), (3, 128, 64), (8, 128, 32), (2, 256, 7), (5, 64, 1)])
+def test_append_and_read(ops, heads, d, page, dtype):
+    g = gen(heads * d + page)
+    tokens, slots = 45, 3
+    rows = [ops.int4.Int4Rows.zeros(60, heads, page, d, DEV) for _ in range(2)]
+    before = [(r.codes.clone(), r.meta.clone()) for r in rows]
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    width = -(-20 // page)
+    table = torch.randperm(60, generator=torch.Generator().manual_seed(1))[:slots * width].reshape(slots, width).to(torch.int32).to(DEV)
+    pos = torch.tensor([i % 15 for i in range(tokens)], dtype=torch.int32, device=DEV)
+    slot = torch.tensor([i // 15 for i in range(tokens)], dtype=torch.int32, device=DEV)
+    slot[4] = -1
+    wide = (randn(g, tokens, 2 * heads + 1, d + 3) * torch.exp(randn(g, d + 3))).to(dtype)        # strides of their own, odd starts
+    k, v = wide[:, :heads, 3:], wide[:, heads + 1:, :d]
+    k[7, 0, :64] = 0.5
+    ops.int4.append(k, v, *rows, table, pos, slot, status)
+    for r, x, b in zip(rows, (k, v), before):
+        codes, step, low = plain.quantise(x, 64)
+        want = plain.values(codes, step, low, 64)
+        want[4] = 0
+        got = ops.int4.read(r, table, pos, slot, status, torch.float32)
+        flip = (got.double() != want.float().double())
+        if bool(flip.any()):                                 # a quotient next to a half, in float32
+            st = step.repeat_interleave(64, -1)
+            u = ((x.double() - low.repeat_interleave(64, -1)) / st)[flip]
+            assert float((u - u.floor() - 0.5).abs().max()) < 2 ** -18
+        assert torch.equal(ops.int4.read(r, table, pos, slot, status), got.to(torch.bfloat16))
+        # nothing but the tokens' rows was written
+        touched = torch.zeros(60, page, dtype=torch.bool, device=DEV)
+        live = slot >= 0
+        touched[table[slot[live].long(), (pos[live] // page).long()].long(), (pos[live] % page).long()] = True
+        assert torch.equal(r.codes.transpose(1, 2)[~touched], b[0].transpose(1, 2)[~touched])
+        assert torch.equal(r.meta.transpose(1, 2)[~touched], b[1].transpose(1, 2)[~touched])
+    assert int(status) == 0
+
+
+def test_rows_whose_numbers_are_not_finite_or_far_apart(ops):
+    k = randn(gen(5), 6, 1, 128).to(torch.bfloat16)
+    k[0, 0, 3], k[1, 0, 100], k[2, 0, 0] = NAN, INF, -INF
+    k[3, 0, :64], k[3, 0, :32] = 3.3e38, -3.3e38
+    k[4, 0, :64] = 1e-40
+    k[4, 0, 0] = 0
+    rows = [ops.int4.Int4Rows.zeros(1, 1, 8, 128, DEV) for _ in range(2)]
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    pos, slot = torch.arange(6, dtype=torch.int32, device=DEV), torch.zeros(6, dtype=torch.int32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.int4.append(k, k, *rows, table, pos, slot, status)
+    got = ops.int4.read(rows[0], table, pos, slot, status, torch.float32)[:, 0]
+    nan = torch.isnan(got.unflatten(1, (2, 64)))
+    assert bool(nan[0, 0].all()) and bool(nan[1, 1].all()) and bool(nan[2, 0].all())
+    assert int(nan.sum()) == 3 * 64
+    # the step is rounded up by at most 2^-7 of itself, and the largest number is 15 steps, twice its own size, above the lowest
+    assert float((got[3, :64].double() / k[3, 0, :64].double() - 1).abs().max()) <= 2 * 2 ** -7
+    assert float((got[4, :64].double() - k[4, 0, :64].double()).abs().max()) <= 1e-40 / 15
+
+
+def test_places_outside_the_cache_are_reported_and_not_written(ops):
+    rows = [ops.int4.Int4Rows.zeros(2, 1, 4, 64, DEV) for _ in range(2)]
+    table = torch.tensor([[0, 1, -1], [5, -1, -1]], dtype=torch.int32, device=DEV)
+    x = randn(gen(1), 1, 1, 64).to(torch.bfloat16)
+    q = randn(gen(2), 1, 2, 64).to(torch.bfloat16)
+    for pos, slot, codes in ((12, 0, (1, 1, 4)), (-1, 0, (1, 1, 4)), (8, 0, (2, 2, 5)), (0, 1, (2, 2, 5)), (0, 2, (1, 1, 4))):
+        p, s = (torch.tensor([t], dtype=torch.int32, device=DEV) for t in (pos, slot))
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        ops.int4.append(x, x, *rows, table, p, s, status)
+        assert int(status) == codes[0]
+        assert not bool(rows[0].codes.any()) and not bool(rows[1].meta.any())
+        status.zero_()
+        assert not bool(ops.int4.read(rows[0], table, p, s, status).any()) and int(status) == codes[1]
+        status.zero_()
+        assert not bool(ops.int4.attention_decode(q, *rows, table, p, s, 0.125, 0, status).any()) and int(status) == codes[2]
+
+
+def check_attention(got, want, bound):
+    bad = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), bad)
+    worst = ((got.double() - want).abs() / (bound + 1e-30))[~bad].max()
+    assert float(worst) <= 1, float(worst)
+
+
+DECODE = [
+    # heads, kv heads, d, page, lengths, window
+    (1, 1, 64, 16, [1], 0),
+    (4, 1, 128, 64, [1, 2, 31, 32, 33, 64, 65, 127, 128, 129], 0),
+    (32, 8, 128, 64, [2048, 5, 700], 0),
+    (16, 2, 64, 32, [300, 1000, 17], 0),
+    (15, 3, 128, 7, [100, 250, 6], 0),
+    (24, 2, 64, 128, [129, 511], 0),
+    (48, 2, 128, 64, [400, 90], 0),
+    (8, 4, 128, 64, [1000, 40, 200], 64),
+    (8, 1, 64, 16, [1000, 40, 333], 37),
+    (3, 1, 128, 64, [500], 1),
+]
+
+
+@pytest.mark.parametrize("splits", [None, 1, 3])
+@pytest.mark.parametrize("heads,kv,d,page,lengths,window", DECODE)
+def test_decode(ops, heads, kv, d, page, lengths, window, splits):
+    g = gen(heads + d + page + len(lengths))
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, lengths, kv, d, page)
+    order = list(range(len(lengths)))
+    random.Random(3).shuffle(order)
+    slots = order[:1] + [-1] + order[1:]                     # an idle row between
+    q = (1.5 * randn(g, len(slots), heads, d)).to(torch.bfloat16)
+    pos = torch.tensor([lengths[s] - 1 if s >= 0 else 0 for s in slots], dtype=torch.int32, device=DEV)
+    slot = torch.tensor(slots, dtype=torch.int32, device=DEV)
+    got = ops.int4.attention_decode(q, k_rows, v_rows, table, pos, slot, d ** -0.5, window, status, n_splits=splits)
+    spans = [(s, i, 1, lengths[s] - 1) for i, s in enumerate(slots) if s >= 0]
+    check_attention(got, *plain.attention(q, k_rows, v_rows, table, spans, d ** -0.5, window))
+    assert int(status) == 0 and not bool(got[1].any())
+    assert torch.equal(got, ops.int4.attention_decode(q, k_rows, v_rows, table, pos, slot, d ** -0.5, window, status, n_splits=splits))
+
+
+def runs_and_blocks(spans, window):
+    runs = sorted(((s, r + a, min(128, n - a), p + a) for s, r, n, p in spans for a in range(0, n, 128)), key=lambda t: -(t[2] + t[3]))
+    blocks = [(s, b) for s, r, n, p in spans for b in range((max(0, p - window + 1) if window else 0) // 64, -(-(p + n) // 64))]
+    return torch.tensor(runs, dtype=torch.int32, device=DEV), torch.tensor(blocks, dtype=torch.int32, device=DEV)
+
+
+PROMPT = [
+    # heads, kv heads, d, page, (cached, new), window
+    (4, 2, 128, 64, [(0, 1)], 0),
+    (4, 1, 64, 16, [(0, 5), (30, 1), (100, 3)], 0),
+    (8, 2, 128, 64, [(500, 4), (64, 4), (0, 2)], 0),
+    (5, 1, 128, 32, [(700, 5), (0, 17)], 40),
+    (32, 8, 128, 64, [(0, 300), (200, 130)], 0),
+    (6, 3, 64, 64, [(0, 129), (1000, 64), (60, 70)], 0),
+    (4, 2, 128, 16, [(300, 200), (0, 40)], 100),
+    (16, 1, 64, 7, [(90, 33), (0, 64)], 0),
+]
+
+
+@pytest.mark.parametrize("heads,kv,d,page,seqs,window", PROMPT)
+def test_prompt(ops, heads, kv, d, page, seqs, window):
+    g = gen(heads + d + page + len(seqs))
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [p + n for p, n in seqs], kv, d, page)
+    spans, row = [], 0
+    for s, (p, n) in enumerate(seqs):
+        spans.append((s, row, n, p))
+        row += n
+    q = (1.5 * randn(g, row + 2, heads, d)).to(torch.bfloat16)        # two rows in no run
+    runs, blocks = runs_and_blocks(spans, window)
+    got = ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, d ** -0.5, window, status)
+    want, bound = plain.attention(q, k_rows, v_rows, table, spans, d ** -0.5, window)
+    # where keys and values are made wide, each of their numbers is rounded to bfloat16, and so are the probabilities
+    wide_bound = bound.clone()
+    for s, r, n, p in spans:
+        kc, ks, kl = plain.sequence(k_rows, table[s], p + n)
+        vc, vs, vl = plain.sequence(v_rows, table[s], p + n)
+        k, v = plain.values(kc, ks, kl, 64), plain.values(vc, vs, vl, 64)
+        for h in range(heads):
+            e = h // (heads // kv)
+            off = 2 ** -8 * (q[r:r + n, h].double().abs() @ k[e].abs().t()).amax(1, keepdim=True) * d ** -0.5
+            wide_bound[r:r + n, h * d:(h + 1) * d] += (2 * off + 2 ** -7) * v[e].abs().amax(0)[None]
+    check_attention(got, want, wide_bound)
+    assert int(status) == 0 and not bool(got[row:].any())
+
+
+def test_values_that_are_not_finite_reach_only_the_tokens_that_see_them(ops):
+    g = gen(9)
+    heads, kv, d, n = 4, 2, 128, 100
+    k_rows, v_rows, table, status, k, v, pos, slot = make_cache(ops, g, [n, n], kv, d, 64)
+    v[50, 0, 70] = NAN                                       # sequence 0, position 50, the second group of key/value head 0
+    ops.int4.append(k, v, k_rows, v_rows, table, pos, slot, status)
+    q = randn(g, 4, heads, d).to(torch.bfloat16)
+    at = torch.tensor([49, 50, 99, 99], dtype=torch.int32, device=DEV)
+    of = torch.tensor([0, 0, 0, 1], dtype=torch.int32, device=DEV)
+    for splits in (1, 2):
+        got = ops.int4.attention_decode(q, k_rows, v_rows, table, at, of, 0.1, 0, status, n_splits=splits)
+        bad = torch.isnan(got).reshape(4, heads, 2, 64)
+        want = torch.zeros_like(bad)
+        want[1:3, :2, 1] = True
+        assert torch.equal(bad, want)
+        q2 = q.clone()
+        q2[2, 3, 5] = INF
+        bad = torch.isnan(ops.int4.attention_decode(q2, k_rows, v_rows, table, at, of, 0.1, 0, status, n_splits=splits)).reshape(4, heads, d)
+        assert bool(bad[2, 3].all()) and not bool(bad[3].any()) and not bool(bad[2, 2].any())
+    k[30, 1, 0] = INF                                        # a key of key/value head 1: every later query of its heads
+    ops.int4.append(k, v, k_rows, v_rows, table, pos, slot, status)
+    bad = torch.isnan(ops.int4.attention_decode(q, k_rows, v_rows, table, at, of, 0.1, 0, status)).reshape(4, heads, d)
+    assert bool(bad[:3, 2:].all()) and not bool(bad[3].any()) and not bool(bad[0, :2].any())
