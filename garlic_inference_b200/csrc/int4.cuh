@@ -3,18 +3,14 @@
 // A number q of 0 .. 15 stands for  step * q + low  (both bfloat16, one pair per group of numbers; two numbers lie in a
 // byte, the first in its low half).  A group with a number that is not finite has step = low = NaN.
 //
-// The products run on mma.sync m16n8k32 with 8-bit floating operands.  The bytes 0 .. 15 read as e4m3 are exactly
-// q * 2^-9 (subnormals up to 7, then the first normal numbers with the same spacing), so unpacking is an AND and a
-// shift: three instructions for eight numbers, where a bfloat16 operand takes eleven, and this part's integer
-// pipe runs only two warp instructions a cycle (measured: lop3, prmt and shf 1.98 per cycle and SM).  The other operand, x, is
-// scaled by a power of two so that its largest magnitude lies in [128, 256), and split into two parts of 8 bits:
-//   hi = e4m3(x')  (4 significant bits, rounded to nearest),  lo = e5m2(x' - hi)  (3 significant bits, down to 2^-16).
-// Where hi is a normal number (x' >= 2^-6), what it leaves of a bfloat16 (8 significant bits) is a whole number of -8 .. 8 in
-// units of x's last place, and all of those have at most 3 significant bits: hi + lo is x' exactly, down to 2^-14 of the
-// largest.  Below, hi is within 2^-10 and lo within an eighth of the rest: 2^-14 absolutely, 2^-21 of the largest.  Measured on a
-// B200: the e4m3 form issues 0.89 per cycle and SM against 0.48 for bfloat16 m16n8k16, so even in two parts it does 1.9
-// times as many products; and it sums its 32 exact products and the accumulator before one rounding to nearest float32
-// (checked: 2^25 + 3 is 2^25 + 4, 2^28 + 32 products of 1 is 2^28 + 32).
+// The products run on mma.sync m16n8k16 with f16 operands.  The bits 0 .. 15 of a nibble in a half word are, read as f16, exactly
+// q * 2^-24 (subnormal numbers are evenly spaced), and four bits further up q * 2^-20: a word of eight numbers becomes four operand
+// registers with a shift and four ANDs, no conversion.  (A bfloat16 operand takes a third more and a subtraction on a pipe that
+// issues two warp instructions a cycle and SM; 8-bit operands are turned into f16 by instructions of their own, 0.14 products
+// of k 32 a cycle measured against 0.47 of k 16 in f16 or bfloat16.)  The other operand x is scaled by a power of two
+// so that its largest magnitude lies in [2^14, 2^15), those that meet numbers four bits up by 2^-4 of that, and converted to
+// f16, which has 11 significant bits: exact for a bfloat16 (8 bits) down to 2^-28 of the largest, and within 2^-36 of the
+// largest below.  Products are exact and summed in float32.
 #pragma once
 #include "common.cuh"
 #include <cuda_fp16.h>
@@ -24,50 +20,32 @@
 #define I4_TILE 1088              // bytes of a weight's tile: 16 outputs x 128 inputs, then 16 x (step, low)
 #define I4_TILE_CODES 1024
 
-// c += a b for a 16 x 32 (codes as e4m3) and b 32 x 8, hi parts e4m3 or lo parts e5m2
-__device__ __forceinline__ void i4_mma_hi(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c += a b for a 16 x 16 (codes) and b 16 x 8
+__device__ __forceinline__ void i4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void i4_mma_lo(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e5m2.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t i4_low(uint32_t w) { return w & 0x0F0F0F0Fu; }              // numbers 0, 2, 4, 6 of eight
-__device__ __forceinline__ uint32_t i4_high(uint32_t w) { return (w >> 4) & 0x0F0F0F0Fu; }      // numbers 1, 3, 5, 7
+#define I4_NEAR 0x000F000Fu       // numbers 0 and 4 of a word (shifted by 8: 2 and 6), as q * 2^-24
+#define I4_FAR 0x00F000F0u        // numbers 1 and 5 (3 and 7), as q * 2^-20
+#define I4_UNIT 5.9604644775390625e-08f      // 2^-24
 
 __device__ __forceinline__ uint32_t i4_f16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Two f16 -> their hi parts (two e4m3 in 16 bits) and lo parts (two e5m2)
-__device__ __forceinline__ void i4_split2(uint32_t x, uint32_t& hi, uint32_t& lo) {
-    uint16_t h, l;
-    uint32_t back, rest;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(x));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(rest) : "r"(x), "r"(back));
-    asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(l) : "r"(rest));
-    hi = h;
-    lo = l;
+// Eight scaled numbers as the registers that meet a word's: (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16
+__device__ __forceinline__ uint4 i4_operand(const float (&a)[8]) {
+    return make_uint4(i4_f16x2(a[0], a[4]), i4_f16x2(a[1] * 0.0625f, a[5] * 0.0625f), i4_f16x2(a[2], a[6]),
+                      i4_f16x2(a[3] * 0.0625f, a[7] * 0.0625f));
 }
-// four scaled numbers -> a word of hi parts and a word of lo parts
-__device__ __forceinline__ void i4_split4(float a, float b, float c, float d, uint32_t& hi, uint32_t& lo) {
-    uint32_t h0, l0, h1, l1;
-    i4_split2(i4_f16x2(a, b), h0, l0);
-    i4_split2(i4_f16x2(c, d), h1, l1);
-    hi = __byte_perm(h0, h1, 0x5410);
-    lo = __byte_perm(l0, l1, 0x5410);
+// The power of two that brings a largest magnitude `most` into [2^14, 2^15), and the exponent e of its inverse 2^(e - 14).  Below 2^-112
+// the factor stays at 2^126 (a larger one is no float32).
+__device__ __forceinline__ float i4_factor(float most, int& e) {
+    e = max((int)(__float_as_uint(most) >> 23) - 127, -112);             // floor(log2 most); -127 for zero and subnormals
+    return __uint_as_float((uint32_t)(14 - e + 127) << 23);
 }
-// The power of two that x is multiplied by so that a largest magnitude `most` lands in [128, 256), and its inverse.  Below 2^-119 the
-// factor stays at 2^126 (a larger one is no float32).
-__device__ __forceinline__ float i4_factor(float most, float& inverse) {
-    int e = (int)(__float_as_uint(most) >> 23) - 127;                    // floor(log2 most); -127 for zero and subnormals
-    e = max(e, -119);
-    inverse = __uint_as_float((uint32_t)(e - 7 + 127) << 23);
-    return __uint_as_float((uint32_t)(7 - e + 127) << 23);
-}
+__device__ __forceinline__ float i4_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
 
 __device__ __forceinline__ float i4_bf16_low(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float i4_bf16_high(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }

@@ -5,16 +5,15 @@
 // over the keys j <= position of the query's own sequence (and j > position - window), query head h reading key/value head
 // h / (n_q / n_kv).  Bound by reading the cache once, 0.56 bytes a number: on a B200 that leaves each SM 200 cycles for
 // 32 keys of 128, so unpacking has to be short.  Codes therefore go to the tensor cores as they are (int4.cuh), with keys
-// and output numbers as the 16-wide side of mma.sync m16n8k32 and the queries as its 8 columns:
+// and output numbers as the 16-wide side of mma.sync m16n8k16 and the queries as its 8 columns:
 //
 //   scores^T [16 keys x 8] = codes of K [16 x 64] . q^T,  then  step_j * that + low_j * sum(q),  per group of 64
-//   out^T [16 numbers x 8] += codes of V^T [16 x 32 keys] . (p_j * step_j)^T,   and  sum_j p_j * (low_j + 8 step_j) beside it
+//   out^T [16 numbers x 8] += codes of V^T [16 x 16 keys] . (p_j * step_j)^T,   and  sum_j p_j * low_j beside it
 //
-// q and p_j * step_j go in as two parts of 8 bits each.  q is split exactly (int4.cuh); p_j * step_j keeps 7 to 8 significant
-// bits, as a probability rounded to bfloat16 does.  What its rounding leaves would be multiplied by codes of 7.5 on
-// average; a constant row of 8s among the codes takes it back out, so that only code - 8 sees it.  Everything else is float32.
-// The transposition that the second product needs of V (its 16-wide side runs along a row of the cache) is four-by-four
-// bytes in registers; that of the probabilities is movmatrix on pairs of keys.
+// q goes in exactly (a scaled f16), p_j * step_j rounded to the 11 significant bits of an f16, scaled by a power of two that
+// follows the largest step so far; a probability of 2^-29 of the largest still has all of them.  Everything else is float32.
+// The transposition that the second product needs of V (its 16-wide side runs along a row of the cache) is two byte permutes
+// for two keys' words; that of the probabilities is movmatrix.
 //
 //  * A block is one run of tokens, one key/value head, one block of 8 NT columns (token, query head of the group) and one
 //    slice of the keys.  Its 4 warps take 32 keys each, in turn, through a queue of their own (cp.async, three chunks deep), and
@@ -160,7 +159,7 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
     for (int i = 0; i < I4A_STAGES - 1; ++i) issue();
 
     // ---- the queries as operand fragments: lane (g, t) holds, of column g, numbers 16 t .. 16 t + 15 of every group
-    uint4 qf[NT][2 * G];                                                       // hi of both words, lo of both
+    uint4 qf[NT][2 * G];                                                       // of its two words each
     float qsum[NT][G][2], cscale[NT][2];                                       // of columns 2t, 2t + 1
     int pcol[NT][2];
 #pragma unroll
@@ -180,10 +179,10 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
             }
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        float inverse;
-        const float f = i4_factor(__uint_as_float(min(most, 0x7F7F0000u)), inverse);
-        // codes are multiples of 2^-9 to the tensor cores; a query with a number that is not finite has no scores
-        const float back = most > 0x7F7FFFFFu ? __uint_as_float(0x7FC00000u) : inverse * 512.f * scale_log2;
+        int ex;
+        const float f = i4_factor(__uint_as_float(min(most, 0x7F7F0000u)), ex);
+        // a query with a number that is not finite has no scores
+        const float back = most > 0x7F7FFFFFu ? __uint_as_float(0x7FC00000u) : i4_pow2(ex) * 1024.f * scale_log2;
         float sum[G];
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
@@ -198,9 +197,7 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
                     a[2 * e + 1] = i4_bf16_high(w[e]) * f;
                     sum[gr] += a[2 * e] + a[2 * e + 1];
                 }
-                uint4& o = qf[nt][gr * 2 + h];
-                i4_split4(a[0], a[2], a[4], a[6], o.x, o.z);
-                i4_split4(a[1], a[3], a[5], a[7], o.y, o.w);
+                qf[nt][gr * 2 + h] = i4_operand(a);
             }
             sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
             sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
@@ -209,14 +206,14 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
         for (int e = 0; e < 2; ++e) {
             const int from = (2 * t + e) * 4;                                  // a lane that holds column 2t + e
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) qsum[nt][gr][e] = __shfl_sync(0xffffffffu, sum[gr], from) * 0.001953125f;
+            for (int gr = 0; gr < G; ++gr) qsum[nt][gr][e] = __shfl_sync(0xffffffffu, sum[gr], from) * I4_UNIT;
             cscale[nt][e] = __shfl_sync(0xffffffffu, back, from);
             const int cc = nt * 8 + 2 * t + e;
             pcol[nt][e] = cc < n_cols ? pos0 + (col0 + cc) / group : -1;       // no key is at or before -1
         }
     }
 
-    float o[G * 4][NT][4], eights[G][NT][4], off_sum[NT][G][2], m[NT][2], l[NT][2];
+    float o[G * 4][NT][4], off_sum[NT][G][2], m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -224,17 +221,13 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) eights[gr][nt][e] = 0.f;
-            off_sum[nt][gr][0] = off_sum[nt][gr][1] = 0.f;
-        }
+        for (int gr = 0; gr < G; ++gr) off_sum[nt][gr][0] = off_sum[nt][gr][1] = 0.f;
         m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.f;
     }
-    int vexp[G];                                                               // exponent that the steps of V are scaled by: their largest so far lands in [128, 256)
+    int vexp[G];                                                               // exponent that the steps of V are scaled by: their largest so far lands in [2^14, 2^15)
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) vexp[gr] = -120;
+    for (int gr = 0; gr < G; ++gr) vexp[gr] = -113;
 
     const int perm = (0x57463120 >> (4 * g)) & 7;                              // row g of a tile is this key, row g + 8 eight behind
     const int kv0 = (0x57463120 >> (8 * t)) & 7, kv1 = (0x57463120 >> (8 * t + 4)) & 7;   // rows 2t, 2t + 1
@@ -266,12 +259,12 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
                 const uint2 w1 = *reinterpret_cast<const uint2*>(sK + i4a_piece<D>(r + 8, gr * 2 + (t >> 1)) + (t & 1) * 8);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t a0 = h ? w0.y : w0.x, a1 = h ? w1.y : w1.x;
-                    const uint32_t a[4] = {i4_low(a0), i4_low(a1), i4_high(a0), i4_high(a1)};
+                    const uint32_t a0 = h ? w0.y : w0.x, a1 = h ? w1.y : w1.x, c0 = a0 >> 8, c1 = a1 >> 8;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        i4_mma_hi(z[gr][nt], a, qf[nt][gr * 2 + h].x, qf[nt][gr * 2 + h].y);
-                        i4_mma_lo(z[gr][nt], a, qf[nt][gr * 2 + h].z, qf[nt][gr * 2 + h].w);
+                        const uint4 b = qf[nt][gr * 2 + h];
+                        i4_mma(z[gr][nt], a0 & I4_NEAR, a1 & I4_NEAR, a0 & I4_FAR, a1 & I4_FAR, b.x, b.y);
+                        i4_mma(z[gr][nt], c0 & I4_NEAR, c1 & I4_NEAR, c0 & I4_FAR, c1 & I4_FAR, b.z, b.w);
                     }
                 }
             }
@@ -342,19 +335,19 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t meta = *reinterpret_cast<const uint32_t*>(sVM + (mt * 16 + perm + 8 * half) * G * 4 + gr * 4);
                     vs[gr][mt][half] = i4_bf16_low(meta);
-                    vo[gr][mt][half] = fmaf(8.f, vs[gr][mt][half], i4_bf16_high(meta));
+                    vo[gr][mt][half] = i4_bf16_high(meta);
                     const uint32_t bits = meta << 16;                          // steps are never negative
                     most = max(most, bits < 0x7F800000u ? bits : 0u);
                 }
             most = __reduce_max_sync(0xffffffffu, most);
-            const int e = max((int)(most >> 23) - 127, -119);
+            const int e = max((int)(most >> 23) - 127, -112);
             grow[gr] = 1.f;
             if (e > vexp[gr]) {                                                // the same for the whole warp
-                grow[gr] = vexp[gr] < -119 ? 0.f : i4a_exp2((float)(vexp[gr] - e));      // nothing summed up yet: 0 times 0
+                grow[gr] = vexp[gr] < -112 ? 0.f : i4a_exp2((float)(vexp[gr] - e));      // nothing summed up yet: 0 times 0
                 vexp[gr] = e;
                 moved = true;
             }
-            const float vscale = __uint_as_float((uint32_t)(7 - vexp[gr] + 127) << 23);
+            const float vscale = i4_pow2(14 - vexp[gr]);
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) vs[gr][mt][0] *= vscale, vs[gr][mt][1] *= vscale;
         }
@@ -366,7 +359,6 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float f = corr[nt][e & 1] * grow[gr];
-                        eights[gr][nt][e] *= f;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[gr * 4 + i][nt][e] *= f;
                     }
@@ -377,58 +369,39 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
         // ---- out^T += codes of V^T . (p step)^T
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-            uint32_t bh[NT][2], bl[NT][2];                                     // second operand: hi and lo parts, keys 0-15 and 16-31
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
+            for (int mt = 0; mt < 2; ++mt) {
+                uint32_t b[NT][2];                                             // second operand: keys of rows 0-7 and 8-15
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    uint32_t h[2], w[2];
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float p0 = s[mt][nt][e], p1 = s[mt][nt][e + 2];
-                        float x0 = p0 * vs[gr][mt][0], x1 = p1 * vs[gr][mt][1], f0 = p0 * vo[gr][mt][0], f1 = p1 * vo[gr][mt][1];
+                    for (int half = 0; half < 2; ++half) {
+                        const float p0 = s[mt][nt][half * 2], p1 = s[mt][nt][half * 2 + 1];
+                        float x0 = p0 * vs[gr][mt][half], x1 = p1 * vs[gr][mt][half], f0 = p0 * vo[gr][mt][half], f1 = p1 * vo[gr][mt][half];
                         if (edge) {                                            // a value that is not finite does not reach the columns that do not see it
                             if (p0 == 0.f) x0 = f0 = 0.f;
                             if (p1 == 0.f) x1 = f1 = 0.f;
                         }
-                        off_sum[nt][gr][e] += f0 + f1;
-                        i4_split2(i4_f16x2(x0, x1), h[e], w[e]);
+                        off_sum[nt][gr][0] += f0;
+                        off_sum[nt][gr][1] += f1;
+                        b[nt][half] = i4a_transpose(i4_f16x2(x0, x1));
                     }
-                    bh[nt][mt] = i4a_transpose(__byte_perm(h[0], h[1], 0x5410));
-                    bl[nt][mt] = i4a_transpose(__byte_perm(w[0], w[1], 0x5410));
-                }
-            const uint32_t a8[4] = {0x08080808u, 0x08080808u, 0x08080808u, 0x08080808u};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                i4_mma_hi(eights[gr][nt], a8, bh[nt][0], bh[nt][1]);
-                i4_mma_lo(eights[gr][nt], a8, bl[nt][0], bl[nt][1]);
-            }
-            // word of numbers 8 g .. 8 g + 7 of the keys that this lane's bytes of the first operand are: rows 2t, 2t + 8, 2t + 1, 2t + 9
-            uint32_t w[2][4];
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
+                // words of numbers 8 g .. 8 g + 7 of the keys of rows 2t, 2t + 1, 2t + 8, 2t + 9
+                uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int r = mt * 16 + (i >> 1 ? kv1 : kv0) + (i & 1) * 8;
-                    w[mt][i] = *reinterpret_cast<const uint32_t*>(sV + i4a_piece<D>(r, gr * 2 + (g >> 2)) + (g & 3) * 4);
+                    const int r = mt * 16 + (i & 1 ? kv1 : kv0) + (i >> 1) * 8;
+                    w[i] = *reinterpret_cast<const uint32_t*>(sV + i4a_piece<D>(r, gr * 2 + (g >> 2)) + (g & 3) * 4);
                 }
-            uint32_t by[2][4];                                                 // byte i of the four keys: numbers 8 g + 2 i and 2 i + 1
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const uint32_t x01 = __byte_perm(w[mt][0], w[mt][1], 0x5140), y01 = __byte_perm(w[mt][0], w[mt][1], 0x7362);
-                const uint32_t x23 = __byte_perm(w[mt][2], w[mt][3], 0x5140), y23 = __byte_perm(w[mt][2], w[mt][3], 0x7362);
-                by[mt][0] = __byte_perm(x01, x23, 0x5410);
-                by[mt][1] = __byte_perm(x01, x23, 0x7632);
-                by[mt][2] = __byte_perm(y01, y23, 0x5410);
-                by[mt][3] = __byte_perm(y01, y23, 0x7632);
-            }
+                for (int h = 0; h < 2; ++h) {                                  // numbers 0-3 of the eight, then 4-7, of two keys each
+                    const uint32_t a = __byte_perm(w[0], w[1], h ? 0x7632 : 0x5410), c = __byte_perm(w[2], w[3], h ? 0x7632 : 0x5410);
+                    const uint32_t a8 = a >> 8, c8 = c >> 8;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a[4] = {i4_low(by[0][i]), i4_high(by[0][i]), i4_low(by[1][i]), i4_high(by[1][i])};
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    i4_mma_hi(o[gr * 4 + i][nt], a, bh[nt][0], bh[nt][1]);
-                    i4_mma_lo(o[gr * 4 + i][nt], a, bl[nt][0], bl[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        i4_mma(o[gr * 4 + 2 * h][nt], a & I4_NEAR, a & I4_FAR, c & I4_NEAR, c & I4_FAR, b[nt][0], b[nt][1]);
+                        i4_mma(o[gr * 4 + 2 * h + 1][nt], a8 & I4_NEAR, a8 & I4_FAR, c8 & I4_NEAR, c8 & I4_FAR, b[nt][0], b[nt][1]);
+                    }
                 }
             }
         }
@@ -455,14 +428,13 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
                 float f = off_sum[nt][gr][e];
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) f += __shfl_xor_sync(0xffffffffu, f, x);
-                // 2^(vexp - 7) for the steps' scale, 2^9 for the codes'
-                const float back = vexp[gr] < -119 ? 0.f : __uint_as_float((uint32_t)(vexp[gr] + 127) << 23);
-                const float eight = eights[gr][nt][e];
+                // 2^(vexp - 14) for the steps' scale, 2^24 for the codes', in two factors of which neither overflows
+                const float back = vexp[gr] < -112 ? 0.f : i4_pow2(vexp[gr]);
                 float* dst = so + (warp * COLS + cc) * LD + gr * 64 + 8 * g;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    dst[2 * i] = fmaf((o[gr * 4 + i][nt][e] - eight) * 4.f, back, f);
-                    dst[2 * i + 1] = fmaf((o[gr * 4 + i][nt][e + 2] - eight) * 4.f, back, f);
+                for (int i = 0; i < 4; ++i) {                                  // numbers four bits up count 16 times
+                    dst[2 * i] = fmaf(o[gr * 4 + i][nt][e] * 1024.f, back, f);
+                    dst[2 * i + 1] = fmaf(o[gr * 4 + i][nt][e + 2] * 64.f, back, f);
                 }
             }
             if (g == 0) {

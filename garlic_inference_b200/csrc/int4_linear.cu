@@ -2,8 +2,8 @@
 //
 //   y[m, n] = sum over groups g of 128 inputs:  step[n, g] * sum_k q[n, k] x[m, k]  +  low[n, g] * sum_k x[m, k]
 //
-// bound by reading W once, 0.53 bytes a number.  16 outputs are the 16 rows of mma.sync m16n8k32, rows of x its 8 columns; the
-// sums over q run on the tensor cores in two parts of x (int4.cuh), step and low join in float32 once per group.
+// bound by reading W once, 0.53 bytes a number.  16 outputs are the 16 rows of mma.sync m16n8k16, rows of x its 8 columns; the
+// sums over q run on the tensor cores with the codes as they are (int4.cuh), step and low join in float32 once per group.
 //
 //  * K is cut over the CTAs of a cluster.  A CTA turns its slice of x into operand fragments in shared memory once (scaled
 //    by a power of two per row and slice) and streams its slice of rows of tiles: each of 8 warps takes a row of tiles (with a
@@ -11,9 +11,9 @@
 //  * The 1,088 bytes of a tile come with cp.async into slots that only this warp reads, a few tiles in flight, so warps never
 //    wait for each other while they stream.  W is nobody's output: the first tiles are on their way before the
 //    kernel waits for the one that makes x.
-//  * Behind a row of tiles the cluster's partial sums meet in distributed shared memory, in rank order (the same bits from
-//    run to run), while the next one streams: two buffers, one cluster barrier per row of tiles, arrived at before
-//    and waited for behind the next row's products.
+//  * Behind a row of tiles every block sends its sums to the block of the cluster that finishes them (16-byte stores into
+//    its shared memory), which adds them in rank order (the same bits from run to run) while the next row streams: two buffers, one
+//    cluster barrier per row of tiles, arrived at behind the stores and waited for behind the next row's products.
 #include "int4.cuh"
 #include "glu.cuh"
 #include <cooperative_groups.h>
@@ -22,7 +22,7 @@ namespace cg = cooperative_groups;
 
 #define I4L_WARPS 8
 #define I4L_THREADS (I4L_WARPS * 32)
-#define I4L_PART 160               // floats of a 16 x 8 block of sums: 8 rows of x, 20 apart (no bank conflicts)
+#define I4L_ODD 0x79800000u        // bits of 2^116: sums of rows with such numbers are not scaled back in float32
 
 __device__ __forceinline__ void i4l_cp16(void* smem, const void* gmem) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(gmem) : "memory");
@@ -49,11 +49,16 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
                    int M, int N, int K, int groups, int slice, int units, int vec, GluShape unit, long long ld_out) {
     static_assert(!GLU || RT == 2, "a gate and its up");
     gi_pdl_launch_dependents();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");       // waited for before the first store into another block
     constexpr int DEPTH = SLOTS / RT;                                // steps (RT tiles of one group) in flight
     extern __shared__ __align__(16) unsigned char i4_smem[];
     unsigned char* ring = i4_smem;                                       // [8 warps][slots][1088]
-    float* part = reinterpret_cast<float*>(ring + I4L_WARPS * SLOTS * I4_TILE);      // [2][8 warps][RT][NT][160]
-    unsigned char* frag = reinterpret_cast<unsigned char*>(part + 2 * I4L_WARPS * RT * NT * I4L_PART);   // [slice][NT][4][32][16]
+    // sums that this block finishes, as the lanes of a warp hold them: [2][unit of the pass][block that sends][RT][NT][32][4]; unit of
+    // warp w belongs to block w mod ranks, as its (w / ranks)-th
+    float4* sums = reinterpret_cast<float4*>(ring + I4L_WARPS * SLOTS * I4_TILE);
+    const int owned = (I4L_WARPS + (int)cg::this_cluster().num_blocks() - 1) / (int)cg::this_cluster().num_blocks();
+    const int half = owned * (int)cg::this_cluster().num_blocks() * RT * NT * 32;        // of one buffer, in float4
+    unsigned char* frag = reinterpret_cast<unsigned char*>(sums + 2 * half);             // [slice][NT][4][32][16]
     float* xsum = reinterpret_cast<float*>(frag + (size_t)slice * NT * 2048);            // [slice][8 NT]
     __shared__ uint32_t s_most[8 * NT];                                  // bits of the largest magnitude of each row of x
     __shared__ uint32_t s_odd;                                           // rows with numbers too large to scale, or not finite
@@ -119,10 +124,10 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
     __syncthreads();
     for (int i = warp; i < G * NT; i += I4L_WARPS) {
         const int gi = i / NT, nt = i % NT, m = nt * 8 + g, k0 = (g0 + gi) * I4_GROUP_W + t * 32;
-        float inverse;
+        int e;
         const uint32_t most = m < M ? s_most[m] : 0;
-        const bool odd = most >= 0x7B800000u;                            // 2^120 and more, infinite or NaN: summed the long way
-        const float f = odd ? 0.f : i4_factor(__uint_as_float(most), inverse);
+        const bool odd = most >= I4L_ODD;                                // 2^116 and more, infinite or NaN: summed the long way
+        const float f = odd ? 0.f : i4_factor(__uint_as_float(most), e);
         if (odd && t == 0) atomicOr(&s_odd, 1u << m);
         uint4* dst = reinterpret_cast<uint4*>(frag + (size_t)(gi * NT + nt) * 2048) + lane;
         float sum = 0.f;
@@ -133,55 +138,63 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
             float a[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                a[2 * e] = i4_bf16_low(w[e]) * f;
-                a[2 * e + 1] = i4_bf16_high(w[e]) * f;
+            for (int h = 0; h < 4; ++h) {
+                a[2 * h] = i4_bf16_low(w[h]) * f;
+                a[2 * h + 1] = i4_bf16_high(w[h]) * f;
             }
-            uint4 o;
-            i4_split4(a[0], a[2], a[4], a[6], o.x, o.z);
-            i4_split4(a[1], a[3], a[5], a[7], o.y, o.w);
-            dst[j * 32] = o;                                             // hi of both, lo of both
+            dst[j * 32] = i4_operand(a);
             sum += ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (t == 0) xsum[gi * 8 * NT + m] = sum * 0.001953125f;          // in units of 512 as the products of codes are
+        if (t == 0) xsum[gi * 8 * NT + m] = sum * I4_UNIT;               // as the products with codes are
     }
     __syncthreads();
     const uint32_t odd_rows = s_odd;
-    float back[NT][2];                                                   // what brings the sums of rows 2t, 2t + 1 back: 512 / factor
+    float back[NT][2];                                                   // what brings the sums of rows 2t, 2t + 1 back
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float inverse;
-            i4_factor(__uint_as_float(min(s_most[nt * 8 + 2 * t + e], 0x7B7F0000u)), inverse);
-            back[nt][e] = inverse * 512.f;
+        for (int h = 0; h < 2; ++h) {
+            int e;
+            i4_factor(__uint_as_float(min(s_most[nt * 8 + 2 * t + h], I4L_ODD - 1)), e);
+            back[nt][h] = i4_pow2(e - 14 + 24);
         }
 
-    // ---- the sums of a finished pass: every CTA of the cluster writes a share of them
+    // ---- the sums of a finished pass that this block finishes: a warp per unit and block of 8 rows of x
     auto finish = [&](int p) {
-        const float* mine = part + (p & 1) * I4L_WARPS * RT * NT * I4L_PART;
-        constexpr int ROWS = GLU ? 1 : RT;                               // results per pair of (warp, 16 outputs)
-        constexpr int TOTAL = I4L_WARPS * ROWS * NT * 128;
-        const int share = (TOTAL + ranks - 1) / ranks;
-        const int end = min(TOTAL, (rank + 1) * share);
-        for (int i = rank * share + threadIdx.x; i < end; i += I4L_THREADS) {
-            const int r = i & 15, m8 = (i >> 4) & 7, nt = (i >> 7) % NT, wr = (i >> 7) / NT;
-            const int w = wr / ROWS, rt = wr % ROWS, m = nt * 8 + m8;
-            const int u = (p * I4L_WARPS + w) * n_cl + cl;
-            const int n = (GLU ? u : u * RT + rt) * 16 + r;
-            if (u >= units || m >= M || n >= (GLU ? N / 2 : N)) continue;
-            const int at = ((w * RT + rt) * NT + nt) * I4L_PART + m8 * 20 + r;
-            float v = 0.f, up = 0.f;
-            for (int c = 0; c < ranks; ++c) {
-                const float* src = ranks > 1 ? cluster.map_shared_rank(mine, c) : mine;
-                v += src[at];
-                if (GLU) up += src[at + NT * I4L_PART];
+        for (int i = warp; i < owned * NT; i += I4L_WARPS) {
+            const int nt = i % NT, w = (i / NT) * ranks + rank, u = (p * I4L_WARPS + w) * n_cl + cl;
+            if (w >= I4L_WARPS || u >= units) continue;
+            const float4* src = sums + (p & 1) * half + (size_t)(i / NT) * ranks * RT * NT * 32 + lane;
+            float4 v[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int c = 0; c < ranks; ++c) {
+                    const float4 a = src[((c * RT + r) * NT + nt) * 32];
+                    v[r].x += a.x, v[r].y += a.y, v[r].z += a.z, v[r].w += a.w;
+                }
             }
-            if (GLU) v = glu_unit(v, up, unit);
-            if (out_f32) reinterpret_cast<float*>(out)[(size_t)m * ld_out + n] = v;
-            else reinterpret_cast<bf16*>(out)[(size_t)m * ld_out + n] = __float2bfloat16_rn(v);
+            auto put = [&](int m, int n, float value) {
+                if (m >= M || n >= (GLU ? N / 2 : N)) return;
+                if (out_f32) reinterpret_cast<float*>(out)[(size_t)m * ld_out + n] = value;
+                else reinterpret_cast<bf16*>(out)[(size_t)m * ld_out + n] = __float2bfloat16_rn(value);
+            };
+            const int m = nt * 8 + 2 * t;
+            if (GLU) {
+                const int n = u * 16 + g;
+                put(m, n, glu_unit(v[0].x, v[RT - 1].x, unit));
+                put(m + 1, n, glu_unit(v[0].y, v[RT - 1].y, unit));
+                put(m, n + 8, glu_unit(v[0].z, v[RT - 1].z, unit));
+                put(m + 1, n + 8, glu_unit(v[0].w, v[RT - 1].w, unit));
+            } else {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const int n = (u * RT + r) * 16 + g;
+                    put(m, n, v[r].x), put(m + 1, n, v[r].y), put(m, n + 8, v[r].z), put(m + 1, n + 8, v[r].w);
+                }
+            }
         }
     };
 
@@ -211,13 +224,13 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
                     mg8[r] = *reinterpret_cast<const uint32_t*>(tile + 1024 + g * 4 + 32);
                 }
                 slot = slot + 1 == DEPTH ? 0 : slot + 1;
-                float z[RT][NT][4];
+                float z[RT][NT][4], zl[RT][NT][4];                       // two chains of products
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) z[r][nt][e] = 0.f;
+                        for (int e = 0; e < 4; ++e) z[r][nt][e] = zl[r][nt][e] = 0.f;
                 const uint4* fr = reinterpret_cast<const uint4*>(frag + (size_t)gi * NT * 2048) + lane;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -228,11 +241,11 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
                     for (int r = 0; r < RT; ++r) {
                         const uint32_t w0 = j == 0 ? c[r][0].x : j == 1 ? c[r][0].y : j == 2 ? c[r][0].z : c[r][0].w;
                         const uint32_t w1 = j == 0 ? c[r][1].x : j == 1 ? c[r][1].y : j == 2 ? c[r][1].z : c[r][1].w;
-                        const uint32_t a[4] = {i4_low(w0), i4_low(w1), i4_high(w0), i4_high(w1)};
+                        const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            i4_mma_hi(z[r][nt], a, b[nt].x, b[nt].y);
-                            i4_mma_lo(z[r][nt], a, b[nt].z, b[nt].w);
+                            i4_mma(z[r][nt], w0 & I4_NEAR, w1 & I4_NEAR, w0 & I4_FAR, w1 & I4_FAR, b[nt].x, b[nt].y);
+                            i4_mma(zl[r][nt], v0 & I4_NEAR, v1 & I4_NEAR, v0 & I4_FAR, v1 & I4_FAR, b[nt].z, b[nt].w);
                         }
                     }
                 }
@@ -243,10 +256,10 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
                     for (int r = 0; r < RT; ++r) {
                         const float s = i4_bf16_low(mg[r]), s8 = i4_bf16_low(mg8[r]);
                         const float l = i4_bf16_high(mg[r]), l8 = i4_bf16_high(mg8[r]);
-                        y[r][nt][0] = fmaf(l, xs.x, fmaf(s, z[r][nt][0], y[r][nt][0]));
-                        y[r][nt][1] = fmaf(l, xs.y, fmaf(s, z[r][nt][1], y[r][nt][1]));
-                        y[r][nt][2] = fmaf(l8, xs.x, fmaf(s8, z[r][nt][2], y[r][nt][2]));
-                        y[r][nt][3] = fmaf(l8, xs.y, fmaf(s8, z[r][nt][3], y[r][nt][3]));
+                        y[r][nt][0] = fmaf(l, xs.x, fmaf(s, z[r][nt][0] + zl[r][nt][0], y[r][nt][0]));
+                        y[r][nt][1] = fmaf(l, xs.y, fmaf(s, z[r][nt][1] + zl[r][nt][1], y[r][nt][1]));
+                        y[r][nt][2] = fmaf(l8, xs.x, fmaf(s8, z[r][nt][2] + zl[r][nt][2], y[r][nt][2]));
+                        y[r][nt][3] = fmaf(l8, xs.y, fmaf(s8, z[r][nt][3] + zl[r][nt][3], y[r][nt][3]));
                     }
                 }
             }
@@ -285,26 +298,21 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
                 }
             }
         }
-        if (p > 0) {                                                     // the sums of the pass before are complete
-            asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-            finish(p - 1);                                               // and so every peer is done with those of pass p - 2
-        }
+        asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        if (p > 0) finish(p - 1);                                        // its sums are complete, and those of pass p - 2 done with
         if (u < units) {
-            float* dst = part + ((p & 1) * I4L_WARPS + warp) * RT * NT * I4L_PART;
+            float4* dst = cluster.map_shared_rank(sums, warp % ranks) + (p & 1) * half + ((size_t)(warp / ranks) * ranks + rank) * RT * NT * 32 + lane;
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        dst[(r * NT + nt) * I4L_PART + (2 * t + (e & 1)) * 20 + g + 8 * (e >> 1)] = y[r][nt][e];
+                    dst[(r * NT + nt) * 32] = make_float4(y[r][nt][0], y[r][nt][1], y[r][nt][2], y[r][nt][3]);
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
     }
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     finish(passes - 1);
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-    if (ranks > 1) cluster.sync();                                       // nobody leaves while a peer still reads its sums
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -337,7 +345,7 @@ static int launch_int4_linear(const bf16* x, const unsigned char* tiles, void* o
     const int groups = (K - 1) / I4_GROUP_W + 1;
     const int slice = (groups + ranks - 1) / ranks;
     const int row_tiles = (N + 15) / 16, units = GLU ? row_tiles / 2 : (row_tiles + RT - 1) / RT;
-    const size_t smem = (size_t)I4L_WARPS * SLOTS * I4_TILE + 2ull * I4L_WARPS * RT * NT * I4L_PART * 4 +
+    const size_t smem = (size_t)I4L_WARPS * SLOTS * I4_TILE + 2ull * ((I4L_WARPS + ranks - 1) / ranks) * ranks * RT * NT * 512 +
                         (size_t)slice * NT * 2048 + (size_t)slice * 8 * NT * 4;
     GI_REQUIRE(smem <= 226 * 1024, "gi_int4_linear: %d inputs are too many for %d rows", K, M);
     auto kernel = int4_linear_kernel<NT, RT, GLU, SLOTS>;

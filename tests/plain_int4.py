@@ -79,11 +79,11 @@ def attention(q, k_rows, v_rows, table, spans, scale, window):
 
     Returns (result [n, n_q * d], the bound).  The bound counts, per number of the result:
       2^-8 of it for its own rounding to bfloat16;
-      2^-7 + 2^-10 of sum p step |code - 8| / sum p for the two parts of p step: the first keeps 4 significant bits, so at most
-      2^-4 of it is left, and the second 3 significant bits of that, off by an eighth; rounding to f16 first;
-      2^-21 of the largest step times 8, per key, over sum p, where p step is so small that the first part is subnormal;
-      and scores: 24 roundings of float32 (2^-24) in sums whose numbers add up to A = sum step code |q| + |low| |q|, what the
-      parts of q leave (2^-21 of the largest |q| times sum step code), exp2 within 2^-22 of itself, all of which a
+      2^-11 of sum p step code / sum p: p step is rounded to f16;
+      float32 sums over the keys, 16 at a time, of numbers that add up to sum p (step code + |low|) / sum p: 2^-23 of that for
+      every 16 keys and 64 more for the ends;
+      and scores: 24 roundings of float32 (2^-24) in sums whose numbers add up to A = sum step code |q| + |low| |q|, what an f16
+      leaves of q (2^-36 of the largest |q| times sum step code), exp2 within 2^-22 of itself, all of which a
       probability sees once, and the result twice (in its sum and in what it is divided by)."""
     n, n_q, d = q.shape
     out = torch.zeros(n, n_q * d, dtype=torch.float64, device=q.device)
@@ -94,7 +94,7 @@ def attention(q, k_rows, v_rows, table, spans, scale, window):
         kc, ks, kl = sequence(k_rows, table[slot], past + count)
         vc, vs, vl = sequence(v_rows, table[slot], past + count)
         k, v = values(kc, ks, kl, 64), values(vc, vs, vl, 64)
-        spread = values((vc - 8).abs(), vs, torch.zeros_like(vl), 64)
+        spread = values(vc, vs, torch.zeros_like(vl), 64)
         heads = k.shape[0]
         i, j = torch.arange(past, past + count, device=q.device)[:, None], torch.arange(past + count, device=q.device)[None]
         hidden = (j > i) | ((j <= i - window) if window else torch.zeros_like(j > i))
@@ -116,10 +116,10 @@ def attention(q, k_rows, v_rows, table, spans, scale, window):
             kq = values(kc[e], ks[e], torch.zeros_like(kl[e]), 64)
             a = (x.abs() @ (kq + (k[e] - kq).abs()).t()).masked_fill(hidden, 0.0) * scale
             most = x.abs().amax(1, keepdim=True)
-            off = 24 * 2 ** -24 * 1.4427 * a + 2 ** -21 * most * (kq.sum(1)[None] * scale) + 2 ** -22 + 2 ** -23 * s.masked_fill(hidden, 0.0).abs()
+            off = 24 * 2 ** -24 * 1.4427 * a + 2 ** -36 * most * (kq.sum(1)[None] * scale) + 2 ** -22 + 2 ** -23 * s.masked_fill(hidden, 0.0).abs()
             off = (off * (p > 0)).amax(1, keepdim=True)
-            sv = seen(v[e])
-            size = ((p / total) @ sv.abs())
-            bound[row:row + count, cols] = 2 ** -8 * o.abs() + (2 ** -7 + 2 ** -10) * (p / total) @ seen(spread[e]) \
-                + 2 ** -21 * 8 * seen(vs[e]).amax() * (~hidden).sum(1, keepdim=True) / total + 2 * off * size + 2 ** -20 * size
+            size = (p / total) @ seen(v[e].abs())
+            parts = (p / total) @ seen(spread[e] + (v[e] - spread[e]).abs())
+            bound[row:row + count, cols] = 2 ** -8 * o.abs() + 2 ** -11 * (p / total) @ seen(spread[e]) + 2 * off * size \
+                + ((past + count) / 16 + 64) * 2 ** -23 * parts
     return out, bound

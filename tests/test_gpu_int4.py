@@ -63,13 +63,13 @@ def test_weights_whose_numbers_are_not_finite(ops):
 
 def linear_bound(x, w):
     """How far the kernel that reads codes may be off: the result's rounding is the caller's.  Float32 roundings of sums whose numbers
-    add up to A = sum step code |x| + |low| |x|: 8 in a group, 2 a group, 8 blocks and 16 of the ends; and what the two parts
-    of x leave, 2^-21 of the row's largest number."""
+    add up to A = sum step code |x| + |low| |x|: 8 in a group, 2 a group, 8 blocks and 16 of the ends; and what f16 leaves of
+    a scaled x, 2^-36 of the row's largest number."""
     codes, step, low = plain.unpack_weight(w)
     zero = torch.zeros_like(low)
     sq, lo = plain.values(codes, step, zero, 128), plain.values(torch.zeros_like(codes), zero, low.abs(), 128)
     a = x.double().abs() @ (sq + lo).t()
-    return (32 + 2 * step.shape[1]) * 2 ** -24 * a + 2 ** -21 * x.double().abs().amax(1, keepdim=True) * sq.sum(1)[None]
+    return (32 + 2 * step.shape[1]) * 2 ** -24 * a + 2 ** -36 * x.double().abs().amax(1, keepdim=True) * sq.sum(1)[None]
 
 
 def random_weight(ops, g, n, k):
