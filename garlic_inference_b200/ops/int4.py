@@ -127,10 +127,10 @@ def dequantize_weight(w: Int4Weight, dtype: torch.dtype = torch.bfloat16, first:
 
 
 def linear_rows(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.bfloat16, unit: Optional[tuple] = None,
-                out: Optional[torch.Tensor] = None, ranks: int = 0) -> torch.Tensor:
+                out: Optional[torch.Tensor] = None, ranks: int = 0, parts: int = 0) -> torch.Tensor:
     """x W^T for 1 to 16 rows of bfloat16 x, reading the weight's codes once; with `unit` (a `kernels.glu_shape` tuple) the gated
     unit of the weight's first half of outputs (a multiple of 16) and its last.  `out` may be columns of a wider matrix.
-    `ranks`: blocks that share the inputs (0: chosen by the entry point)."""
+    `ranks`, `parts`: blocks that share the inputs, and parts of a block's share that its warps take (0: chosen by the entry point)."""
     l = require_gpu()
     _dense(x, "x", torch.bfloat16), _on_gpu(w.tiles, "w")
     if x.dim() != 2 or x.shape[1] != w.k:
@@ -143,7 +143,7 @@ def linear_rows(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.b
         raise KernelError(f"out {tuple(out.shape)} for a result of {(m, n)}")
     ld = out.stride(0) if m > 1 else max(n, out.stride(0))
     check(l.gi_int4_linear(_ptr(x), _ptr(w.tiles), _ptr(out), code(out_dtype), ld, m, w.n, w.k, int(unit is not None),
-                           *(unit or (0, 1.0, float("inf"), float("inf"), 0.0)), int(ranks), _stream()), l)
+                           *(unit or (0, 1.0, float("inf"), float("inf"), 0.0)), int(ranks), int(parts), _ptr(kernels.tcgen05_error_flag(x.device)), _stream()), l)
     return out
 
 

@@ -114,7 +114,8 @@ _SIGNATURES = {
     "gi_sample_uniform_from_hash": ([c_ulonglong], F),
     "gi_int4_quantize_weight": ([P, I, L, P, I, I, P], I),
     "gi_int4_dequantize_weight": ([P, P, I, I, I, I, I, P], I),
-    "gi_int4_linear": ([P, P, P, I, L, I, I, I, I, I, F, F, F, F, I, P], I),
+    "gi_int4_linear": ([P, P, P, I, L, I, I, I, I, I, F, F, F, F, I, I, P, P], I),
+    "gi_int4_linear_takes": ([I, I, I, I], I),
     "gi_int4_append": ([P, L, L, P, L, L, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, P], I),
     "gi_int4_read": ([P, P, P, I, P, P, P, I, I, I, I, I, I, I, P, P], I),
     "gi_int4_gather": ([P, P, P, P, P, P, P, P, I, P, I, I, I, I, I, I, I, P, P], I),

@@ -99,14 +99,18 @@ def test_linear(ops, m, n, k, out_dtype):
     assert torch.equal(got, ops.linear(x, w, out_dtype))
 
 
+@pytest.mark.parametrize("m,n,k", [(7, 1500, 1152), (16, 300, 700), (8, 20000, 640)])
 @pytest.mark.parametrize("ranks", range(1, 9))
-def test_linear_with_any_number_of_blocks_to_share_the_inputs(ops, ranks):
-    g = gen(ranks)
-    w = random_weight(ops, g, 1500, 1152)                    # 9 groups: uneven shares, and none for some
-    x = randn(g, 7, 1152).to(torch.bfloat16)
+def test_linear_cut_in_any_way(ops, ranks, m, n, k):
+    g = gen(ranks + n)
+    w = random_weight(ops, g, n, k)                          # 9, 6 and 5 groups: uneven shares, and none for some
+    x = randn(g, m, k).to(torch.bfloat16)
     want = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
-    got = ops.int4.linear_rows(x, w, torch.float32, ranks=ranks)
-    assert float(((got.double() - want).abs() / (linear_bound(x, w) + 2 ** -24 * want.abs())).max()) <= 1
+    for parts in (1, 2, 4, 8, 16) if ranks <= -(-k // 128) else []:
+        if parts > -(-(-(-k // 128)) // ranks):
+            continue
+        got = ops.int4.linear_rows(x, w, torch.float32, ranks=ranks, parts=parts)
+        assert float(((got.double() - want).abs() / (linear_bound(x, w) + 2 ** -24 * want.abs())).max()) <= 1
 
 
 @pytest.mark.parametrize("m", [1, 7, 16, 33])
