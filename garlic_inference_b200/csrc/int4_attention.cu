@@ -11,15 +11,16 @@
 //   out^T [16 numbers x 8] += codes of V^T [16 x 16 keys] . (p_j * step_j)^T,   and  sum_j p_j * low_j beside it
 //
 // q goes in exactly (a scaled f16), p_j * step_j rounded to the 11 significant bits of an f16, scaled by a power of two that
-// follows the largest step so far; a probability of 2^-29 of the largest still has all of them.  Everything else is float32.
-// The transposition that the second product needs of V (its 16-wide side runs along a row of the cache) is two byte permutes
-// for two keys' words; that of the probabilities is movmatrix.
+// follows the largest step so far; a probability of 2^-20 of the largest still has all of them.  Everything else is float32.
+// The transposition that the second product needs of V (its 16-wide side runs along a row of the cache) is ldmatrix's, on half words of
+// four numbers; that of the probabilities is movmatrix.
 //
 //  * A block is one run of tokens, one key/value head, one block of 8 NT columns (token, query head of the group) and one
-//    slice of the keys.  Its 4 warps take 32 keys each, in turn, through a queue of their own (cp.async, three chunks deep), and
+//    slice of the keys.  Its 4 warps take 32 keys each, in turn, through a queue of their own (cp.async, three chunks deep), 16 at a time, and
 //    are merged in shared memory at the end; slices are merged by gi_attention_decode_combine, or there is one only.
-//  * In a chunk, row r of the 16 x 32 tile is key perm(r), so that the reads of K (8 rows x 4 pieces of 8 bytes) and of V (4 rows x 8 words)
-//    touch every bank once.
+//  * The reference of the softmax is moved only when a score lies 2^8 above it, and the scale of the steps only when one outgrows it:
+//    one vote a step instead of reductions and products over all sums.
+//  * What runs once a block is kept small and rolled up: such instructions come from the instruction cache's next level at about 20 cycles each.
 #include "int4.cuh"
 
 #include <type_traits>
@@ -64,26 +65,35 @@ template <int D> struct Int4Chunk {
     static constexpr int BYTES = 2 * (CODES + META);
     static constexpr int PIECES = ROW / 16;                              // 16-byte pieces of a row
 };
-// Where piece c of row r lies in a chunk: with rows of 64 bytes the pieces of every other pair of rows change places, so that four
-// rows whose numbers differ mod 4 cover all banks with any one group
+// Where piece c of row r lies in a chunk: eight rows' pieces of one number cover all banks
 template <int D> __device__ __forceinline__ int i4a_piece(int r, int c) {
-    return r * Int4Chunk<D>::ROW + (D == 128 ? c ^ (((r >> 1) & 1) << 1) : c) * 16;
+    return r * Int4Chunk<D>::ROW + (D == 128 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1)) * 16;
 }
+// Four 8 x 8 matrices of half words, as they are or transposed; a lane gives the address of a row of 16 bytes
+__device__ __forceinline__ void i4a_matrix(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void i4a_matrix_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+#define I4A_SLACK 8.f              // a score may lie this far (in powers of two) above the reference
+#define I4A_STEP_TOP 6             // the largest step so far is scaled to [2^6, 2^7): times 2^8 it stays below f16's largest number
 
 // runs[i] = {slot, first row, rows, position of the first row}; without runs, run i is the single token i.
 template <int D, int NT>
-__global__ void __launch_bounds__(I4A_THREADS, NT == 1 ? 4 : 2)
+__global__ void __launch_bounds__(I4A_THREADS, NT == 1 ? 4 : 3)
 int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __restrict__ table, const int4* __restrict__ runs,
                       const int* __restrict__ tok_pos, const int* __restrict__ tok_slot, bf16* __restrict__ out,
                       float* __restrict__ part_o, float* __restrict__ part_ml, int n_q, int n_kv, int n_slots, int max_pages,
-                      int page_size, int n_pages, int window, float scale_log2, int n_splits, int col_tiles, int* __restrict__ status) {
+                      int page_size, int n_pages, int window, float scale_log2, int n_splits, int group, int whole, int* __restrict__ status) {
     typedef Int4Chunk<D> C;
     constexpr int G = C::G, COLS = 8 * NT;
-    gi_pdl_start();
     extern __shared__ __align__(16) unsigned char i4a_smem[];
+    __shared__ uint4 s_frag[NT * 2 * G * 32];                                  // the queries as operand fragments: [column block][group, word][lane]
+    __shared__ float s_back[COLS], s_sum[G][COLS];                             // what brings a column's scores back; its sums per group
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % n_splits, ct = blockIdx.x / n_splits, kvh = blockIdx.y, run = blockIdx.z;
-    const int group = n_q / n_kv;
+    const int split = blockIdx.x % n_splits, col0 = blockIdx.x / n_splits * COLS, kvh = blockIdx.y, run = blockIdx.z;
+    gi_pdl_start();
 
     int slot, row0, rows, pos0;
     if (runs) {
@@ -92,13 +102,14 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
     } else {
         slot = tok_slot[run], row0 = run, rows = 1, pos0 = tok_pos[run];
     }
-    const int col0 = ct * COLS, n_cols = min(rows * group - col0, COLS);       // columns of this block: (token, head of the group)
+    const int n_cols = min(rows * group - col0, COLS);                         // columns of this block: (token, head of the group)
     if (n_cols <= 0) return;
+    auto token_of = [&](int c) { return rows == 1 ? 0 : (col0 + c) / group; };
     auto result_row = [&](int c) {                                             // row of the result that column c is: (token, query head)
-        const int col = col0 + c;
-        return (size_t)(row0 + col / group) * n_q + kvh * group + col % group;
+        const int tok = token_of(c);
+        return (size_t)(row0 + tok) * n_q + kvh * group + (col0 + c - tok * group);
     };
-    const int first = pos0 + col0 / group, hi = pos0 + (col0 + n_cols - 1) / group;       // positions of the block's tokens
+    const int first = pos0 + token_of(0), hi = pos0 + token_of(n_cols - 1);    // positions of the block's tokens
     bool ok = slot >= 0;
     if (ok && (pos0 < 0 || slot >= n_slots || hi / page_size >= max_pages)) {
         if (threadIdx.x == 0) atomicExch(status, 4);
@@ -109,170 +120,187 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
     const int per = (n_chunks + n_splits - 1) / n_splits;
     const int c_begin = chunk0 + split * per, c_end = chunk0 + min(n_chunks, (split + 1) * per);
     if (!ok || c_begin >= c_end) {
-        for (int i = threadIdx.x; i < n_cols; i += I4A_THREADS)
-            if (n_splits > 1) {
+        if (n_splits > 1) {
+            for (int i = threadIdx.x; i < n_cols; i += I4A_THREADS) {
                 float* ml = part_ml + (result_row(i) * n_splits + split) * 2;
                 ml[0] = -INFINITY, ml[1] = 0.f;
             }
-        if (n_splits == 1)
+        } else {
             for (int i = threadIdx.x; i < n_cols * D; i += I4A_THREADS) out[result_row(i / D) * D + i % D] = __float2bfloat16_rn(0.f);
+        }
         return;
     }
     const int* bt = table + (size_t)slot * max_pages;
 
     // ---- the warp's queue: chunk c_begin + warp + 4 i
     unsigned char* ring = i4a_smem + warp * I4A_STAGES * C::BYTES;
-    const bool whole = page_size % I4A_KEYS == 0;                              // a chunk lies in one page
+    constexpr int ROWS = 32 / C::PIECES;                                       // rows that a copy of the warp takes
+    const int my_r = lane / C::PIECES, my_dst = i4a_piece<D>(my_r, lane % C::PIECES);      // of the first copy; others lie ROWS rows on
     int next = c_begin + warp, slot_in = 0;
     bool unmapped = false;
     auto issue = [&]() {
         if (next < c_end) {
-            const int j = next * I4A_KEYS + lane, lp = j / page_size;          // this lane's row of the chunk
-            int page = -1;
-            if (j <= hi) {                                                     // then lp is within the table
-                page = __ldg(bt + lp);
-                if (page < 0 || page >= n_pages) page = -1, unmapped = true;
-            }
-            const long long row = page < 0 ? -1 : ((long long)page * n_kv + kvh) * page_size + (j - lp * page_size);
+            const int j0 = next * I4A_KEYS, here = hi - j0 + 1;                // rows of the chunk that exist
             unsigned char* dst = ring + slot_in * C::BYTES;
-            const long long base = __shfl_sync(0xffffffffu, row, 0);
-            constexpr int ROWS = 32 / C::PIECES;                               // rows that a copy of the warp takes
+            if (whole) {                                                       // a chunk lies in one page: its rows are contiguous
+                const int lp = j0 / page_size, page = __ldg(bt + lp);
+                const bool mapped = page >= 0 && page < n_pages;
+                unmapped |= !mapped;
+                const int rows_here = mapped ? here : 0;
+                const size_t row = mapped ? ((size_t)page * n_kv + kvh) * page_size + (j0 - lp * page_size) : 0;
+                const unsigned char *k = cache.k + row * C::ROW + lane * 16, *v = cache.v + row * C::ROW + lane * 16;
+                const unsigned char *km = cache.km + (row + lane) * (G * 4), *vm = cache.vm + (row + lane) * (G * 4);
+                unsigned char *to = dst + my_dst, *mto = dst + 2 * C::CODES + lane * G * 4;
+                if (rows_here >= I4A_KEYS) {
 #pragma unroll
-            for (int i = 0; i < C::PIECES; ++i) {
-                const int r = i * ROWS + lane / C::PIECES, c = lane % C::PIECES;
-                long long at;
-                if (whole) at = next * I4A_KEYS + r <= hi && base >= 0 ? base + r : -1;
-                else at = __shfl_sync(0xffffffffu, row, r);
-                const size_t off = at < 0 ? 0 : (size_t)at * C::ROW + c * 16;
-                i4a_cp(dst + i4a_piece<D>(r, c), cache.k + off, at >= 0, std::integral_constant<int, 16>());
-                i4a_cp(dst + C::CODES + i4a_piece<D>(r, c), cache.v + off, at >= 0, std::integral_constant<int, 16>());
+                    for (int i = 0; i < C::PIECES; ++i) {
+                        i4a_cp(to + i * 512, k + i * 512, true, std::integral_constant<int, 16>());
+                        i4a_cp(to + C::CODES + i * 512, v + i * 512, true, std::integral_constant<int, 16>());
+                    }
+                    i4a_cp(mto, km, true, std::integral_constant<int, G * 4>());
+                    i4a_cp(mto + C::META, vm, true, std::integral_constant<int, G * 4>());
+                } else {                                                       // rows that do not exist are zeros, and read nowhere
+#pragma unroll 1
+                    for (int i = 0; i < C::PIECES; ++i) {
+                        const bool in = i * ROWS + my_r < rows_here;
+                        i4a_cp(to + i * 512, in ? k + i * 512 : cache.k, in, std::integral_constant<int, 16>());
+                        i4a_cp(to + C::CODES + i * 512, in ? v + i * 512 : cache.v, in, std::integral_constant<int, 16>());
+                    }
+                    const bool in = lane < rows_here;
+                    i4a_cp(mto, in ? km : cache.km, in, std::integral_constant<int, G * 4>());
+                    i4a_cp(mto + C::META, in ? vm : cache.vm, in, std::integral_constant<int, G * 4>());
+                }
+            } else {
+                const int lp = (j0 + lane) / page_size;                        // this lane's row of the chunk
+                long long row = -1;
+                if (lane < here) {                                             // then lp is within the table
+                    const int page = __ldg(bt + lp);
+                    if (page >= 0 && page < n_pages) row = ((long long)page * n_kv + kvh) * page_size + (j0 + lane - lp * page_size);
+                    else unmapped = true;
+                }
+#pragma unroll 1
+                for (int i = 0; i < C::PIECES; ++i) {
+                    const long long at = __shfl_sync(0xffffffffu, row, i * ROWS + my_r);
+                    const size_t off = at < 0 ? 0 : (size_t)at * C::ROW + lane % C::PIECES * 16;
+                    i4a_cp(dst + my_dst + i * 512, cache.k + off, at >= 0, std::integral_constant<int, 16>());
+                    i4a_cp(dst + C::CODES + my_dst + i * 512, cache.v + off, at >= 0, std::integral_constant<int, 16>());
+                }
+                const size_t m = row < 0 ? 0 : (size_t)row * G * 4;
+                i4a_cp(dst + 2 * C::CODES + lane * G * 4, cache.km + m, row >= 0, std::integral_constant<int, G * 4>());
+                i4a_cp(dst + 2 * C::CODES + C::META + lane * G * 4, cache.vm + m, row >= 0, std::integral_constant<int, G * 4>());
             }
-            const size_t moff = row < 0 ? 0 : (size_t)row * G * 4;
-            i4a_cp(dst + 2 * C::CODES + lane * G * 4, cache.km + moff, row >= 0, std::integral_constant<int, G * 4>());
-            i4a_cp(dst + 2 * C::CODES + C::META + lane * G * 4, cache.vm + moff, row >= 0, std::integral_constant<int, G * 4>());
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");                 // an empty group when nothing is left
         next += I4A_WARPS;
         slot_in = slot_in + 1 == I4A_STAGES ? 0 : slot_in + 1;
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < I4A_STAGES - 1; ++i) issue();
 
-    // ---- the queries as operand fragments: lane (g, t) holds, of column g, numbers 16 t .. 16 t + 15 of every group
-    uint4 qf[NT][2 * G];                                                       // of its two words each
-    float qsum[NT][G][2], cscale[NT][2];                                       // of columns 2t, 2t + 1
-    int pcol[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int c = nt * 8 + g;
-        const bool live = c < n_cols;
-        uint4 raw[G][2];
+    // ---- the queries as operand fragments: a thread has 8 numbers of a column
+    constexpr int CHUNKS = D / 8;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < COLS * CHUNKS; i += I4A_THREADS) {           // whole warps, and the threads of a column, go on or stop together
+        const int c = i / CHUNKS, k = i % CHUNKS;
+        const uint4 raw = c < n_cols ? __ldg(reinterpret_cast<const uint4*>(q + result_row(c) * D + k * 8)) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
         uint32_t most = 0;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr)
+        for (int e = 0; e < 4; ++e) most = max(most, max((w[e] & 0x7FFFu) << 16, w[e] & 0x7FFF0000u));
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                raw[gr][h] = live ? __ldg(reinterpret_cast<const uint4*>(q + result_row(c) * D + gr * 64 + t * 16 + h * 8)) : make_uint4(0, 0, 0, 0);
-                const uint32_t w[4] = {raw[gr][h].x, raw[gr][h].y, raw[gr][h].z, raw[gr][h].w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) most = max(most, max((w[e] & 0x7FFFu) << 16, w[e] & 0x7FFF0000u));
-            }
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        for (int o = CHUNKS / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
         int ex;
         const float f = i4_factor(__uint_as_float(min(most, 0x7F7F0000u)), ex);
-        // a query with a number that is not finite has no scores
-        const float back = most > 0x7F7FFFFFu ? __uint_as_float(0x7FC00000u) : i4_pow2(ex) * 1024.f * scale_log2;
-        float sum[G];
+        float a[8], sum = 0.f;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-            sum[gr] = 0.f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t w[4] = {raw[gr][h].x, raw[gr][h].y, raw[gr][h].z, raw[gr][h].w};
-                float a[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    a[2 * e] = i4_bf16_low(w[e]) * f;
-                    a[2 * e + 1] = i4_bf16_high(w[e]) * f;
-                    sum[gr] += a[2 * e] + a[2 * e + 1];
-                }
-                qf[nt][gr * 2 + h] = i4_operand(a);
-            }
-            sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
-            sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+        for (int e = 0; e < 4; ++e) {
+            a[2 * e] = i4_bf16_low(w[e]) * f;
+            a[2 * e + 1] = i4_bf16_high(w[e]) * f;
+            sum += a[2 * e] + a[2 * e + 1];
         }
+        // numbers 32 h + 8 t .. of group k / 8: word h of lane (column, t)
+        s_frag[((c >> 3) * 2 * G + (k >> 2)) * 32 + (c & 7) * 4 + (k & 3)] = i4_operand(a);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int from = (2 * t + e) * 4;                                  // a lane that holds column 2t + e
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr) qsum[nt][gr][e] = __shfl_sync(0xffffffffu, sum[gr], from) * I4_UNIT;
-            cscale[nt][e] = __shfl_sync(0xffffffffu, back, from);
-            const int cc = nt * 8 + 2 * t + e;
-            pcol[nt][e] = cc < n_cols ? pos0 + (col0 + cc) / group : -1;       // no key is at or before -1
-        }
+        for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if ((k & 7) == 0) s_sum[k >> 3][c] = sum * I4_UNIT;
+        // codes are multiples of 2^-24 to the tensor cores; a query with a number that is not finite has no scores
+        if (k == 0) s_back[c] = most > 0x7F7FFFFFu ? __uint_as_float(0x7FC00000u) : i4_pow2(ex) * 1024.f * scale_log2;
     }
-
-    float o[G * 4][NT][4], off_sum[NT][G][2], m[NT][2], l[NT][2];
+    __syncthreads();
+    uint4 qf[NT][2 * G];
+    float qsum[NT][G][2], cscale[NT][2], m[NT][2], use[NT][2], limit[NT][2], l[NT][2], off_sum[NT][G][2], o[G * 4][NT][4];      // of columns 2t, 2t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i) qf[nt][i] = s_frag[(nt * 2 * G + i) * 32 + lane];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            cscale[nt][e] = s_back[nt * 8 + 2 * t + e];
+            m[nt][e] = limit[nt][e] = -INFINITY;
+            use[nt][e] = l[nt][e] = 0.f;                                       // the reference; 0 while no key was seen
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                qsum[nt][gr][e] = s_sum[gr][nt * 8 + 2 * t + e];
+                off_sum[nt][gr][e] = 0.f;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < G * 4; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) off_sum[nt][gr][0] = off_sum[nt][gr][1] = 0.f;
-        m[nt][0] = m[nt][1] = -INFINITY;
-        l[nt][0] = l[nt][1] = 0.f;
     }
-    int vexp[G];                                                               // exponent that the steps of V are scaled by: their largest so far lands in [2^14, 2^15)
+    int vexp[G];                                                               // exponent of the largest step so far
+    float vscale[G], vlimit[G];                                                // what scales it to [2^6, 2^7); steps from here on outgrow it
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) vexp[gr] = -113;
+    for (int gr = 0; gr < G; ++gr) vexp[gr] = -113, vscale[gr] = 0.f, vlimit[gr] = -1.f;
 
-    const int perm = (0x57463120 >> (4 * g)) & 7;                              // row g of a tile is this key, row g + 8 eight behind
-    const int kv0 = (0x57463120 >> (8 * t)) & 7, kv1 = (0x57463120 >> (8 * t + 4)) & 7;   // rows 2t, 2t + 1
+    uint32_t matrix[G];                                                        // this lane's row of the four matrices of a group, K's and V's
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) matrix[gr] = (uint32_t)i4a_piece<D>(((lane >> 3) & 1) * 8 + (lane & 7), gr * 2 + (lane >> 4));
     int slot_out = 0;
     for (int c = c_begin + warp; c < c_end; c += I4A_WARPS) {
         issue();
         asm volatile("cp.async.wait_group %0;\n" ::"n"(I4A_STAGES - 1) : "memory");
         __syncwarp();
-        const unsigned char* sK = ring + slot_out * C::BYTES;
-        const unsigned char* sV = sK + C::CODES;
-        const unsigned char* sKM = sV + C::CODES;
-        const unsigned char* sVM = sKM + C::META;
+        const unsigned char* const chunk = ring + slot_out * C::BYTES;
         slot_out = slot_out + 1 == I4A_STAGES ? 0 : slot_out + 1;
-        const int j0 = c * I4A_KEYS;
-
-        // ---- scores of 32 keys, in powers of two
-        float s[2][NT][4];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            const int r = mt * 16 + perm;
-            float z[G][NT][4];
+#pragma unroll 1
+        for (int half16 = 0; half16 < 2; ++half16) {
+            const int j0 = c * I4A_KEYS + half16 * 16;
+            if (j0 > hi) break;
+            const uint32_t sK = (uint32_t)__cvta_generic_to_shared(chunk) + half16 * 16 * C::ROW;
+            const unsigned char* sKM = chunk + 2 * C::CODES + (half16 * 16 + g) * G * 4;
+            const unsigned char* sVM = sKM + C::META;
+            // ---- scores of 16 keys, in powers of two
+            float s[NT][4], z[G][NT][4];
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) z[gr][nt][e] = 0.f;
-                const uint2 w0 = *reinterpret_cast<const uint2*>(sK + i4a_piece<D>(r, gr * 2 + (t >> 1)) + (t & 1) * 8);
-                const uint2 w1 = *reinterpret_cast<const uint2*>(sK + i4a_piece<D>(r + 8, gr * 2 + (t >> 1)) + (t & 1) * 8);
+                uint32_t w[4];                                                 // rows g, g + 8 of numbers 8 t .., then of 32 + 8 t ..
+                i4a_matrix(w, sK + matrix[gr]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t a0 = h ? w0.y : w0.x, a1 = h ? w1.y : w1.x, c0 = a0 >> 8, c1 = a1 >> 8;
+                    const uint32_t a0 = w[2 * h], a1 = w[2 * h + 1], c0 = a0 >> 8, c1 = a1 >> 8;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const uint4 b = qf[nt][gr * 2 + h];
-                        i4_mma(z[gr][nt], a0 & I4_NEAR, a1 & I4_NEAR, a0 & I4_FAR, a1 & I4_FAR, b.x, b.y);
+                        if (h == 0) i4_mma_first(z[gr][nt], a0 & I4_NEAR, a1 & I4_NEAR, a0 & I4_FAR, a1 & I4_FAR, b.x, b.y);
+                        else i4_mma(z[gr][nt], a0 & I4_NEAR, a1 & I4_NEAR, a0 & I4_FAR, a1 & I4_FAR, b.x, b.y);
                         i4_mma(z[gr][nt], c0 & I4_NEAR, c1 & I4_NEAR, c0 & I4_FAR, c1 & I4_FAR, b.z, b.w);
                     }
                 }
             }
+            float vs[G][2], vo[G][2];                                          // steps and low values of this lane's two values per group
+            bool moved = false;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                uint32_t meta[G];
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) meta[gr] = *reinterpret_cast<const uint32_t*>(sKM + (r + 8 * half) * G * 4 + gr * 4);
+                uint32_t km[G], vm[G];
+                const int at = half * 8 * (G * 4);
+                if (G == 2) {
+                    const uint2 a = *reinterpret_cast<const uint2*>(sKM + at), b = *reinterpret_cast<const uint2*>(sVM + at);
+                    km[0] = a.x, km[G - 1] = a.y, vm[0] = b.x, vm[G - 1] = b.y;
+                } else {
+                    km[0] = *reinterpret_cast<const uint32_t*>(sKM + at), vm[0] = *reinterpret_cast<const uint32_t*>(sVM + at);
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -280,127 +308,113 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
                         float v = 0.f;
 #pragma unroll
                         for (int gr = 0; gr < G; ++gr)
-                            v = fmaf(i4_bf16_low(meta[gr]), z[gr][nt][half * 2 + e], fmaf(i4_bf16_high(meta[gr]), qsum[nt][gr][e], v));
-                        s[mt][nt][half * 2 + e] = v * cscale[nt][e];
+                            v = fmaf(i4_bf16_low(km[gr]), z[gr][nt][half * 2 + e], fmaf(i4_bf16_high(km[gr]), qsum[nt][gr][e], v));
+                        s[nt][half * 2 + e] = fmaf(v, cscale[nt][e], -use[nt][e]);      // above the reference
                     }
-            }
-        }
-        // ---- keys that a column does not see
-        const bool edge = j0 + I4A_KEYS - 1 > first || (window > 0 && j0 <= hi - window);
-        if (edge) {
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
+                for (int gr = 0; gr < G; ++gr) {
+                    vs[gr][half] = i4_bf16_low(vm[gr]);
+                    vo[gr][half] = i4_bf16_high(vm[gr]);
+                    moved |= vs[gr][half] >= vlimit[gr];
+                }
+            }
+            // ---- keys that a column does not see, and values there that are not finite
+            const bool edge = j0 + 15 > first || (window > 0 && j0 <= hi - window);
+            bool odd = false;
+            if (edge) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int j = j0 + mt * 16 + perm + (e >> 1) * 8, p = pcol[nt][e & 1];
-                        if (j > p || (window > 0 && j <= p - window)) s[mt][nt][e] = -INFINITY;
+                        const int j = j0 + g + (e >> 1) * 8, cc = nt * 8 + 2 * t + (e & 1), p = cc < n_cols ? pos0 + token_of(cc) : -1;
+                        if (j > p || (window > 0 && j <= p - window)) s[nt][e] = -INFINITY;
                     }
-        }
-        // ---- running maximum, probabilities
-        float corr[NT][2];
-        bool moved = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                const float m_new = fmaxf(m[nt][e], mx), use = m_new == -INFINITY ? 0.f : m_new;
-                moved |= m_new > m[nt][e];
-                corr[nt][e] = i4a_exp2(m[nt][e] - use);
-                m[nt][e] = m_new;
-                float sum = 0.f;
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        float& v = s[mt][nt][half * 2 + e];
-                        v = i4a_exp2(v - use);
-                        sum += v;
-                    }
-                l[nt][e] = l[nt][e] * corr[nt][e] + sum;
+                for (int gr = 0; gr < G; ++gr) odd |= !(vs[gr][0] <= 3.4e38f) || !(vs[gr][1] <= 3.4e38f) || !(fabsf(vo[gr][0]) <= 3.4e38f) || !(fabsf(vo[gr][1]) <= 3.4e38f);
+                odd = __any_sync(0xffffffffu, odd);
             }
-        // ---- steps and offsets of this lane's four values per group; a larger step changes the scale of what is summed up
-        float vs[G][2][2], vo[G][2][2];                                        // [tile][row g, g + 8]
-        float grow[G];
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-            uint32_t most = 0;
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t meta = *reinterpret_cast<const uint32_t*>(sVM + (mt * 16 + perm + 8 * half) * G * 4 + gr * 4);
-                    vs[gr][mt][half] = i4_bf16_low(meta);
-                    vo[gr][mt][half] = i4_bf16_high(meta);
-                    const uint32_t bits = meta << 16;                          // steps are never negative
-                    most = max(most, bits < 0x7F800000u ? bits : 0u);
-                }
-            most = __reduce_max_sync(0xffffffffu, most);
-            const int e = max((int)(most >> 23) - 127, -112);
-            grow[gr] = 1.f;
-            if (e > vexp[gr]) {                                                // the same for the whole warp
-                grow[gr] = vexp[gr] < -112 ? 0.f : i4a_exp2((float)(vexp[gr] - e));      // nothing summed up yet: 0 times 0
-                vexp[gr] = e;
-                moved = true;
-            }
-            const float vscale = i4_pow2(14 - vexp[gr]);
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) vs[gr][mt][0] *= vscale, vs[gr][mt][1] *= vscale;
-        }
-        if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
+                for (int e = 0; e < 4; ++e) moved |= s[nt][e] > limit[nt][e & 1];
+            // ---- a new reference for the columns' sums, or a new scale for the steps
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
+                    const uint32_t b0 = __float_as_uint(vs[gr][0]), b1 = __float_as_uint(vs[gr][1]);      // never negative; NaN and infinities aside
+                    const uint32_t most = __reduce_max_sync(0xffffffffu, max(b0 < 0x7F800000u ? b0 : 0u, b1 < 0x7F800000u ? b1 : 0u));
+                    const int e = max(max((int)(most >> 23) - 127, -112), vexp[gr]);
+                    const float grow = vexp[gr] < -112 ? 0.f : i4a_exp2((float)(vexp[gr] - e));      // nothing summed up yet: 0 times 0
+                    vexp[gr] = e;
+                    vscale[gr] = i4_pow2(I4A_STEP_TOP - e);
+                    vlimit[gr] = e < 127 ? i4_pow2(e + 1) : INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float f = corr[nt][e & 1] * grow[gr];
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[gr * 4 + i][nt][e] *= f;
-                    }
-                    off_sum[nt][gr][0] *= corr[nt][0];
-                    off_sum[nt][gr][1] *= corr[nt][1];
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) o[gr * 4 + i][nt][x] *= grow;
                 }
-        }
-        // ---- out^T += codes of V^T . (p step)^T
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                uint32_t b[NT][2];                                             // second operand: keys of rows 0-7 and 8-15
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float p0 = s[mt][nt][half * 2], p1 = s[mt][nt][half * 2 + 1];
-                        float x0 = p0 * vs[gr][mt][half], x1 = p1 * vs[gr][mt][half], f0 = p0 * vo[gr][mt][half], f1 = p1 * vo[gr][mt][half];
-                        if (edge) {                                            // a value that is not finite does not reach the columns that do not see it
-                            if (p0 == 0.f) x0 = f0 = 0.f;
-                            if (p1 == 0.f) x1 = f1 = 0.f;
-                        }
-                        off_sum[nt][gr][0] += f0;
-                        off_sum[nt][gr][1] += f1;
-                        b[nt][half] = i4a_transpose(i4_f16x2(x0, x1));
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                        const float m_new = fmaxf(m[nt][e], mx + use[nt][e]), corr = m_new == -INFINITY ? 1.f : i4a_exp2(m[nt][e] - m_new);
+                        const float to = m_new == -INFINITY ? 0.f : m_new;
+                        s[nt][e] += use[nt][e] - to, s[nt][e + 2] += use[nt][e] - to;
+                        m[nt][e] = m_new, use[nt][e] = to;
+                        limit[nt][e] = m_new == -INFINITY ? -INFINITY : I4A_SLACK;
+                        l[nt][e] *= corr;
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) off_sum[nt][gr][e] *= corr;
+#pragma unroll
+                        for (int i = 0; i < G * 4; ++i) o[i][nt][e] *= corr, o[i][nt][e + 2] *= corr;
                     }
-                // words of numbers 8 g .. 8 g + 7 of the keys of rows 2t, 2t + 1, 2t + 8, 2t + 9
-                uint32_t w[4];
+            }
+            // ---- probabilities
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = mt * 16 + (i & 1 ? kv1 : kv0) + (i >> 1) * 8;
-                    w[i] = *reinterpret_cast<const uint32_t*>(sV + i4a_piece<D>(r, gr * 2 + (g >> 2)) + (g & 3) * 4);
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[nt][e] = i4a_exp2(s[nt][e]);
+                    s[nt][e + 2] = i4a_exp2(s[nt][e + 2]);
+                    l[nt][e] += s[nt][e] + s[nt][e + 2];
                 }
+            // ---- out^T += codes of V^T . (p step)^T
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {                                  // numbers 0-3 of the eight, then 4-7, of two keys each
-                    const uint32_t a = __byte_perm(w[0], w[1], h ? 0x7632 : 0x5410), c = __byte_perm(w[2], w[3], h ? 0x7632 : 0x5410);
-                    const uint32_t a8 = a >> 8, c8 = c >> 8;
+            for (int gr = 0; gr < G; ++gr) {
+                uint32_t b[NT][2];                                             // second operand: keys of rows 0-7 and 8-15
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float step = vs[gr][half] * vscale[gr];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        i4_mma(o[gr * 4 + 2 * h][nt], a & I4_NEAR, a & I4_FAR, c & I4_NEAR, c & I4_FAR, b[nt][0], b[nt][1]);
-                        i4_mma(o[gr * 4 + 2 * h + 1][nt], a8 & I4_NEAR, a8 & I4_FAR, c8 & I4_NEAR, c8 & I4_FAR, b[nt][0], b[nt][1]);
+                        const float p0 = s[nt][half * 2], p1 = s[nt][half * 2 + 1];
+                        float x0 = p0 * step, x1 = p1 * step;
+                        if (odd) {                                             // not to the columns that do not see it
+                            x0 = p0 == 0.f ? 0.f : x0, x1 = p1 == 0.f ? 0.f : x1;
+                            off_sum[nt][gr][0] += p0 == 0.f ? 0.f : p0 * vo[gr][half];
+                            off_sum[nt][gr][1] += p1 == 0.f ? 0.f : p1 * vo[gr][half];
+                        } else {
+                            off_sum[nt][gr][0] = fmaf(p0, vo[gr][half], off_sum[nt][gr][0]);
+                            off_sum[nt][gr][1] = fmaf(p1, vo[gr][half], off_sum[nt][gr][1]);
+                        }
+                        b[nt][half] = i4a_transpose(i4_f16x2(x0, x1));
+                    }
+                }
+                // half words of numbers 4 g .. of keys 2 t, 2 t + 1; of keys 8 on; of numbers 32 + 4 g ..
+                uint32_t w[4];
+                i4a_matrix_trans(w, sK + C::CODES + matrix[gr]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t a = w[2 * h], d = w[2 * h + 1], a8 = a >> 8, d8 = d >> 8;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        i4_mma(o[gr * 4 + 2 * h][nt], a & I4_NEAR, a & I4_FAR, d & I4_NEAR, d & I4_FAR, b[nt][0], b[nt][1]);
+                        i4_mma(o[gr * 4 + 2 * h + 1][nt], a8 & I4_NEAR, a8 & I4_FAR, d8 & I4_NEAR, d8 & I4_FAR, b[nt][0], b[nt][1]);
                     }
                 }
             }
@@ -428,22 +442,23 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
                 float f = off_sum[nt][gr][e];
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) f += __shfl_xor_sync(0xffffffffu, f, x);
-                // 2^(vexp - 14) for the steps' scale, 2^24 for the codes', in two factors of which neither overflows
+                // 2^(vexp - 6) for the steps' scale, 2^24 for the codes', in two factors of which neither overflows
                 const float back = vexp[gr] < -112 ? 0.f : i4_pow2(vexp[gr]);
-                float* dst = so + (warp * COLS + cc) * LD + gr * 64 + 8 * g;
+                float* dst = so + (warp * COLS + cc) * LD + gr * 64 + 4 * g;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {                                  // numbers four bits up count 16 times
-                    dst[2 * i] = fmaf(o[gr * 4 + i][nt][e] * 1024.f, back, f);
-                    dst[2 * i + 1] = fmaf(o[gr * 4 + i][nt][e + 2] * 64.f, back, f);
+                    dst[(i >> 1) * 32 + (i & 1) * 2] = fmaf(o[gr * 4 + i][nt][e] * 262144.f, back, f);
+                    dst[(i >> 1) * 32 + (i & 1) * 2 + 1] = fmaf(o[gr * 4 + i][nt][e + 2] * 16384.f, back, f);
                 }
             }
             if (g == 0) {
-                // a sum that is NaN (a key, a query that is not finite) keeps its place whatever the maximum is
+                // a sum that is NaN (a key, a query that is not finite) keeps its place whatever the reference is
                 sml[(warp * COLS + cc) * 2] = sum == sum ? m[nt][e] : 0.f;
                 sml[(warp * COLS + cc) * 2 + 1] = sum;
             }
         }
     __syncthreads();
+#pragma unroll 1
     for (int i = threadIdx.x; i < n_cols * (D / 4); i += I4A_THREADS) {
         const int cc = i / (D / 4), d4 = (i % (D / 4)) * 4;
         float M = -INFINITY;
@@ -451,7 +466,7 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
         for (int w = 0; w < I4A_WARPS; ++w) M = fmaxf(M, sml[(w * COLS + cc) * 2]);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float L = 0.f;
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < I4A_WARPS; ++w) {
             const float mw = sml[(w * COLS + cc) * 2];
             if (mw == -INFINITY) continue;                                     // saw no key
@@ -502,8 +517,8 @@ extern "C" int gi_int4_attention(const void* q, const void* k_codes, const void*
         if (int rc = gi_reserve_smem((const void*)int4_attention_kernel<DD, NN>, smem, "gi_int4_attention")) return rc;              \
         gi_launch(int4_attention_kernel<DD, NN>, dim3((unsigned)(col_tiles * n_splits), n_kv, n_runs), dim3(I4A_THREADS), smem,      \
                   (cudaStream_t)stream, (const bf16*)q, cache, table, (const int4*)runs, tok_pos, tok_slot, (bf16*)out, part_o,      \
-                  part_ml, n_q, n_kv, n_slots, max_pages, page_size, n_pages, window, scale * I4A_LOG2E, n_splits, (int)col_tiles,   \
-                  status);                                                                                                           \
+                  part_ml, n_q, n_kv, n_slots, max_pages, page_size, n_pages, window, scale * I4A_LOG2E, n_splits, n_q / n_kv,       \
+                  page_size % I4A_KEYS == 0, status);                                                                                                           \
     }
     if (d == 64) { if (nt == 1) GI_I4A(64, 1) else GI_I4A(64, 2) }
     else { if (nt == 1) GI_I4A(128, 1) else GI_I4A(128, 2) }
