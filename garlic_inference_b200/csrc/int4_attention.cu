@@ -17,7 +17,7 @@
 //
 //  * A block is one run of tokens, one key/value head, one block of 8 NT columns (token, query head of the group) and one
 //    slice of the keys.  Its 4 warps take 32 keys each, in turn, through a queue of their own (cp.async, three chunks deep), 16 at a time, and
-//    are merged in shared memory at the end; slices are merged by gi_attention_decode_combine, or there is one only.
+//    are merged in shared memory at the end; slices are joined by a second kernel, or there is one only.
 //  * The reference of the softmax is moved only when a score lies 2^8 above it, and the scale of the steps only when one outgrows it:
 //    one vote a step instead of reductions and products over all sums.
 //  * What runs once a block is kept small and rolled up: such instructions come from the instruction cache's next level at about 20 cycles each.
@@ -79,31 +79,24 @@ __device__ __forceinline__ void i4a_matrix_trans(uint32_t (&r)[4], uint32_t at) 
 #define I4A_SLACK 8.f              // a score may lie this far (in powers of two) above the reference
 #define I4A_STEP_TOP 6             // the largest step so far is scaled to [2^6, 2^7): times 2^8 it stays below f16's largest number
 
-// runs[i] = {slot, first row, rows, position of the first row}; without runs, run i is the single token i.
+// Columns col0 .. of a run (rows row0 .. row0 + rows - 1 of q, at positions pos0 ..) over slice `split` of its keys, by a whole block.
 template <int D, int NT>
-__global__ void __launch_bounds__(I4A_THREADS, NT == 1 ? 4 : 3)
-int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __restrict__ table, const int4* __restrict__ runs,
-                      const int* __restrict__ tok_pos, const int* __restrict__ tok_slot, bf16* __restrict__ out,
-                      float* __restrict__ part_o, float* __restrict__ part_ml, int n_q, int n_kv, int n_slots, int max_pages,
-                      int page_size, int n_pages, int window, float scale_log2, int n_splits, int group, int whole, int* __restrict__ status) {
+__device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const Int4Cache& cache, const int* __restrict__ table, bf16* __restrict__ out,
+                                            float* __restrict__ part_o, float* __restrict__ part_ml, int slot, int row0, int rows, int pos0, int col0,
+                                            int kvh, int split, int n_q, int n_kv, int n_slots, int max_pages, int page_size, int n_pages, int window,
+                                            float scale_log2, int n_splits, int group, int whole, int* __restrict__ status) {
     typedef Int4Chunk<D> C;
     constexpr int G = C::G, COLS = 8 * NT;
     extern __shared__ __align__(16) unsigned char i4a_smem[];
-    __shared__ uint4 s_frag[NT * 2 * G * 32];                                  // the queries as operand fragments: [column block][group, word][lane]
-    __shared__ float s_back[COLS], s_sum[G][COLS];                             // what brings a column's scores back; its sums per group
+    // the queries as operand fragments [column block][group, word][lane], what brings a column's scores back, its sums per group: in the
+    // last stage of the first warp's ring, which is filled only once all have read them.  Beyond the rings they would cost the fourth
+    // block of an SM (4 x 55,296 bytes of 233,472, a kilobyte a block taken)
+    static_assert(NT * 2 * G * 512 + (1 + G) * COLS * 4 <= C::BYTES, "the fragments' place");
+    uint4* const s_frag = reinterpret_cast<uint4*>(i4a_smem + (I4A_STAGES - 1) * C::BYTES);
+    float* const s_back = reinterpret_cast<float*>(s_frag + NT * 2 * G * 32);
+    float* const s_sum = s_back + COLS;                                        // [G][COLS]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % n_splits, col0 = blockIdx.x / n_splits * COLS, kvh = blockIdx.y, run = blockIdx.z;
-    gi_pdl_start();
-
-    int slot, row0, rows, pos0;
-    if (runs) {
-        const int4 r = runs[run];
-        slot = r.x, row0 = r.y, rows = r.z, pos0 = r.w;
-    } else {
-        slot = tok_slot[run], row0 = run, rows = 1, pos0 = tok_pos[run];
-    }
-    const int n_cols = min(rows * group - col0, COLS);                         // columns of this block: (token, head of the group)
-    if (n_cols <= 0) return;
+    const int n_cols = min(rows * group - col0, COLS);                         // columns: (token, head of the group)
     auto token_of = [&](int c) { return rows == 1 ? 0 : (col0 + c) / group; };
     auto result_row = [&](int c) {                                             // row of the result that column c is: (token, query head)
         const int tok = token_of(c);
@@ -117,7 +110,7 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
     }
     const int lo = window > 0 ? max(0, first - window + 1) : 0;
     const int chunk0 = lo / I4A_KEYS, n_chunks = hi / I4A_KEYS - chunk0 + 1;
-    const int per = (n_chunks + n_splits - 1) / n_splits;
+    const int per = max((n_chunks + n_splits - 1) / n_splits, 2 * I4A_WARPS);   // fewer chunks do not pay for a block's start
     const int c_begin = chunk0 + split * per, c_end = chunk0 + min(n_chunks, (split + 1) * per);
     if (!ok || c_begin >= c_end) {
         if (n_splits > 1) {
@@ -222,7 +215,7 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
         s_frag[((c >> 3) * 2 * G + (k >> 2)) * 32 + (c & 7) * 4 + (k & 3)] = i4_operand(a);
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if ((k & 7) == 0) s_sum[k >> 3][c] = sum * I4_UNIT;
+        if ((k & 7) == 0) s_sum[(k >> 3) * COLS + c] = sum * I4_UNIT;
         // codes are multiples of 2^-24 to the tensor cores; a query with a number that is not finite has no scores
         if (k == 0) s_back[c] = most > 0x7F7FFFFFu ? __uint_as_float(0x7FC00000u) : i4_pow2(ex) * 1024.f * scale_log2;
     }
@@ -240,7 +233,7 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
             use[nt][e] = l[nt][e] = 0.f;                                       // the reference; 0 while no key was seen
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-                qsum[nt][gr][e] = s_sum[gr][nt * 8 + 2 * t + e];
+                qsum[nt][gr][e] = s_sum[gr * COLS + nt * 8 + 2 * t + e];
                 off_sum[nt][gr][e] = 0.f;
             }
         }
@@ -257,6 +250,7 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
     uint32_t matrix[G];                                                        // this lane's row of the four matrices of a group, K's and V's
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) matrix[gr] = (uint32_t)i4a_piece<D>(((lane >> 3) & 1) * 8 + (lane & 7), gr * 2 + (lane >> 4));
+    __syncthreads();                                                           // the fragments are read: their place may be filled
     int slot_out = 0;
     for (int c = c_begin + warp; c < c_end; c += I4A_WARPS) {
         issue();
@@ -489,26 +483,117 @@ int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __
     }
 }
 
-// runs [n_runs, 4] (first token of the longest: most_rows), or none: every token is a sequence of its own.  With n_splits > 1 the
-// result is left in part_o [tokens, n_q, n_splits, d] and part_ml [tokens, n_q, n_splits, 2] for gi_attention_decode_combine.
+// The run of a block: slot, first row, rows, position of the first row; without runs, run i is the single token i.  False: there is none.
+__device__ __forceinline__ bool i4a_run(const int4* __restrict__ runs, const int* __restrict__ tok_pos, const int* __restrict__ tok_slot, int run,
+                                        int n_rows, int4& r, int* status) {
+    if (!runs) {
+        r = make_int4(tok_slot[run], run, 1, tok_pos[run]);
+        return true;
+    }
+    r = runs[run];
+    if (r.z <= 0) return false;
+    if (r.y >= 0 && r.z <= n_rows && r.y <= n_rows - r.z && r.w <= 2147483647 - r.z) return true;
+    if (threadIdx.x == 0 && status) atomicExch(status, 4);
+    return false;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(I4A_THREADS, NT == 1 ? 4 : 3)
+int4_attention_kernel(const bf16* __restrict__ q, Int4Cache cache, const int* __restrict__ table, const int4* __restrict__ runs,
+                      const int* __restrict__ tok_pos, const int* __restrict__ tok_slot, bf16* __restrict__ out,
+                      float* __restrict__ part_o, float* __restrict__ part_ml, int n_rows, int n_q, int n_kv, int n_slots, int max_pages,
+                      int page_size, int n_pages, int window, float scale_log2, int n_splits, int group, int whole, int* __restrict__ status) {
+    gi_pdl_start();
+    int4 r;
+    if (!i4a_run(runs, tok_pos, tok_slot, blockIdx.z, n_rows, r, status)) return;
+    const int split = blockIdx.x % n_splits, step = gridDim.x / n_splits * (8 * NT);
+#pragma unroll 1
+    for (int col0 = blockIdx.x / n_splits * (8 * NT); col0 < r.z * group; col0 += step) {
+        if (col0 >= step) __syncthreads();                                     // the last columns' sums are read
+        i4a_columns<D, NT>(q, cache, table, out, part_o, part_ml, r.x, r.y, r.z, r.w, col0, blockIdx.y, split, n_q, n_kv, n_slots, max_pages,
+                           page_size, n_pages, window, scale_log2, n_splits, group, whole, status);
+    }
+}
+
+// Joins the slices of a row (token, query head): warp w takes slices w, w + 4 ..; the sums of the four warps meet in shared memory.  A block
+// goes through its run's rows, gridDim.y apart.
+template <int D>
+__global__ void __launch_bounds__(128)
+int4_attention_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int4* __restrict__ runs,
+                           bf16* __restrict__ out, int n_rows, int n_q, int n_splits) {
+    constexpr int V = D / 32, AHEAD = 4;                                       // numbers of a lane; slices whose loads are in flight
+    __shared__ float s_o[4][D], s_l[4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    gi_pdl_start();
+    int4 r = make_int4(0, blockIdx.z, 1, 0);
+    if (runs && !i4a_run(runs, nullptr, nullptr, blockIdx.z, n_rows, r, nullptr)) return;
+#pragma unroll 1
+    for (int tok = blockIdx.y; tok < r.z; tok += gridDim.y) {
+        const size_t row = (size_t)(r.y + tok) * n_q + blockIdx.x;
+        const float* ml = part_ml + row * n_splits * 2;
+        const float* o = part_o + row * n_splits * D + lane * V;
+        float M = -INFINITY;
+        for (int s = lane; s < n_splits; s += 32) M = fmaxf(M, ml[2 * s]);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+        float acc[V], L = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll 1
+        for (int s0 = warp; s0 < n_splits; s0 += 4 * AHEAD) {
+            float m[AHEAD], v[AHEAD][V];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int s = s0 + 4 * j;
+                m[j] = s < n_splits ? ml[2 * s] : -INFINITY;
+                if (m[j] != -INFINITY) {                                           // an empty slice wrote no output
+                    L = fmaf(i4a_exp2(m[j] - M), ml[2 * s + 1], L);
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) *reinterpret_cast<float2*>(&v[j][i]) = *reinterpret_cast<const float2*>(o + (size_t)s * D + i);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+                if (m[j] != -INFINITY) {
+                    const float f = i4a_exp2(m[j] - M);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] = fmaf(f, v[j][i], acc[i]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = acc[i];
+        if (lane == 0) s_l[warp] = L;
+        __syncthreads();
+        if (threadIdx.x < D) {
+            const float sum = s_l[0] + s_l[1] + s_l[2] + s_l[3], v = s_o[0][threadIdx.x] + s_o[1][threadIdx.x] + s_o[2][threadIdx.x] + s_o[3][threadIdx.x];
+            out[row * D + threadIdx.x] = __float2bfloat16_rn(sum == 0.f ? 0.f : v / sum);
+        }
+        __syncthreads();
+    }
+}
+
+// runs [n_runs, 4], or none: every token is a sequence of its own.  With n_splits > 1 the
+// slices lie in part_o [tokens, n_q, n_splits, d] and part_ml [tokens, n_q, n_splits, 2], and a second kernel joins them.
 extern "C" int gi_int4_attention(const void* q, const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta,
-                                 const int* table, const int* runs, int n_runs, int most_rows, const int* tok_pos, const int* tok_slot,
+                                 const int* table, const int* runs, int n_runs, int n_rows, const int* tok_pos, const int* tok_slot,
                                  void* out, float* part_o, float* part_ml, int n_q, int n_kv, int d, int n_slots, int max_pages,
                                  int page_size, int n_pages, int window, float scale, int n_splits, int* status, void* stream) {
     GI_REQUIRE(d == 64 || d == 128, "gi_int4_attention: heads of %d; 64 and 128 are possible", d);
     GI_REQUIRE(n_kv > 0 && n_q > 0 && n_q % n_kv == 0 && n_kv <= 65535, "gi_int4_attention: %d query heads over %d key/value heads", n_q, n_kv);
-    GI_REQUIRE(n_runs >= 0 && n_runs <= 65535 && most_rows >= 1, "gi_int4_attention: %d runs of up to %d tokens", n_runs, most_rows);
+    GI_REQUIRE(n_runs >= 0 && n_runs <= 65535 && n_rows >= (runs ? 0 : n_runs) && n_rows <= 1 << 24,
+               "gi_int4_attention: %d runs of %d rows", n_runs, n_rows);
     GI_REQUIRE(page_size > 0 && max_pages > 0 && n_slots > 0 && window >= 0, "gi_int4_attention: page and table sizes must be positive");
     GI_REQUIRE(n_splits >= 1 && n_splits <= 256 && (n_splits == 1 || (part_o && part_ml)), "gi_int4_attention: %d slices", n_splits);
     GI_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_meta % 8 == 0 &&
                (uintptr_t)v_meta % 8 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)part_o % 16 == 0 && (uintptr_t)runs % 16 == 0,
                "gi_int4_attention: operands must start on 16 bytes");
-    if (n_runs == 0) return 0;
+    if (n_runs == 0 || n_rows == 0) return 0;
     const Int4Cache cache = {(const unsigned char*)k_codes, (const unsigned char*)v_codes, (const unsigned char*)k_meta, (const unsigned char*)v_meta};
-    const long long cols = (long long)most_rows * (n_q / n_kv);
+    const int group = n_q / n_kv;
+    const long long cols = ((long long)n_rows * group + n_runs - 1) / n_runs;   // of a run, on average
     const int nt = cols > 8 ? 2 : 1;
     const long long col_tiles = (cols + 8 * nt - 1) / (8 * nt);
-    GI_REQUIRE(col_tiles * n_splits < 2147483647LL, "gi_int4_attention: runs of %d tokens are too long", most_rows);
+    GI_REQUIRE(col_tiles * n_splits < 2147483647LL, "gi_int4_attention: %d rows in %d runs are too many", n_rows, n_runs);
 #define GI_I4A(DD, NN)                                                                                                               \
     {                                                                                                                                \
         size_t smem = (size_t)I4A_WARPS * I4A_STAGES * Int4Chunk<DD>::BYTES;                                                         \
@@ -517,11 +602,17 @@ extern "C" int gi_int4_attention(const void* q, const void* k_codes, const void*
         if (int rc = gi_reserve_smem((const void*)int4_attention_kernel<DD, NN>, smem, "gi_int4_attention")) return rc;              \
         gi_launch(int4_attention_kernel<DD, NN>, dim3((unsigned)(col_tiles * n_splits), n_kv, n_runs), dim3(I4A_THREADS), smem,      \
                   (cudaStream_t)stream, (const bf16*)q, cache, table, (const int4*)runs, tok_pos, tok_slot, (bf16*)out, part_o,      \
-                  part_ml, n_q, n_kv, n_slots, max_pages, page_size, n_pages, window, scale * I4A_LOG2E, n_splits, n_q / n_kv,       \
-                  page_size % I4A_KEYS == 0, status);                                                                                                           \
+                  part_ml, n_rows, n_q, n_kv, n_slots, max_pages, page_size, n_pages, window, scale * I4A_LOG2E, n_splits, group,    \
+                  page_size % I4A_KEYS == 0, status);                                                                                \
     }
     if (d == 64) { if (nt == 1) GI_I4A(64, 1) else GI_I4A(64, 2) }
     else { if (nt == 1) GI_I4A(128, 1) else GI_I4A(128, 2) }
 #undef GI_I4A
-    return gi_check_launch("gi_int4_attention");
+    if (int rc = gi_check_launch("gi_int4_attention")) return rc;
+    if (n_splits == 1) return 0;
+    const int per = runs ? (n_rows + n_runs - 1) / n_runs : 1;
+    const dim3 joins(n_q, per < 65535 ? per : 65535, n_runs);
+    if (d == 64) gi_launch(int4_attention_join_kernel<64>, joins, dim3(128), 0, (cudaStream_t)stream, part_o, part_ml, (const int4*)runs, (bf16*)out, n_rows, n_q, n_splits);
+    else gi_launch(int4_attention_join_kernel<128>, joins, dim3(128), 0, (cudaStream_t)stream, part_o, part_ml, (const int4*)runs, (bf16*)out, n_rows, n_q, n_splits);
+    return gi_check_launch("gi_int4_attention (slices)");
 }

@@ -34,6 +34,7 @@
 #define I4L_COPIERS 4              // warps that ask for copies
 #define I4L_ERR_COPY 95            // a copy of W did not land
 #define I4L_ERR_SUMS 96            // another block's sums did not arrive
+#define I4L_POLLS (1 << 22)        // of a copying lane for room; a poll that fails takes some tens of cycles
 #define I4L_ERR_ROOM 97            // a place in a ring was not given back
 
 __device__ __forceinline__ void i4l_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -171,7 +172,7 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
                     left = row < my_rows;
                 }
                 if (++slot == I4L_STAGES) slot = 0, ++round;
-            } else if (spin > T5_SPIN_LIMIT || *(volatile int*)&s_abort) {      // bounded: the warps that wait for these copies give up too
+            } else if (spin > I4L_POLLS || *(volatile int*)&s_abort) {      // bounded: the warps that wait for these copies give up too
                 s_abort = 1;
                 atomicExch(error_flag, I4L_ERR_ROOM);
                 break;

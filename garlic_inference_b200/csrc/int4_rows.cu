@@ -3,8 +3,9 @@
 // Pages are codes [pages, heads, page size, d / 2] bytes and meta [pages, heads, page size, d / 64] words (step, low as two
 // bfloat16): a row of d numbers takes d / 2 + d / 16 bytes, 4.5 bits a number.  A group of 64 numbers of a head has one step:
 //   low = min,  step = (max - min) / 15 rounded up to bfloat16,  q = round((x - low) / step) in 0 .. 15
-// so that a number comes back within half a step.  Every kernel gives a group to 16 lanes, 4 numbers each: 8 bytes
-// of a bfloat16 row, 2 bytes of codes.  All are bound by the 16-bit side (2 bytes a number against 0.56).
+// so that a number comes back within half a step.  Writing gives a group to 8 lanes, 8 numbers each (16 bytes of a bfloat16 row, 4 of codes);
+// reading gives it to 4 lanes, 16 numbers each (8 bytes of codes, 32 of the result).  All are bound by the 16-bit side (2 bytes a number
+// against 0.56), a step of a few tokens by the launch.
 #include "int4.cuh"
 
 #define I4R_THREADS 256
@@ -29,37 +30,38 @@ __global__ void __launch_bounds__(I4R_THREADS)
 int4_append_kernel(const T* __restrict__ k, long long k_ts, long long k_hs, const T* __restrict__ v, long long v_ts, long long v_hs,
                    Int4Pool kp, Int4Pool vp, const int* __restrict__ table, const int* __restrict__ tok_pos,
                    const int* __restrict__ tok_slot, int n_kv, int groups, int n_slots, int max_pages, int page_size, int n_pages,
-                   int vec, long long items, int* __restrict__ status) {
+                   int vec, int* __restrict__ status) {
     gi_pdl_launch_dependents();
-    const long long item = ((long long)blockIdx.x * I4R_THREADS + threadIdx.x) >> 4;
-    const int l = threadIdx.x & 15;
-    const bool live = item < items;                                      // 16 lanes alike; the other half of the warp may differ
-    const int grp = (int)(item % groups), head = (int)(item / groups % n_kv);
-    const bool values = (int)(item / groups / n_kv % 2);
-    const int tok = live ? (int)(item / groups / n_kv / 2) : 0;
+    const int at_group = (blockIdx.y * blockDim.x + threadIdx.x) >> 3, l = threadIdx.x & 7, tok = blockIdx.x;      // group: of keys, then of values
+    const bool live = at_group < 2 * n_kv * groups;                      // 8 lanes alike; others of the warp may differ
+    const bool values = at_group >= n_kv * groups;
+    const int of_kind = values ? at_group - n_kv * groups : at_group, head = of_kind / groups, grp = of_kind - head * groups;
     // positions, slots and the block table are set before the step's first kernel: read before the wait
     long long page = 0;
     int row = 0;
     const int pos = tok_pos[tok], slot = tok_slot[tok];
     gi_pdl_wait();
     const bool there = i4r_place(pos, slot, table, n_slots, max_pages, page_size, n_pages, status, live && l == 0, page, row) && live;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (there) {
-        const T* src = (values ? v + tok * v_ts + head * v_hs : k + tok * k_ts + head * k_hs) + grp * I4_GROUP_KV + l * 4;
+        const T* src = (values ? v + tok * v_ts + head * v_hs : k + tok * k_ts + head * k_hs) + grp * I4_GROUP_KV + l * 8;
         if (vec) {
-            const float4 f = load4_act(src);
-            x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+            const float4 f = load4_act(src), h = load4_act(src + 4);
+            x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w, x[4] = h.x, x[5] = h.y, x[6] = h.z, x[7] = h.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = to_f32(src[i]);
+            for (int i = 0; i < 8; ++i) x[i] = to_f32(src[i]);
         }
     }
-    float mn = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    float mn = x[0], mx = x[0];
     int odd = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) odd |= !(fabsf(x[i]) <= 3.402823466e38f);
+    for (int i = 0; i < 8; ++i) {
+        mn = fminf(mn, x[i]), mx = fmaxf(mx, x[i]);
+        odd |= !(fabsf(x[i]) <= 3.402823466e38f);
+    }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
+    for (int o = 4; o > 0; o >>= 1) {
         mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         odd |= __shfl_xor_sync(0xffffffffu, odd, o);
@@ -69,18 +71,35 @@ int4_append_kernel(const T* __restrict__ k, long long k_ts, long long k_hs, cons
     i4_step_low(mn, mx, !odd, step, low);
     uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bits |= i4_code(x[i], step, low) << (4 * i);
+    for (int i = 0; i < 8; ++i) bits |= i4_code(x[i], step, low) << (4 * i);
     const Int4Pool pool = values ? vp : kp;
     const size_t at = (((size_t)page * n_kv + head) * page_size + row) * groups + grp;
-    reinterpret_cast<uint16_t*>(pool.codes)[at * 16 + l] = (uint16_t)bits;
+    reinterpret_cast<uint32_t*>(pool.codes)[at * 8 + l] = bits;
     if (l == 0) pool.meta[at] = i4_meta(step, low);
 }
 
+// 16 numbers
 template <typename T>
-__device__ __forceinline__ void i4r_unpack4(T* dst, uint32_t bits, uint32_t meta) {
+__device__ __forceinline__ void i4r_unpack(T* dst, uint2 bits, uint32_t meta) {
     const float step = i4_bf16_low(meta), low = i4_bf16_high(meta);
-    store4_act(dst, make_float4(fmaf(step, (float)(bits & 15), low), fmaf(step, (float)((bits >> 4) & 15), low),
-                                fmaf(step, (float)((bits >> 8) & 15), low), fmaf(step, (float)((bits >> 12) & 15), low)));
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const uint32_t b = (i < 8 ? bits.x : bits.y) >> (4 * (i & 7));
+        store4_act(dst + i, make_float4(fmaf(step, (float)(b & 15), low), fmaf(step, (float)((b >> 4) & 15), low),
+                                        fmaf(step, (float)((b >> 8) & 15), low), fmaf(step, (float)((b >> 12) & 15), low)));
+    }
+}
+__device__ __forceinline__ void i4r_unpack(bf16* dst, uint2 bits, uint32_t meta) {
+    const float step = i4_bf16_low(meta), low = i4_bf16_high(meta);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t b = h ? bits.y : bits.x;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<__nv_bfloat162*>(&w[i]) = __floats2bfloat162_rn(fmaf(step, (float)((b >> (8 * i)) & 15), low), fmaf(step, (float)((b >> (8 * i + 4)) & 15), low));
+        reinterpret_cast<uint4*>(dst)[h] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 // What the pages hold of the listed tokens: out [tokens, n_kv, d], zeros for padding and where no page is mapped.
@@ -88,21 +107,22 @@ template <typename T>
 __global__ void __launch_bounds__(I4R_THREADS)
 int4_read_kernel(Int4Pool pool, T* __restrict__ out, const int* __restrict__ table, const int* __restrict__ tok_pos,
                  const int* __restrict__ tok_slot, int n_kv, int groups, int n_slots, int max_pages, int page_size, int n_pages,
-                 long long items, int* __restrict__ status) {
+                 int items, int* __restrict__ status) {
     gi_pdl_start();
-    const long long item = ((long long)blockIdx.x * I4R_THREADS + threadIdx.x) >> 4;
+    const int item = blockIdx.x * I4R_THREADS + threadIdx.x;
     if (item >= items) return;
-    const int l = threadIdx.x & 15;
-    const int grp = (int)(item % groups), head = (int)(item / groups % n_kv), tok = (int)(item / groups / n_kv);
+    const int l = item & 3, head_group = item >> 2, per = n_kv * groups, tok = head_group / per, of_tok = head_group - tok * per;
+    const int head = of_tok / groups, grp = of_tok - head * groups;
     long long page;
     int row;
-    uint32_t bits = 0, meta = 0;
+    uint2 bits = make_uint2(0, 0);
+    uint32_t meta = 0;
     if (i4r_place(tok_pos[tok], tok_slot[tok], table, n_slots, max_pages, page_size, n_pages, status, l == 0, page, row)) {
         const size_t at = (((size_t)page * n_kv + head) * page_size + row) * groups + grp;
-        bits = reinterpret_cast<const uint16_t*>(pool.codes)[at * 16 + l];
+        bits = reinterpret_cast<const uint2*>(pool.codes)[at * 4 + l];
         meta = pool.meta[at];
     }
-    i4r_unpack4(out + item * I4_GROUP_KV + l * 4, bits, meta);
+    i4r_unpack(out + (size_t)item * 16, bits, meta);
 }
 
 // Blocks of 64 positions of the step's sequences as bfloat16 pages of their own, [blocks, n_kv, 64, d], for the prompt kernel on
@@ -122,19 +142,20 @@ int4_gather_kernel(Int4Pool kp, Int4Pool vp, bf16* __restrict__ k_out, bf16* __r
     const int head = blockIdx.y >> 1;
     const Int4Pool pool = blockIdx.y & 1 ? vp : kp;
     bf16* out = (blockIdx.y & 1 ? v_out : k_out) + ((size_t)blockIdx.x * n_kv + head) * 64 * groups * I4_GROUP_KV;
-    // 64 rows x groups x 16 lanes; groups is 1 or 2, so a thread's lane and group stay the same from row to row
-    for (int i = threadIdx.x; i < 64 * groups * 16; i += I4R_THREADS) {
-        const int l = i & 15, grp = (i >> 4) % groups, r = (i >> 4) / groups, pos = b.y * 64 + r, lp = pos / page_size;
-        uint32_t bits = 0, meta = 0;
+    // 64 rows x groups x 4 lanes: the lanes of a warp lie in 8 or 4 rows of a page, or of two
+    for (int i = threadIdx.x; i < 64 * groups * 4; i += I4R_THREADS) {
+        const int l = i & 3, of_row = i >> 2, r = of_row / groups, grp = of_row - r * groups, pos = b.y * 64 + r, lp = pos / page_size;
+        uint2 bits = make_uint2(0, 0);
+        uint32_t meta = 0;
         if (ok && lp < max_pages) {
             const int page = __ldg(table + (size_t)b.x * max_pages + lp);
             if (page >= 0 && page < n_pages) {
                 const size_t at = (((size_t)page * n_kv + head) * page_size + (pos - lp * page_size)) * groups + grp;
-                bits = reinterpret_cast<const uint16_t*>(pool.codes)[at * 16 + l];
+                bits = reinterpret_cast<const uint2*>(pool.codes)[at * 4 + l];
                 meta = pool.meta[at];
             }
         }
-        i4r_unpack4(out + (size_t)(r * groups + grp) * I4_GROUP_KV + l * 4, bits, meta);
+        i4r_unpack(out + (size_t)i * 16, bits, meta);
     }
 }
 
@@ -154,15 +175,15 @@ extern "C" int gi_int4_append(const void* k, long long k_ts, long long k_hs, con
     GI_REQUIRE(n_tokens >= 0, "gi_int4_append: %d tokens", n_tokens);
     if (n_tokens == 0) return 0;
     const int groups = d / I4_GROUP_KV;
-    const long long items = (long long)n_tokens * n_kv * 2 * groups, blocks = (items * 16 + I4R_THREADS - 1) / I4R_THREADS;
-    GI_REQUIRE(blocks < 2147483647LL, "gi_int4_append: too many (token, head) pairs");
-    const size_t four = dtype == GI_DTYPE_F32 ? 16 : 8;                  // bytes of four numbers
-    const int vec = (uintptr_t)k % four == 0 && (uintptr_t)v % four == 0 && k_ts % 4 == 0 && k_hs % 4 == 0 && v_ts % 4 == 0 && v_hs % 4 == 0;
+    const int lanes = n_kv * 2 * groups * 8, threads = lanes < I4R_THREADS ? lanes + 31 & ~31 : I4R_THREADS;
+    GI_REQUIRE(n_kv <= 32768, "gi_int4_append: %d heads", n_kv);
+    const size_t eight = dtype == GI_DTYPE_F32 ? 32 : 16;                // bytes of eight numbers
+    const int vec = (uintptr_t)k % eight == 0 && (uintptr_t)v % eight == 0 && k_ts % 8 == 0 && k_hs % 8 == 0 && v_ts % 8 == 0 && v_hs % 8 == 0;
     const Int4Pool kp = {(unsigned char*)k_codes, (uint32_t*)k_meta}, vp = {(unsigned char*)v_codes, (uint32_t*)v_meta};
     cudaStream_t s = (cudaStream_t)stream;
 #define GI_APPEND(T)                                                                                                                 \
-    gi_launch(int4_append_kernel<T>, dim3((unsigned)blocks), dim3(I4R_THREADS), 0, s, (const T*)k, k_ts, k_hs, (const T*)v, v_ts,    \
-              v_hs, kp, vp, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, vec, items, status)
+    gi_launch(int4_append_kernel<T>, dim3(n_tokens, (lanes + threads - 1) / threads), dim3(threads), 0, s, (const T*)k, k_ts, k_hs, (const T*)v, v_ts,    \
+              v_hs, kp, vp, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, vec, status)
     if (dtype == GI_DTYPE_F32) GI_APPEND(float);
     else if (dtype == GI_DTYPE_BF16) GI_APPEND(bf16);
     else GI_REQUIRE(false, "gi_int4_append: dtype %d", dtype);
@@ -177,14 +198,14 @@ extern "C" int gi_int4_read(const void* codes, const void* meta, void* out, int 
     GI_REQUIRE(n_tokens >= 0 && (uintptr_t)out % 16 == 0, "gi_int4_read: %d tokens, the output must start on 16 bytes", n_tokens);
     if (n_tokens == 0) return 0;
     const int groups = d / I4_GROUP_KV;
-    const long long items = (long long)n_tokens * n_kv * groups, blocks = (items * 16 + I4R_THREADS - 1) / I4R_THREADS;
-    GI_REQUIRE(blocks < 2147483647LL, "gi_int4_read: too many (token, head) pairs");
+    GI_REQUIRE((long long)n_tokens * n_kv * groups * 4 < 2147483647LL - I4R_THREADS, "gi_int4_read: too many (token, head) pairs");
+    const int items = n_tokens * n_kv * groups * 4, blocks = (items + I4R_THREADS - 1) / I4R_THREADS;
     const Int4Pool pool = {(unsigned char*)codes, (uint32_t*)meta};
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == GI_DTYPE_F32)
-        gi_launch(int4_read_kernel<float>, dim3((unsigned)blocks), dim3(I4R_THREADS), 0, s, pool, (float*)out, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, items, status);
+        gi_launch(int4_read_kernel<float>, dim3(blocks), dim3(I4R_THREADS), 0, s, pool, (float*)out, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, items, status);
     else if (dtype == GI_DTYPE_BF16)
-        gi_launch(int4_read_kernel<bf16>, dim3((unsigned)blocks), dim3(I4R_THREADS), 0, s, pool, (bf16*)out, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, items, status);
+        gi_launch(int4_read_kernel<bf16>, dim3(blocks), dim3(I4R_THREADS), 0, s, pool, (bf16*)out, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, items, status);
     else GI_REQUIRE(false, "gi_int4_read: dtype %d", dtype);
     return gi_check_launch("gi_int4_read");
 }

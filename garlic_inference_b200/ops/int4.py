@@ -19,12 +19,13 @@ from typing import Optional
 import torch
 
 from . import kernels
-from .kernels import BF16, _dense, _ptr, _stream, code
+from .kernels import code
 from .library import KernelError, check, require_gpu
 
 GROUP_WEIGHT = 128          # inputs that share a step
 GROUP_ROWS = 64             # numbers of a head that share a step
 TILE_BYTES = 1088           # 16 outputs x 128 inputs: 1,024 bytes of codes, then (step, low) of the 16 outputs
+_NO_UNIT = (0, 1.0, float("inf"), float("inf"), 0.0)
 LINEAR_MAX_ROWS = 16        # rows of x that the kernel reading a weight's codes takes
 
 
@@ -39,8 +40,7 @@ class Int4Weight:
 
     def __post_init__(self):
         want = (-(-self.n // 16), -(-self.k // GROUP_WEIGHT), TILE_BYTES)
-        if self.n < 1 or self.k < 1 or self.tiles.dtype != torch.uint8 or tuple(self.tiles.shape) != want or \
-                not self.tiles.is_contiguous():
+        if self.n < 1 or self.k < 1 or self.tiles.dtype is not torch.uint8 or self.tiles.shape != want or not self.tiles.is_contiguous():
             raise KernelError(f"tiles {tuple(self.tiles.shape)} of {self.tiles.dtype} for a weight of {self.n} x {self.k} in 4 "
                               f"bits: dense uint8 {want} holds it")
 
@@ -68,8 +68,9 @@ class Int4Rows:
 
     def __post_init__(self):
         c, m = self.codes, self.meta
-        if c.dim() != 4 or c.dtype != torch.uint8 or c.shape[3] < 32 or c.shape[3] % 32 or m.dtype != torch.bfloat16 or \
-                tuple(m.shape) != (*c.shape[:3], c.shape[3] // 32, 2) or not (c.is_contiguous() and m.is_contiguous()):
+        shape = c.shape
+        if len(shape) != 4 or c.dtype is not torch.uint8 or shape[3] < 32 or shape[3] % 32 or m.dtype is not torch.bfloat16 or \
+                m.shape != (*shape[:3], shape[3] // 32, 2) or not (c.is_contiguous() and m.is_contiguous()):
             raise KernelError(f"codes {tuple(c.shape)} of {c.dtype} and steps {tuple(m.shape)} of {m.dtype} are no pages in 4 bits: "
                               "dense uint8 [pages, heads, page size, d / 2] and bfloat16 [pages, heads, page size, d / 64, 2], "
                               "d a multiple of 64")
@@ -92,37 +93,52 @@ class Int4Rows:
 
 
 # ------------------------------------------------------------------------------------------------------------ weights
-def _on_gpu(t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda:
-        raise KernelError(f"{name} is on {t.device}; the kernels run on the GPU only")
+def _stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _check(device: int, t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dense: bool = True) -> int:
+    """The tensor's address, after checking that it lies on the current device, `device` (the kernels are launched there)."""
+    if t.get_device() != device:
+        raise KernelError(f"{name} is on {t.device}; the kernels run on the current GPU, cuda:{device}")
+    if dtype is not None and t.dtype is not dtype:
+        raise KernelError(f"{name} is {t.dtype}, the kernel wants {dtype}")
+    if dense and not t.is_contiguous():
+        raise KernelError(f"{name} of shape {tuple(t.shape)} and strides {t.stride()} is not dense")
+    return t.data_ptr()
+
+
+def _start() -> tuple:
+    return require_gpu(), torch._C._cuda_getDevice()
 
 
 def quantize_weight(w: torch.Tensor) -> Int4Weight:
     """The weight [n, k] (bfloat16 or float32, rows may lie apart) in 4 bits: low = the group's smallest number, step =
     (largest - smallest) / 15, both rounded to bfloat16 so that the range covers the group; every number the nearest of the 16."""
-    l = require_gpu()
-    kernels._rows(w, "w")
+    l, dev = _start()
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1 or w.stride(1) != 1:
+        raise KernelError(f"a weight of shape {tuple(w.shape)} and strides {w.stride()}: [n, k] with dense rows, n and k at least 1")
     n, k = w.shape
-    if n < 1 or k < 1:
-        raise KernelError(f"a weight of {n} x {k} has nothing to hold")
+    at = _check(dev, w, "w", dense=False)
     tiles = torch.empty((-(-n // 16), -(-k // GROUP_WEIGHT), TILE_BYTES), dtype=torch.uint8, device=w.device)
-    check(l.gi_int4_quantize_weight(_ptr(w), code(w.dtype), w.stride(0) if n > 1 else k, _ptr(tiles), n, k, _stream()), l)
+    check(l.gi_int4_quantize_weight(at, code(w.dtype), w.stride(0) if n > 1 else k, tiles.data_ptr(), n, k, _stream(dev)), l)
     return Int4Weight(tiles, n, k)
 
 
 def dequantize_weight(w: Int4Weight, dtype: torch.dtype = torch.bfloat16, first: int = 0, rows: Optional[int] = None,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Outputs first .. first + rows - 1 of the weight as [rows, k] in `dtype` (rounded once)."""
-    l = require_gpu()
-    _on_gpu(w.tiles, "w")
+    l, dev = _start()
+    tiles = _check(dev, w.tiles, "w")
     rows = w.n - first if rows is None else rows
     if not 0 <= first <= first + rows <= w.n or rows < 1:
         raise KernelError(f"outputs {first} .. {first + rows - 1} of a weight of {w.n}")
     if out is None:
         out = torch.empty((rows, w.k), dtype=dtype, device=w.device)
-    if _dense(out, "out", dtype).shape != (rows, w.k):
+    at = _check(dev, out, "out", dtype)
+    if out.shape != (rows, w.k):
         raise KernelError(f"out {tuple(out.shape)} for {rows} outputs of {w.k} inputs")
-    check(l.gi_int4_dequantize_weight(_ptr(w.tiles), _ptr(out), code(dtype), first, rows, w.n, w.k, _stream()), l)
+    check(l.gi_int4_dequantize_weight(tiles, at, code(dtype), first, rows, w.n, w.k, _stream(dev)), l)
     return out
 
 
@@ -131,47 +147,52 @@ def linear_rows(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.b
     """x W^T for 1 to 16 rows of bfloat16 x, reading the weight's codes once; with `unit` (a `kernels.glu_shape` tuple) the gated
     unit of the weight's first half of outputs (a multiple of 16) and its last.  `out` may be columns of a wider matrix.
     `ranks`, `parts`: blocks that share the inputs, and parts of a block's share that its warps take (0: chosen by the entry point)."""
-    l = require_gpu()
-    _dense(x, "x", torch.bfloat16), _on_gpu(w.tiles, "w")
+    l, dev = _start()
+    at, tiles = _check(dev, x, "x", torch.bfloat16), _check(dev, w.tiles, "w")
     if x.dim() != 2 or x.shape[1] != w.k:
         raise KernelError(f"x {tuple(x.shape)} does not fit a weight {w.shape} ([out, in])")
     m, n = x.shape[0], w.n // 2 if unit is not None else w.n
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=x.device)
-    kernels._rows(out, "out", out_dtype)
-    if out.shape != (m, n):
-        raise KernelError(f"out {tuple(out.shape)} for a result of {(m, n)}")
-    ld = out.stride(0) if m > 1 else max(n, out.stride(0))
-    check(l.gi_int4_linear(_ptr(x), _ptr(w.tiles), _ptr(out), code(out_dtype), ld, m, w.n, w.k, int(unit is not None),
-                           *(unit or (0, 1.0, float("inf"), float("inf"), 0.0)), int(ranks), int(parts), _ptr(kernels.tcgen05_error_flag(x.device)), _stream()), l)
+        out = x.new_empty((m, n), dtype=out_dtype)
+    elif out.shape != (m, n) or n > 1 and out.stride(1) != 1:
+        raise KernelError(f"out {tuple(out.shape)} (strides {out.stride()}) for a result of {(m, n)} with dense rows")
+    to = _check(dev, out, "out", out_dtype, dense=False)
+    flag = kernels._tcgen05_flag.get(dev)
+    if flag is None:
+        flag = kernels.tcgen05_error_flag(x.device)
+    check(l.gi_int4_linear(at, tiles, to, code(out_dtype), out.stride(0) if m > 1 else n, m, w.n, w.k, int(unit is not None),
+                           *(unit or _NO_UNIT), ranks, parts, flag.data_ptr(), _stream(dev)), l)
     return out
 
 
 # -------------------------------------------------------------------------------------------------------------- cache
-def _pools(k_rows: Int4Rows, v_rows: Int4Rows) -> tuple:
-    for r, name in ((k_rows, "k_rows"), (v_rows, "v_rows")):
-        if not isinstance(r, Int4Rows):
-            raise KernelError(f"{name} is a {type(r).__name__}; pages in 4 bits are an Int4Rows")
-        _on_gpu(r.codes, name)
-    if k_rows.shape != v_rows.shape:
-        raise KernelError(f"pages of keys {k_rows.shape} and of values {v_rows.shape} differ")
-    return k_rows.shape
+def _pools(dev: int, k_rows: Int4Rows, v_rows: Int4Rows) -> tuple:
+    """(shape, addresses of the keys' codes and steps, the values')"""
+    if not isinstance(k_rows, Int4Rows) or not isinstance(v_rows, Int4Rows):
+        raise KernelError(f"pages in 4 bits are an Int4Rows, not {type(k_rows).__name__} and {type(v_rows).__name__}")
+    shape = k_rows.shape
+    if v_rows is not k_rows and shape != v_rows.shape:
+        raise KernelError(f"pages of keys {shape} and of values {v_rows.shape} differ")
+    return shape, (_check(dev, k_rows.codes, "k_rows"), _check(dev, k_rows.meta, "k_rows"), _check(dev, v_rows.codes, "v_rows"),
+                   _check(dev, v_rows.meta, "v_rows"))
 
 
-def _ints(**named) -> None:
-    for name, t in named.items():
-        _dense(t, name, torch.int32)
-
-
-def _tokens(n: int, tok_pos: torch.Tensor, tok_slot: torch.Tensor) -> None:
-    if tok_pos.numel() < n or tok_slot.numel() < n:
-        raise KernelError("tok_pos / tok_slot are shorter than the token rows")
-
-
-def _table(block_table: torch.Tensor) -> tuple:
+def _table(dev: int, block_table: torch.Tensor) -> tuple:
     if block_table.dim() != 2:
         raise KernelError(f"a block table is [slots, pages], not {tuple(block_table.shape)}")
-    return tuple(block_table.shape)
+    return _check(dev, block_table, "block_table", torch.int32), *block_table.shape
+
+
+def _tokens(dev: int, n: int, tok_pos: torch.Tensor, tok_slot: torch.Tensor) -> tuple:
+    if tok_pos.numel() < n or tok_slot.numel() < n:
+        raise KernelError("tok_pos / tok_slot are shorter than the token rows")
+    return _check(dev, tok_pos, "tok_pos", torch.int32), _check(dev, tok_slot, "tok_slot", torch.int32)
+
+
+def _status(dev: int, status: torch.Tensor) -> int:
+    if status.numel() < 1:
+        raise KernelError("status is one int32")
+    return _check(dev, status, "status", torch.int32)
 
 
 def append(k: torch.Tensor, v: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor, tok_pos: torch.Tensor,
@@ -179,34 +200,31 @@ def append(k: torch.Tensor, v: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows,
     """Keys and values [n, heads, d] (bfloat16 or float32; tokens and heads may lie apart, numbers of a head may not) of the step's
     tokens into their pages.  Tokens with slot -1 are padding; a place outside the cache is reported in `status` and not
     written.  The tokens' places are distinct."""
-    l = require_gpu()
-    n_pages, heads, page_size, d = _pools(k_rows, v_rows)
-    for t, name in ((k, "k"), (v, "v")):
-        _on_gpu(t, name)
-        if t.dim() != 3 or tuple(t.shape[1:]) != (heads, d) or t.stride(2) != 1 or t.dtype != k.dtype or t.shape != k.shape:
-            raise KernelError(f"{name} {tuple(t.shape)} of {t.dtype} (strides {t.stride()}) is no [n, {heads}, {d}] with dense heads")
-    _ints(block_table=block_table, tok_pos=tok_pos, tok_slot=tok_slot, status=status)
+    l, dev = _start()
+    (n_pages, heads, page_size, d), pools = _pools(dev, k_rows, v_rows)
     n = k.shape[0]
-    _tokens(n, tok_pos, tok_slot)
-    n_slots, width = _table(block_table)
-    check(l.gi_int4_append(_ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), code(k.dtype), _ptr(k_rows.codes),
-                           _ptr(k_rows.meta), _ptr(v_rows.codes), _ptr(v_rows.meta), _ptr(block_table), _ptr(tok_pos), _ptr(tok_slot),
-                           n, heads, d, n_slots, width, page_size, n_pages, _ptr(status), _stream()), l)
+    if k.shape != (n, heads, d) or v.shape != k.shape or v.dtype is not k.dtype or k.stride(2) != 1 or v.stride(2) != 1:
+        raise KernelError(f"k {tuple(k.shape)} and v {tuple(v.shape)} of {k.dtype} and {v.dtype} (strides {k.stride()}, {v.stride()}) are no "
+                          f"[n, {heads}, {d}] of one type with dense heads")
+    table, n_slots, width = _table(dev, block_table)
+    pos, slot = _tokens(dev, n, tok_pos, tok_slot)
+    check(l.gi_int4_append(_check(dev, k, "k", dense=False), k.stride(0), k.stride(1), _check(dev, v, "v", dense=False), v.stride(0),
+                           v.stride(1), code(k.dtype), *pools, table, pos, slot, n, heads, d, n_slots, width, page_size, n_pages,
+                           _status(dev, status), _stream(dev)), l)
 
 
 def read(rows: Int4Rows, block_table: torch.Tensor, tok_pos: torch.Tensor, tok_slot: torch.Tensor, status: torch.Tensor,
          dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """What the pages hold of the listed tokens, [n, heads, d] in `dtype`; zeros for slot -1 and where nothing is mapped (which
     `status` reports)."""
-    l = require_gpu()
-    n_pages, heads, page_size, d = _pools(rows, rows)
-    _ints(block_table=block_table, tok_pos=tok_pos, tok_slot=tok_slot, status=status)
+    l, dev = _start()
+    (n_pages, heads, page_size, d), pools = _pools(dev, rows, rows)
     n = tok_pos.numel()
-    _tokens(n, tok_pos, tok_slot)
-    n_slots, width = _table(block_table)
-    out = torch.empty((n, heads, d), dtype=dtype, device=rows.codes.device)
-    check(l.gi_int4_read(_ptr(rows.codes), _ptr(rows.meta), _ptr(out), code(dtype), _ptr(block_table), _ptr(tok_pos), _ptr(tok_slot),
-                         n, heads, d, n_slots, width, page_size, n_pages, _ptr(status), _stream()), l)
+    table, n_slots, width = _table(dev, block_table)
+    pos, slot = _tokens(dev, n, tok_pos, tok_slot)
+    out = rows.meta.new_empty((n, heads, d), dtype=dtype)
+    check(l.gi_int4_read(pools[0], pools[1], out.data_ptr(), code(dtype), table, pos, slot, n, heads, d, n_slots, width, page_size,
+                         n_pages, _status(dev, status), _stream(dev)), l)
     return out
 
 
@@ -215,32 +233,44 @@ def attention_takes(dtype: torch.dtype, head_dim: int) -> bool:
     return dtype == torch.bfloat16 and head_dim in (64, 128)
 
 
-def _queries(q: torch.Tensor, shape: tuple) -> tuple:
-    _dense(q, "q", torch.bfloat16)
+def _queries(dev: int, q: torch.Tensor, shape: tuple) -> int:
     if q.dim() != 3 or q.shape[2] != shape[3] or q.shape[2] not in (64, 128) or q.shape[1] % shape[1] or q.shape[1] < 1:
         raise KernelError(f"queries {tuple(q.shape)} over pages of {shape[1]} heads of {shape[3]}: [n, a multiple of the heads, 64 or 128]")
-    return tuple(q.shape)
+    return _check(dev, q, "q", torch.bfloat16)
 
 
-def _few(q, k_rows, v_rows, block_table, runs, n_runs, most_rows, tok_pos, tok_slot, scale, window, status, out, n_splits) -> None:
-    l = require_gpu()
-    n_pages, heads, page_size, d = k_rows.shape
+def _few(l, dev: int, q: torch.Tensor, at: int, shape: tuple, pools: tuple, table: tuple, runs, n_runs: int, pos, slot, scale: float,
+         window: int, status: torch.Tensor, out: torch.Tensor, n_splits: int) -> torch.Tensor:
+    n_pages, heads, page_size, d = shape
     n, n_q, _ = q.shape
     part_o = part_ml = None
+    if n_splits > 1:                                         # one workspace: the slices' sums, then their maxima and weights
+        room = q.new_empty((n * n_q * n_splits * (d + 2),), dtype=torch.float32)
+        part_o = room.data_ptr()
+        part_ml = part_o + n * n_q * n_splits * d * 4
+    check(l.gi_int4_attention(at, *pools, table[0], runs, n_runs, n, pos, slot, out.data_ptr(), part_o, part_ml, n_q, heads, d, table[1],
+                              table[2], page_size, n_pages, window, scale, n_splits, _status(dev, status), _stream(dev)), l)
     if n_splits > 1:
-        part_o = torch.empty((n * n_q * n_splits * d,), dtype=torch.float32, device=q.device)
-        part_ml = torch.empty((n * n_q * n_splits * 2,), dtype=torch.float32, device=q.device)
-    check(l.gi_int4_attention(_ptr(q), _ptr(k_rows.codes), _ptr(k_rows.meta), _ptr(v_rows.codes), _ptr(v_rows.meta), _ptr(block_table),
-                              _ptr(runs), n_runs, most_rows, _ptr(tok_pos), _ptr(tok_slot), _ptr(out), _ptr(part_o), _ptr(part_ml),
-                              n_q, heads, d, block_table.shape[0], block_table.shape[1], page_size, n_pages, int(window or 0),
-                              float(scale), n_splits, _ptr(status), _stream()), l)
-    if n_splits > 1:
-        check(l.gi_attention_decode_combine(_ptr(part_o), _ptr(part_ml), _ptr(out), n * n_q, d, n_splits, _stream()), l)
+        kernels.counters.launches += 1                       # the kernel that joins the slices
+    return out
 
 
-def decode_splits(n_runs: int, heads: int) -> int:
-    """Slices of the keys per (run, key/value head, block of columns)."""
-    return max(1, min(64, -(-888 // max(1, n_runs * heads))))
+def decode_splits(n_runs: int, heads: int, keys: int, slots: int = 592, uneven: int = 1024) -> int:
+    """Slices of the keys per (run, key/value head): as many as fill the 148 SMs with 4 blocks each (`slots`), a run of many keys among
+    others one for every `uneven` keys up to 8 (lengths may differ, and are not known here), none of fewer than 256 keys.
+    `keys`: what the table's width or the window lets a run see.  Heads of 128, in us by slices:
+      8 runs of 2,048 keys, 8 heads    1: 25.0   4: 13.8   9: 13.7   14: 13.9   74: 21.9        (9 taken)
+      1 run of 131,000 keys, 8 heads   37: 51.1   55: 45.8   74: 43.0   111: 51.9               (74)
+      48 runs of 1 .. 8,000, 8 heads   1: 99   4: 64.4   7: 61.2   9: 62.9   14: 68.7           (7)
+      64 runs of 500 keys, 8 heads     1: 16.2   4: 23.7   9: 27.7                              (1)
+      1 run of 100 keys, 8 heads       1: 4.4   4: 7.0   74: 9.1                                (1)"""
+    return max(1, min(max(slots // max(1, n_runs * heads), min(8, keys // uneven)), -(-keys // 256), 74))
+
+
+# Up to how many columns (tokens x query heads of a key/value head) of a run, on average, `attention_prompt` reads the codes.  12 runs of
+# 3,000 keys, 8 heads of 128, in us against 153 with wide pages: 20 columns 51, 64 columns 82, 96 columns 137, 128 columns 154; 40 runs
+# of 1,000 keys against 163: 62, 96, 147, 185.
+FEW_COLUMNS = 96
 
 
 def attention_decode(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor, tok_pos: torch.Tensor,
@@ -249,37 +279,47 @@ def attention_decode(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
     """Attention of one token per sequence, q [n, n_q, d] bfloat16 at positions `tok_pos` (their own keys are in the cache), over
     what the cache holds of their sequences; `window` > 0: the last `window` keys.  Returns [n, n_q * d]; rows of slot
     -1 are zeros.  d is 64 or 128."""
-    shape = _pools(k_rows, v_rows)
-    n, n_q, d = _queries(q, shape)
-    _ints(block_table=block_table, tok_pos=tok_pos, tok_slot=tok_slot, status=status)
-    _tokens(n, tok_pos, tok_slot)
-    _table(block_table)
-    out = torch.empty((n, n_q * d), dtype=q.dtype, device=q.device)
-    _few(q, k_rows, v_rows, block_table, None, n, 1, tok_pos, tok_slot, scale, window, status, out, n_splits or decode_splits(n, shape[1]))
-    return out
+    l, dev = _start()
+    shape, pools = _pools(dev, k_rows, v_rows)
+    at = _queries(dev, q, shape)
+    n, n_q, d = q.shape
+    pos, slot = _tokens(dev, n, tok_pos, tok_slot)
+    table = _table(dev, block_table)
+    window = int(window or 0)
+    if not n_splits:
+        keys = table[2] * shape[2]
+        n_splits = decode_splits(n, shape[1], min(keys, window) if window else keys)
+    return _few(l, dev, q, at, shape, pools, table, None, n, pos, slot, scale, window, status, q.new_empty((n, n_q * d)), n_splits)
 
 
 def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor, runs: torch.Tensor,
                      blocks: torch.Tensor, scale: float, window: int, status: torch.Tensor) -> torch.Tensor:
     """Attention of prompts, or portions of prompts, q [n, n_q, d] bfloat16, over the cache (the tokens' own keys are in it).  `runs`
     int32 [n_runs, 4] cuts the rows into runs of at most 128 consecutive tokens of one sequence: {slot, first row, rows, position
-    of the first row}; rows in no run are zeros.  `blocks` int32 [n_blocks, 2] lists, each once, the blocks of 64 positions
-    that any of them sees: {slot, position / 64}.  The blocks' keys and values are rounded to bfloat16 pages for the tensor-memory
-    kernel.  Returns [n, n_q * d]."""
-    l = require_gpu()
-    shape = _pools(k_rows, v_rows)
+    of the first row}; rows in no run are zeros, no row is in two.  `blocks` int32 [n_blocks, 2] lists, each once, the blocks of 64
+    positions that any of them sees: {slot, position / 64}.  Runs of a few tokens read the cache as single tokens do;
+    for longer ones the blocks' keys and values are rounded to bfloat16 pages for the tensor-memory kernel.  Returns [n, n_q * d]."""
+    l, dev = _start()
+    shape, pools = _pools(dev, k_rows, v_rows)
     n_pages, heads, page_size, d = shape
-    n, n_q, _ = _queries(q, shape)
-    _ints(block_table=block_table, runs=runs, blocks=blocks, status=status)
+    at = _queries(dev, q, shape)
+    n, n_q, _ = q.shape
     if runs.dim() != 2 or runs.shape[1] != 4 or blocks.dim() != 2 or blocks.shape[1] != 2:
         raise KernelError(f"runs {tuple(runs.shape)} and blocks {tuple(blocks.shape)} are no int32 [n_runs, 4] and [n_blocks, 2]")
-    n_slots, width = _table(block_table)
-    if runs.shape[0] == 0 or n == 0:
-        return torch.zeros((n, n_q * d), dtype=q.dtype, device=q.device)
-    n_blocks, max_blocks = blocks.shape[0], -(-width * page_size // 64)
-    pages = torch.empty((2, n_blocks, heads, 64, d), dtype=q.dtype, device=q.device)
-    table = torch.full((n_slots, max_blocks), -1, dtype=torch.int32, device=q.device)
-    check(l.gi_int4_gather(_ptr(k_rows.codes), _ptr(k_rows.meta), _ptr(v_rows.codes), _ptr(v_rows.meta), _ptr(pages[0]), _ptr(pages[1]),
-                           _ptr(table), _ptr(blocks), n_blocks, _ptr(block_table), heads, d, n_slots, width, max_blocks, page_size,
-                           n_pages, _ptr(status), _stream()), l)
-    return kernels.attention_prefill_tcgen05(q, pages[0], pages[1], table, runs, scale, window)
+    runs_at, blocks_at = _check(dev, runs, "runs", torch.int32), _check(dev, blocks, "blocks", torch.int32)
+    table = _table(dev, block_table)
+    _, n_slots, width = table
+    window, n_runs, n_blocks = int(window or 0), runs.shape[0], blocks.shape[0]
+    if n_runs == 0 or n == 0:
+        return q.new_zeros((n, n_q * d))
+    columns = -(-n * (n_q // heads) // n_runs)
+    if columns <= FEW_COLUMNS:
+        tiles, slots = (1, 592) if columns <= 8 else (-(-columns // 16), 444)      # wider columns: 3 blocks an SM
+        return _few(l, dev, q, at, shape, pools, table, runs_at, n_runs, None, None, scale, window, status, q.new_zeros((n, n_q * d)),
+                    decode_splits(n_runs * tiles, heads, 64 * n_blocks // n_runs, slots, 2048))
+    max_blocks = -(-width * page_size // 64)
+    pages = q.new_empty((2, n_blocks, heads, 64, d))
+    new_table = block_table.new_full((n_slots, max_blocks), -1)
+    check(l.gi_int4_gather(*pools, pages[0].data_ptr(), pages[1].data_ptr(), new_table.data_ptr(), blocks_at, n_blocks, table[0], heads, d,
+                           n_slots, width, max_blocks, page_size, n_pages, _status(dev, status), _stream(dev)), l)
+    return kernels.attention_prefill_tcgen05(q, pages[0], pages[1], new_table, runs, scale, window)

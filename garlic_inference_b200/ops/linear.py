@@ -83,6 +83,8 @@ def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Opt
     if unit is not None and w.n % 2:
         raise KernelError(f"linear: {w.n} outputs cannot be a gate and an up half")
     m, n = x.shape[0], w.n if unit is None else w.n // 2
+    if 0 < m <= int4.LINEAR_MAX_ROWS and x.dtype is torch.bfloat16 and (unit is None or n % 16 == 0):
+        return int4.linear_rows(x, w, out_dtype, unit, out)
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype, device=x.device)
     if m == 0:
