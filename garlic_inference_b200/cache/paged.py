@@ -26,6 +26,7 @@ from typing import Optional, Sequence, Union
 import numpy as np
 import torch
 
+from ..ops.int4 import Int4Rows
 from .allocator import CacheError, GroupTable, SlotAllocator
 
 TOKEN_UNIT = 64     # capacities are counted per sequence in units of this many tokens
@@ -43,6 +44,8 @@ class KVRequirement:
     mean_block: Optional[int] = None    # P: beside the tokens' rows one row (key and value) for every whole block of P
                                         # positions, kept for the sequence's whole life on pages of its own
     keep_first: int = 0               # with a window: the first positions of a sequence stay beside it
+    bits: Optional[int] = None        # 4: rows of 4-bit numbers with a step per 64 (the view's pools are `Int4Rows`); None: the
+                                      # cache's type
 
     @property
     def value_shape(self) -> tuple:
@@ -91,8 +94,8 @@ class MeansView:
 @dataclass
 class KVView:
     """What a mixer gets for one cache entry in one step."""
-    k_pool: torch.Tensor          # [n_pages, n_kv, page_size, d]
-    v_pool: torch.Tensor
+    k_pool: Union[torch.Tensor, Int4Rows]      # [n_pages, n_kv, page_size, d]
+    v_pool: Union[torch.Tensor, Int4Rows]
     block_table: torch.Tensor     # int32 [max_slots, max_pages_per_seq], -1 = no page
     page_size: int
     window: Optional[int]
@@ -128,7 +131,13 @@ class _KVGroup:
         if req.planes not in (1, 2):
             raise CacheError(f"a paged entry holds 1 or 2 rows per position, not {req.planes}")
         self.storage = self.k_storage = self.v_storage = None
-        if req.value_shape == (req.n_kv_heads, req.head_dim) or req.planes == 1:
+        self.rows: Optional[list] = None             # pages in 4 bits: (keys, values) of each entry
+        if req.bits is not None:
+            if req.bits != 4 or req.planes != 2 or req.value_shape != (req.n_kv_heads, req.head_dim) or req.mean_block or req.keep_first:
+                raise CacheError(f"rows of {req.bits} bits: 4 are possible, for plain keys and values of one shape ({req})")
+            self.rows = [tuple(Int4Rows.zeros(n_pages, req.n_kv_heads, page_size, req.head_dim, device) for _ in range(2))
+                         for _ in entries]
+        elif req.value_shape == (req.n_kv_heads, req.head_dim) or req.planes == 1:
             self.storage = torch.zeros((len(entries), req.planes, n_pages, req.n_kv_heads, page_size, req.head_dim),
                                        dtype=dtype, device=device)
         else:                                    # keys and values of different shapes: a tensor each
@@ -139,11 +148,15 @@ class _KVGroup:
         self.table = torch.full((max_slots, max_pages_per_seq), -1, dtype=torch.int32, device=device)
 
     def pools(self, i: int) -> tuple:
+        if self.rows is not None:
+            return self.rows[i]
         if self.storage is not None:
             return self.storage[i, 0], self.storage[i, self.req.planes - 1]
         return self.k_storage[i], self.v_storage[i]
 
     def bytes_per_token(self) -> int:
+        if self.rows is not None:
+            return len(self.entries) * 2 * self.req.n_kv_heads * (self.req.head_dim // 2 + self.req.head_dim // 64 * 4)
         vh, vd = self.req.value_shape
         per = self.req.n_kv_heads * self.req.head_dim + (vh * vd if self.req.planes == 2 else 0)
         size = (self.storage if self.storage is not None else self.k_storage).element_size()

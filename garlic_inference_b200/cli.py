@@ -40,6 +40,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--stop-ids", default=None, help="token ids that end a request, '7,8' (default: the folder's "
                     "generation_config.json eos_token_id, else none)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default=None, choices=["int4"],
+                    help="keep attention projections and dense feed-forwards in 4 bits (default: as stored)")
+    ap.add_argument("--cache", default=None, choices=["int4"],
+                    help="keep keys and values in 4 bits (default: the activation type)")
     ap.add_argument("--max-tokens", type=int, default=None,
                     help="cache size in tokens (default: what the given prompts need)")
     ap.add_argument("--max-batch", type=int, default=None, help="most requests in one batch")
@@ -78,11 +82,11 @@ def main(argv=None) -> int:
     if args.random_weights:
         model = AutoModel.from_random(load_config(args.model_dir), seed=args.weights_seed, device=args.device,
                                       dtype=args.dtype, max_tokens=args.max_tokens or need, page_size=args.page_size,
-                                      max_slots=args.max_slots)
+                                      max_slots=args.max_slots, weights=args.weights, cache=args.cache)
     else:
         model = AutoModel.from_pretrained(args.model_dir, device=args.device, dtype=args.dtype,
                                           max_tokens=args.max_tokens or need, page_size=args.page_size,
-                                          max_slots=args.max_slots)
+                                          max_slots=args.max_slots, weights=args.weights, cache=args.cache)
     if args.print_logits > 0:
         for i, p in enumerate(prompts):
             slot = model.alloc_slot()

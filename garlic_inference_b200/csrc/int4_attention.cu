@@ -169,7 +169,7 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
                 if (lane < here) {                                             // then lp is within the table
                     const int page = __ldg(bt + lp);
                     if (page >= 0 && page < n_pages) row = ((long long)page * n_kv + kvh) * page_size + (j0 + lane - lp * page_size);
-                    else unmapped = true;
+                    else unmapped |= j0 + lane >= lo;                          // pages behind the window may have been given back
                 }
 #pragma unroll 1
                 for (int i = 0; i < C::PIECES; ++i) {

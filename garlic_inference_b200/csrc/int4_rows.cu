@@ -9,19 +9,19 @@
 #include "int4.cuh"
 
 #define I4R_THREADS 256
+#define I4R_ROPE_WARPS 4
 
 struct Int4Pool { unsigned char* codes; uint32_t* meta; };
 
-// Where a token's rows of the cache are: the page's first row and the row in it, or false.  Bad indexes are reported.
-__device__ __forceinline__ bool i4r_place(int pos, int slot, const int* __restrict__ table, int n_slots, int max_pages, int page_size,
-                                          int n_pages, int* status, bool report, long long& page, int& row) {
-    if (slot < 0) return false;                                          // padding
+// Where a token's rows of the cache are: the page and the row in it.  0, or what is wrong with the position (1) or the page (2).
+__device__ __forceinline__ int i4r_place(int pos, int slot, const int* __restrict__ table, int n_slots, int max_pages, int page_size, int n_pages,
+                                         long long& page, int& row) {
     const int lp = pos / page_size;
-    if (pos < 0 || lp >= max_pages || slot >= n_slots) { if (report) atomicExch(status, 1); return false; }
+    if (pos < 0 || lp >= max_pages || slot >= n_slots) return 1;
     page = table[(size_t)slot * max_pages + lp];
-    if (page < 0 || page >= n_pages) { if (report) atomicExch(status, 2); return false; }
+    if (page < 0 || page >= n_pages) return 2;
     row = pos - lp * page_size;
-    return true;
+    return 0;
 }
 
 // Keys and values of the step's tokens into their pages; k and v: a token's heads k_hs (v_hs) numbers apart, tokens k_ts (v_ts) apart.
@@ -40,8 +40,10 @@ int4_append_kernel(const T* __restrict__ k, long long k_ts, long long k_hs, cons
     long long page = 0;
     int row = 0;
     const int pos = tok_pos[tok], slot = tok_slot[tok];
+    const int bad = slot < 0 ? 0 : i4r_place(pos, slot, table, n_slots, max_pages, page_size, n_pages, page, row);
     gi_pdl_wait();
-    const bool there = i4r_place(pos, slot, table, n_slots, max_pages, page_size, n_pages, status, live && l == 0, page, row) && live;
+    if (bad && live && l == 0) atomicExch(status, bad);
+    const bool there = live && slot >= 0 && !bad;
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (there) {
         const T* src = (values ? v + tok * v_ts + head * v_hs : k + tok * k_ts + head * k_hs) + grp * I4_GROUP_KV + l * 8;
@@ -76,6 +78,94 @@ int4_append_kernel(const T* __restrict__ k, long long k_ts, long long k_hs, cons
     const size_t at = (((size_t)page * n_kv + head) * page_size + row) * groups + grp;
     reinterpret_cast<uint32_t*>(pool.codes)[at * 8 + l] = bits;
     if (l == 0) pool.meta[at] = i4_meta(step, low);
+}
+
+// What the attention layers do to the joined projection qkv [tokens, (n_q + 2 n_kv) d] before the cache: RMSNorm over each head of q and k
+// (with weights), rotation of the first rotary_dim numbers by cos/sin [positions, rotary_dim / 2] (number i with i + rotary_dim / 2), q
+// rounded to q_out [tokens, n_q, d], k (float32, not rounded before) and v into their pages.  A warp takes a head of a token.
+template <int EPL>
+__global__ void __launch_bounds__(I4R_ROPE_WARPS * 32)
+int4_qk_norm_rope_append_kernel(const bf16* __restrict__ qkv, bf16* __restrict__ q_out, Int4Pool kp, Int4Pool vp, const void* __restrict__ q_w,
+                                const void* __restrict__ k_w, int w_dtype, float eps, const float* __restrict__ cos_t,
+                                const float* __restrict__ sin_t, int rotary_dim, const int* __restrict__ tok_pos,
+                                const int* __restrict__ tok_slot, const int* __restrict__ table, int n_q, int n_kv, int n_slots,
+                                int max_pages, int page_size, int n_pages, int max_positions, int heads_here, int* __restrict__ status) {
+    constexpr int d = EPL * 32, LANES = I4_GROUP_KV / EPL;              // lanes of a group
+    __shared__ float s_head[I4R_ROPE_WARPS][d];
+    gi_pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tok = blockIdx.x, h = blockIdx.y * I4R_ROPE_WARPS + warp;
+    const int half = rotary_dim / 2;
+    const bool is_q = h < n_q, is_v = h >= n_q + n_kv;
+    // positions, slots, the block table and the rotation table are set before the step's first kernel: read before the wait
+    const int pos = tok_pos[tok], slot = is_q ? 0 : tok_slot[tok];
+    long long page = 0;
+    int row = 0, bad = 0;
+    if (!is_q && slot >= 0) bad = i4r_place(pos, slot, table, n_slots, max_pages, page_size, n_pages, page, row);
+    if (!bad && !is_v && (pos < 0 || pos >= max_positions)) bad = 3;
+    gi_pdl_wait();                                                      // by every block, whatever it finds: the next kernel's start rests on it
+    if (h >= heads_here || slot < 0) return;
+    if (bad) {
+        if (lane == 0) atomicExch(status, bad);
+        return;
+    }
+    float x[EPL];
+    const bf16* src = qkv + ((size_t)tok * (n_q + 2 * n_kv) + h) * d + lane * EPL;
+#pragma unroll
+    for (int e = 0; e < EPL; e += 2) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(src + e);
+        x[e] = i4_bf16_low(w), x[e + 1] = i4_bf16_high(w);
+    }
+    if (!is_v) {
+        const void* w = is_q ? q_w : k_w;
+        if (w) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) ss += x[e] * x[e];
+            const float inv = rsqrtf(warp_sum(ss) / (float)d + eps);
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) x[e] = x[e] * inv * load_w(w, w_dtype, lane * EPL + e);
+        }
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) s_head[warp][lane * EPL + e] = x[e];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int i = lane * EPL + e;
+            if (i < rotary_dim) {
+                const int j = i < half ? i : i - half;
+                const float c = cos_t[(size_t)pos * half + j], s = sin_t[(size_t)pos * half + j], other = s_head[warp][i < half ? i + half : j];
+                x[e] = i < half ? x[e] * c - other * s : x[e] * c + other * s;
+            }
+        }
+    }
+    if (is_q) {
+        bf16* dst = q_out + ((size_t)tok * n_q + h) * d + lane * EPL;
+#pragma unroll
+        for (int e = 0; e < EPL; e += 2) *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(x[e], x[e + 1]);
+        return;
+    }
+    float mn = x[0], mx = x[0], step, low;
+    int odd = 0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        mn = fminf(mn, x[e]), mx = fmaxf(mx, x[e]);
+        odd |= !(fabsf(x[e]) <= 3.402823466e38f);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        odd |= __shfl_xor_sync(0xffffffffu, odd, o);
+    }
+    i4_step_low(mn, mx, !odd, step, low);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) bits |= i4_code(x[e], step, low) << (4 * e);
+    const Int4Pool pool = is_v ? vp : kp;
+    const size_t at = (((size_t)page * n_kv + (h - n_q - (is_v ? n_kv : 0))) * page_size + row) * (d / I4_GROUP_KV) + lane / LANES;
+    if (EPL == 4) reinterpret_cast<uint16_t*>(pool.codes)[at * 16 + lane % LANES] = (uint16_t)bits;
+    else pool.codes[at * 32 + lane % LANES] = (unsigned char)bits;
+    if (lane % LANES == 0) pool.meta[at] = i4_meta(step, low);
 }
 
 // 16 numbers
@@ -117,7 +207,10 @@ int4_read_kernel(Int4Pool pool, T* __restrict__ out, const int* __restrict__ tab
     int row;
     uint2 bits = make_uint2(0, 0);
     uint32_t meta = 0;
-    if (i4r_place(tok_pos[tok], tok_slot[tok], table, n_slots, max_pages, page_size, n_pages, status, l == 0, page, row)) {
+    const int pos = tok_pos[tok], slot = tok_slot[tok];
+    const int bad = slot < 0 ? 0 : i4r_place(pos, slot, table, n_slots, max_pages, page_size, n_pages, page, row);
+    if (bad && l == 0) atomicExch(status, bad);
+    if (slot >= 0 && !bad) {
         const size_t at = (((size_t)page * n_kv + head) * page_size + row) * groups + grp;
         bits = reinterpret_cast<const uint2*>(pool.codes)[at * 4 + l];
         meta = pool.meta[at];
@@ -189,6 +282,33 @@ extern "C" int gi_int4_append(const void* k, long long k_ts, long long k_hs, con
     else GI_REQUIRE(false, "gi_int4_append: dtype %d", dtype);
 #undef GI_APPEND
     return gi_check_launch("gi_int4_append");
+}
+
+extern "C" int gi_int4_qk_norm_rope_append(const void* qkv, void* q_out, void* k_codes, void* k_meta, void* v_codes, void* v_meta,
+                                           const void* q_w, const void* k_w, int w_dtype, float eps, const float* cos_t,
+                                           const float* sin_t, int rotary_dim, const int* tok_pos, const int* tok_slot, const int* table,
+                                           int n_tokens, int n_q, int n_kv, int d, int n_slots, int max_pages, int page_size,
+                                           int n_pages, int max_positions, int append, int* status, void* stream) {
+    const char* who = "gi_int4_qk_norm_rope_append";
+    if (int rc = check_pool(who, k_codes, k_meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
+    if (int rc = check_pool(who, v_codes, v_meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
+    GI_REQUIRE(d == 64 || d == 128, "%s: heads of %d; 64 and 128 are possible", who, d);
+    GI_REQUIRE(n_tokens >= 0 && n_q > 0 && (long long)n_q + 2LL * n_kv <= 65535 * I4R_ROPE_WARPS, "%s: %d tokens, %d query heads", who, n_tokens, n_q);
+    GI_REQUIRE(rotary_dim >= 0 && rotary_dim <= d && rotary_dim % 2 == 0, "%s: rotary_dim %d must be even and at most %d", who, rotary_dim, d);
+    GI_REQUIRE((q_w == nullptr) == (k_w == nullptr), "%s: q and k norm weights go together", who);
+    GI_REQUIRE((uintptr_t)qkv % 4 == 0 && (uintptr_t)q_out % 4 == 0, "%s: qkv and q must start on 4 bytes", who);
+    if (n_tokens == 0) return 0;
+    const int heads_here = append ? n_q + 2 * n_kv : n_q;
+    const Int4Pool kp = {(unsigned char*)k_codes, (uint32_t*)k_meta}, vp = {(unsigned char*)v_codes, (uint32_t*)v_meta};
+    const dim3 grid(n_tokens, (heads_here + I4R_ROPE_WARPS - 1) / I4R_ROPE_WARPS);
+#define GI_ROPE4(EPL)                                                                                                                \
+    gi_launch(int4_qk_norm_rope_append_kernel<EPL>, grid, dim3(I4R_ROPE_WARPS * 32), 0, (cudaStream_t)stream, (const bf16*)qkv,      \
+              (bf16*)q_out, kp, vp, q_w, k_w, w_dtype, eps, cos_t, sin_t, rotary_dim, tok_pos, tok_slot, table, n_q, n_kv, n_slots,  \
+              max_pages, page_size, n_pages, max_positions, heads_here, status)
+    if (d == 64) GI_ROPE4(2);
+    else GI_ROPE4(4);
+#undef GI_ROPE4
+    return gi_check_launch(who);
 }
 
 extern "C" int gi_int4_read(const void* codes, const void* meta, void* out, int dtype, const int* table, const int* tok_pos,

@@ -31,6 +31,13 @@ def engine_dtype(dtype) -> torch.dtype:
         raise ValueError(f"dtype must be 'bfloat16' or 'float32', not {dtype!r}") from None
 
 
+def _kept(weights, cache) -> dict:
+    for name, v in (("weights", weights), ("cache", cache)):
+        if v not in (None, "int4"):
+            raise ValueError(f"{name} must be None or 'int4', not {v!r}")
+    return {"weights": weights, "cache": cache}
+
+
 def _device(device) -> torch.device:
     if isinstance(device, int):
         return torch.device("cuda", device)
@@ -61,9 +68,13 @@ class LanguageModel:
     # ---- construction ----------------------------------------------------------------
     @classmethod
     def from_pretrained(cls, model_dir, device=0, dtype="bfloat16", max_tokens: int = 8192,
-                        page_size: int = 64, use_graphs: bool = True, max_slots: Optional[int] = None) -> "LanguageModel":
+                        page_size: int = 64, use_graphs: bool = True, max_slots: Optional[int] = None,
+                        weights: Optional[str] = None, cache: Optional[str] = None) -> "LanguageModel":
         """`max_tokens` sizes the cache (tokens that live requests hold, each request's count in units of 64);
-        `max_slots` is the most requests that can be live at once (default: one per 64 tokens of the cache)."""
+        `max_slots` is the most requests that can be live at once (default: one per 64 tokens of the cache).
+        `weights="int4"`: attention projections (grouped-query) and dense feed-forwards in 4 bits, quantised as they are loaded.
+        `cache="int4"`: keys and values of grouped-query attention in 4 bits (bfloat16, heads of 64 or 128)."""
+        kept = _kept(weights, cache)
         from ..ops import require_gpu
         dev = _device(device)
         if dev.type == "cuda":
@@ -75,7 +86,7 @@ class LanguageModel:
             config = config.with_shapes({n: tuple(ckpt.shape(n)) for n in ckpt.names()})
         plan = config.plan()
         ckpt.check(wanted_tensors(plan))
-        model = DecoderModel(plan, ckpt, Runtime(engine_dtype(dtype), dev))
+        model = DecoderModel(plan, ckpt, Runtime(engine_dtype(dtype), dev, **kept))
         stop = ()
         gen_cfg = Path(model_dir) / "generation_config.json"
         if gen_cfg.is_file():
@@ -86,8 +97,11 @@ class LanguageModel:
     @classmethod
     def from_random(cls, config, seed: int = 0, device=0, dtype="bfloat16", max_tokens: int = 8192,
                     page_size: int = 64, std: float = 0.02, norm_std: float = 0.0,
-                    use_graphs: bool = True, max_slots: Optional[int] = None) -> "LanguageModel":
-        """Random weights made on the device (bfloat16 storage), nothing written to disk."""
+                    use_graphs: bool = True, max_slots: Optional[int] = None,
+                    weights: Optional[str] = None, cache: Optional[str] = None) -> "LanguageModel":
+        """Random weights made on the device (bfloat16 storage; `weights` and `cache` as for `from_pretrained`), nothing
+        written to disk."""
+        kept = _kept(weights, cache)
         from ..ops import require_gpu
         dev = _device(device)
         if dev.type == "cuda":
@@ -96,7 +110,7 @@ class LanguageModel:
         plan = config.plan()
         source = RandomSource(wanted_tensors(plan), seed=seed, std=std, norm_std=norm_std,
                               dtype=torch.bfloat16, device=dev)
-        return cls(config, DecoderModel(plan, source, Runtime(engine_dtype(dtype), dev)), max_tokens, page_size,
+        return cls(config, DecoderModel(plan, source, Runtime(engine_dtype(dtype), dev, **kept)), max_tokens, page_size,
                    use_graphs=use_graphs, max_slots=max_slots)
 
     # ---- stepping ----------------------------------------------------------------------

@@ -9,10 +9,12 @@ needs with its shape, which is also what random initialisation writes.
 """
 from __future__ import annotations
 
+import weakref
 from typing import Optional
 
 import torch
 
+from ..ops.int4 import Int4Weight
 from ..config.base import ModelPlan, PartSpec
 from ..parts import Part, Runtime, StepContext, part_class, settle_normed
 from ..weights.loader import TensorWant, WeightError, device_dtype
@@ -64,15 +66,17 @@ class _PartLoader:
         if out is not None:
             out.copy_(self.source.tensor(name))
             return out
-        if name not in self.shared:                 # a tensor named by two parts is loaded once
-            self.shared[name] = self.source.tensor(name).to(device=self.rt.device, dtype=self.dtype(local)).contiguous()
-        return self.shared[name]
+        t = self.shared.get(name)                   # a tensor named by two parts is loaded once
+        if t is None:
+            t = self.source.tensor(name).to(device=self.rt.device, dtype=self.dtype(local)).contiguous()
+            self.shared[name] = t
+        return t
 
 
 class DecoderModel:
     def __init__(self, plan: ModelPlan, source, rt: Runtime):
         self.plan, self.rt = plan, rt
-        shared: dict[str, torch.Tensor] = {}
+        shared = weakref.WeakValueDictionary()       # a tensor is shared while a part keeps it (4-bit weights let go of theirs)
 
         def make(spec: PartSpec):
             return part_class(spec.kind)(spec.params, _PartLoader(spec, source, rt, shared), rt)
@@ -96,6 +100,8 @@ class DecoderModel:
                                          self.positions.get(layer.position), rt, **extra))
         self.final_norm = make(plan.final_norm)
         self.head = make(plan.head)
+        if rt.weights is not None and not any(isinstance(v, Int4Weight) for p in self._all_parts() for v in vars(p).values()):
+            raise ValueError(f"weights={rt.weights!r}: none of this model's parts keeps its weights so")
         self.schedule = tuple(plan.schedule)
         for e in self.schedule:
             if not 0 <= e.layer < len(self.blocks):
@@ -138,6 +144,8 @@ class DecoderModel:
                 raise ValueError(f"the schedule reads cache entry {e.cache} before any layer wrote it")
             reqs[e.cache] = req
             written[e.cache] = written[e.cache] or e.writes_cache
+        if self.rt.cache is not None and not any(getattr(split_requirement(r)[0], "bits", None) for r in reqs):
+            raise ValueError(f"cache={self.rt.cache!r}: none of this model's mixers keeps its keys and values so")
         own = self.embedding.cache_requirement()
         return reqs if own is None else reqs + [own]     # behind the layers' entries
 
@@ -194,6 +202,9 @@ class DecoderModel:
         seen, total = set(), 0
         for obj in self._all_parts():
             for v in vars(obj).values():
+                if isinstance(v, Int4Weight) and v.tiles.data_ptr() not in seen:
+                    seen.add(v.tiles.data_ptr())
+                    total += v.bytes()
                 if isinstance(v, torch.Tensor) and v.is_floating_point() and v.data_ptr() not in seen and v.numel():
                     seen.add(v.data_ptr())
                     total += v.numel() * v.element_size()

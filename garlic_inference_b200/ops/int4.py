@@ -5,7 +5,7 @@ A number q of 0 .. 15 stands for step * q + low, both bfloat16: one pair for 128
 A group with a number that is not finite stands for NaN.
 
   weights   `quantize_weight`, `dequantize_weight`; `linear` and its kin (linear.py) take an `Int4Weight` for their weight
-  cache     `append` writes a step's keys and values, `read` gives back what the pages hold of given tokens,
+  cache     `append` writes a step's keys and values (`qk_norm_rope_append`: out of the joined projection), `read` gives back what the pages hold of given tokens,
             `attention_decode` and `attention_prompt` read them
 
 Products and attention compute with the numbers that the codes stand for, not with these rounded again, save where
@@ -211,6 +211,40 @@ def append(k: torch.Tensor, v: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows,
     check(l.gi_int4_append(_check(dev, k, "k", dense=False), k.stride(0), k.stride(1), _check(dev, v, "v", dense=False), v.stride(0),
                            v.stride(1), code(k.dtype), *pools, table, pos, slot, n, heads, d, n_slots, width, page_size, n_pages,
                            _status(dev, status), _stream(dev)), l)
+
+
+def qk_norm_rope_append(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_weight: Optional[torch.Tensor],
+                        k_weight: Optional[torch.Tensor], eps: float, cos: torch.Tensor, sin: torch.Tensor, rotary_dim: int,
+                        tok_pos: torch.Tensor, tok_slot: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor,
+                        status: torch.Tensor, append: bool = True) -> torch.Tensor:
+    """`kernels.qk_norm_rope_append` over pages in 4 bits: norm and rotate q and k of packed projections [n, (n_q + 2 n_kv) d];
+    returns q [n, n_q, d] and (with `append`) writes k (not rounded to bfloat16 before) and v of every token with a slot."""
+    l, dev = _start()
+    shape, pools = _pools(dev, k_rows, v_rows)
+    n_pages, heads, page_size, d = shape
+    at = _check(dev, qkv, "qkv", torch.bfloat16)
+    if (heads, d) != (n_kv, head_dim) or qkv.dim() != 2 or qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
+        raise KernelError(f"projections {tuple(qkv.shape)} and pages {shape} do not fit {n_q} query heads and {n_kv} key/value heads of "
+                          f"{head_dim}")
+    n = qkv.shape[0]
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] * 2 != rotary_dim:
+        raise KernelError(f"rotary tables {tuple(cos.shape)} and {tuple(sin.shape)} do not fit rotary_dim {rotary_dim}")
+    q_w = k_w = None
+    w_code = 0
+    if (q_weight is None) != (k_weight is None):
+        raise KernelError("q and k norm weights go together")
+    if q_weight is not None:
+        q_w, k_w, w_code = _check(dev, q_weight, "q_weight"), _check(dev, k_weight, "k_weight", q_weight.dtype), code(q_weight.dtype)
+        if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
+            raise KernelError("q/k norm weights must have head_dim elements")
+    table, n_slots, width = _table(dev, block_table)
+    pos, slot = _tokens(dev, n, tok_pos, tok_slot)
+    q = qkv.new_empty((n, n_q, head_dim))
+    check(l.gi_int4_qk_norm_rope_append(at, q.data_ptr(), *pools, q_w, k_w, w_code, float(eps), _check(dev, cos, "cos", torch.float32),
+                                        _check(dev, sin, "sin", torch.float32), rotary_dim, pos, slot, table, n, n_q, n_kv, head_dim,
+                                        n_slots, width, page_size, n_pages, cos.shape[0], int(append), _status(dev, status),
+                                        _stream(dev)), l)
+    return q
 
 
 def read(rows: Int4Rows, block_table: torch.Tensor, tok_pos: torch.Tensor, tok_slot: torch.Tensor, status: torch.Tensor,

@@ -10,6 +10,9 @@ head h reads key/value head h // (n_heads // n_kv_heads).
 The three projections are packed into one weight at load time so that one
 product makes q, k and v (upstream runs three).  All sizes, the eps of the
 q/k norm, the window and the softmax scale are parameters.
+
+With `weights="int4"` (`Runtime`) the two packed weights are kept in 4 bits, with `cache="int4"` the keys and values
+(bfloat16 activations, heads of 64 or 128).
 """
 from __future__ import annotations
 
@@ -17,7 +20,7 @@ import numpy as np
 import torch
 
 from ..cache import KVRequirement
-from ..ops import kernels, linear
+from ..ops import int4, kernels, linear
 from ..weights.loader import TensorWant
 from .base import Mixer, register_part
 
@@ -31,6 +34,13 @@ def query_runs(shape, rows: int) -> np.ndarray:
             for r0 in range(0, n, rows)]
     runs.sort(key=lambda t: -(t[3] + t[2]))
     return np.asarray(runs, dtype=np.int32).reshape(-1, 4)
+
+
+def key_blocks(shape, window: int) -> np.ndarray:
+    """The blocks of 64 positions that the step's rows see, each once: int32 [n_blocks, 2] = {slot, position / 64}."""
+    rows = [(s, b) for s, n, p in zip(shape.seq_slots, shape.seq_lens, shape.seq_past) if n
+            for b in range(max(0, p - window + 1) // 64 if window else 0, -(-(p + n) // 64))]
+    return np.asarray(rows, dtype=np.int32).reshape(-1, 2)
 
 
 def _key_tiles(shape, window: int, chunk: int, keep: int) -> tuple:
@@ -90,13 +100,16 @@ class GQAAttention(Mixer):
         load("q_proj", out=self.w_qkv[:q_rows])
         load("k_proj", out=self.w_qkv[q_rows:q_rows + kv_rows])
         load("v_proj", out=self.w_qkv[q_rows + kv_rows:])
-        self.w_o = load("o_proj")
+        self.w_qkv, self.w_o = rt.held(self.w_qkv), rt.held(load("o_proj"))
+        self.bits = 4 if rt.cache == "int4" else None
+        if self.bits and not int4.attention_takes(rt.dtype, self.d):
+            raise ValueError(f"keys and values in 4 bits want bfloat16 activations and heads of 64 or 128, not {rt.dtype} and {self.d}")
         self.q_norm = load("q_norm") if self.qk_norm else None
         self.k_norm = load("k_norm") if self.qk_norm else None
         self._no_rotary = None
 
     def cache_requirement(self):
-        return KVRequirement(self.n_kv, self.d, self.window)
+        return KVRequirement(self.n_kv, self.d, self.window, bits=self.bits)
 
     def step(self, x, ctx, cache, position, writes_cache=True):
         kv = cache.kv
@@ -109,9 +122,10 @@ class GQAAttention(Mixer):
             tables = self._no_rotary
         cos, sin, rotary_dim = tables
         qkv = linear(x, self.w_qkv)
-        q = kernels.qk_norm_rope_append(qkv, self.n_q, self.n_kv, self.d, self.q_norm, self.k_norm, self.eps,
-                                        cos, sin, rotary_dim, ctx.tok_pos, ctx.tok_slot, kv.k_pool, kv.v_pool,
-                                        kv.block_table, ctx.status, append=writes_cache)
+        prepare = int4.qk_norm_rope_append if self.bits else kernels.qk_norm_rope_append
+        q = prepare(qkv, self.n_q, self.n_kv, self.d, self.q_norm, self.k_norm, self.eps,
+                    cos, sin, rotary_dim, ctx.tok_pos, ctx.tok_slot, kv.k_pool, kv.v_pool,
+                    kv.block_table, ctx.status, append=writes_cache)
         o = self.attend(q, kv, ctx)
         return linear(o, self.w_o)
 
@@ -124,15 +138,21 @@ class GQAAttention(Mixer):
         return 64 if kernels.mma_attention_takes(self.rt.dtype, self.d) else 0
 
     def step_arrays(self, shape, cache):
+        if self.bits and not shape.all_single:
+            w = self.window or 0
+            return {"query_runs_128": lambda: query_runs(shape, 128), f"key_blocks_{w}": lambda: key_blocks(shape, w)}
         rows = 0 if shape.all_single else self._run_rows(cache.kv, shape)
         return {f"query_runs_{rows}": lambda: query_runs(shape, rows)} if rows else {}
 
+    def _array(self, ctx, name: str, make) -> torch.Tensor:
+        a = ctx.arrays.get(name)
+        if a is None:                         # a context put together by hand: make and copy here
+            a = torch.from_numpy(make()).to(ctx.tok_pos.device)
+            ctx.arrays[name] = a
+        return a
+
     def _runs(self, ctx, rows: int) -> torch.Tensor:
-        runs = ctx.arrays.get(f"query_runs_{rows}")
-        if runs is None:                      # a context put together by hand: cut and copy here
-            runs = torch.from_numpy(query_runs(ctx, rows)).to(ctx.tok_pos.device)
-            ctx.arrays[f"query_runs_{rows}"] = runs
-        return runs
+        return self._array(ctx, f"query_runs_{rows}", lambda: query_runs(ctx, rows))
 
     def attend(self, q, kv, ctx):
         """Attention of q [n, n_q, d] over the cache; returns [n, n_q * d].
@@ -141,7 +161,13 @@ class GQAAttention(Mixer):
         attention for runs of tokens, for heads of 64 too unless they see few keys; split-KV when every sequence brings
         one token and the group is at most 16).  Otherwise bfloat16 with a head size the mma.sync kernels take: the split-KV kernel for single
         tokens, the flash kernel for runs.  Everything else (float32, other head sizes, larger groups in
-        decode) goes to the exact-order kernel."""
+        decode) goes to the exact-order kernel.  Pages in 4 bits have kernels of their own."""
+        if self.bits:
+            w = self.window or 0
+            if ctx.all_single or not ctx.seq_lens:
+                return int4.attention_decode(q, kv.k_pool, kv.v_pool, kv.block_table, ctx.tok_pos, ctx.tok_slot, self.scale, w, ctx.status)
+            return int4.attention_prompt(q, kv.k_pool, kv.v_pool, kv.block_table, self._runs(ctx, 128),
+                                         self._array(ctx, f"key_blocks_{w}", lambda: key_blocks(ctx, w)), self.scale, w, ctx.status)
         covered = (not ctx.all_single) and ctx.n_tokens == sum(ctx.seq_lens)
         if ctx.all_single:
             if kernels.tcgen05_decode_takes(q.dtype, self.d, kv.page_size, self.n_q // self.n_kv):

@@ -46,6 +46,7 @@ from typing import Callable, Optional
 
 import torch
 
+from ..ops import int4
 from ..weights.loader import TensorWant
 
 _PARTS: dict[str, type] = {}
@@ -74,6 +75,12 @@ class Runtime:
     """Where and in which precision a model runs."""
     dtype: torch.dtype                  # activation and cache type: bfloat16 or float32
     device: torch.device
+    weights: Optional[str] = None       # "int4": parts that can keep their projections in 4 bits do; None: the stored types
+    cache: Optional[str] = None         # "int4": mixers that can keep keys and values in 4 bits do; None: the activation type
+
+    def held(self, w: torch.Tensor):
+        """A projection's weight as this run keeps it."""
+        return int4.quantize_weight(w) if self.weights == "int4" else w
 
 
 @dataclass

@@ -289,8 +289,8 @@ class ParallelResidualBlock(Block):
         self.w_out = None
         ff = feed_forward
         if ff is not None and hasattr(mixer, "pre_output") and getattr(mixer, "w_o", None) is not None and \
-                hasattr(ff, "pre_output") and getattr(ff, "w_down", None) is not None and \
-                mixer.w_o.dtype == ff.w_down.dtype and mixer.w_o.shape[1] % 8 == 0:
+                hasattr(ff, "pre_output") and isinstance(getattr(ff, "w_down", None), torch.Tensor) and \
+                isinstance(mixer.w_o, torch.Tensor) and mixer.w_o.dtype == ff.w_down.dtype and mixer.w_o.shape[1] % 8 == 0:
             self.k_mixer = mixer.w_o.shape[1]
             self.w_out = torch.cat([mixer.w_o, ff.w_down], dim=1).contiguous()
             mixer.w_o = ff.w_down = None             # the sublayers' own copies are let go: only pre_output runs

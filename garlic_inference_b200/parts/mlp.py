@@ -16,7 +16,9 @@ the product, src/src-cuda/activations/silu.cu:35-67, hadamard.cu:48-67).
 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))) or "swish" (z sigmoid(`swish_alpha` z)); gate and up packed
 like SwiGLU's.  Optional limits make it down( act(min(gate x, `gate_max`)) * (clamp(up x, -`up_limit`, `up_limit`)
 + `up_shift`) ).  With "silu" and no limits it runs SwiGLU's fused products.  `pre_output` hands over what goes
-into the down projection, for arrangements that join it with another product."""
+into the down projection, for arrangements that join it with another product.
+
+With `weights="int4"` (`Runtime`) all of them keep their weights in 4 bits."""
 from __future__ import annotations
 
 import torch
@@ -42,7 +44,7 @@ class SwiGLUMLP(FeedForward):
                                      device=rt.device)
         load("gate_proj", out=self.w_gate_up[:self.inter])
         load("up_proj", out=self.w_gate_up[self.inter:])
-        self.w_down = load("down_proj")
+        self.w_gate_up, self.w_down = rt.held(self.w_gate_up), rt.held(load("down_proj"))
 
     def step(self, x, ctx):
         return linear(swiglu_product(x, self.w_gate_up), self.w_down)
@@ -69,7 +71,7 @@ class GluMLP(FeedForward):
         self.w_gate_up = torch.empty((2 * self.inter, self.hidden), dtype=load.dtype("gate", "up"), device=rt.device)
         load("gate", out=self.w_gate_up[:self.inter])
         load("up", out=self.w_gate_up[self.inter:])
-        self.w_down = load("down")
+        self.w_gate_up, self.w_down = rt.held(self.w_gate_up), rt.held(load("down"))
 
     def pre_output(self, x, ctx, out=None):
         """unit(gate x, up x): [n, intermediate_size] in the activation type, into `out` (columns of a wider matrix)
@@ -93,7 +95,7 @@ class XieluMLP(FeedForward):
 
     def __init__(self, params, load, rt):
         super().__init__(params, load, rt)
-        self.w_up, self.w_down, self.act = load("up"), load("down"), load("act")
+        self.w_up, self.w_down, self.act = rt.held(load("up")), rt.held(load("down")), load("act")
 
     def step(self, x, ctx):
         return linear(kernels.xielu(linear(x, self.w_up), self.act), self.w_down)

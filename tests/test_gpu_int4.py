@@ -397,3 +397,201 @@ def test_values_that_are_not_finite_reach_only_the_tokens_that_see_them(ops):
     ops.int4.append(k, v, k_rows, v_rows, table, pos, slot, status)
     bad = torch.isnan(ops.int4.attention_decode(q, k_rows, v_rows, table, at, of, 0.1, 0, status)).reshape(4, heads, d)
     assert bool(bad[:3, 2:].all()) and not bool(bad[3].any()) and not bool(bad[0, :2].any())
+
+
+# -------------------------------------------------------------------------------------------- a layer's step, as it is used
+def rotary(count, half, g):
+    angle = torch.arange(count, device=DEV)[:, None] * torch.exp(-3 * torch.rand(half, generator=g, device=DEV))[None]
+    return torch.cos(angle), torch.sin(angle)
+
+
+@pytest.mark.parametrize("heads,kv,d,rot,norm,page", [(4, 2, 128, 128, torch.bfloat16, 64), (3, 1, 64, 64, None, 16), (6, 2, 64, 32, torch.float32, 7),
+                                                      (5, 5, 128, 0, torch.bfloat16, 64), (2, 1, 128, 34, None, 32), (32, 8, 128, 128, torch.float32, 64)])
+def test_projections_are_normed_rotated_and_appended(ops, heads, kv, d, rot, norm, page):
+    """Bounds: q is rounded to bfloat16 (2^-8); float32 before that: the sum of d squares, its root, two products and a sum, 32
+    roundings of 2^-24 of |a cos| + |b sin| at most.  k stays within half a step of its group (2^-18 of a step for the quotient)."""
+    g = gen(heads * d + rot)
+    lengths = [40, 3, 90]
+    rows = [ops.int4.Int4Rows.zeros(60, kv, page, d, DEV) for _ in range(2)]
+    width = -(-128 // page)
+    table = torch.randperm(60, generator=torch.Generator().manual_seed(2))[:3 * width].reshape(3, width).to(torch.int32).to(DEV)
+    pos = torch.tensor([0, 39, 17, 2, 89, 64, 5], dtype=torch.int32, device=DEV)
+    slot = torch.tensor([0, 0, -1, 1, 2, 2, 2], dtype=torch.int32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    qkv = (randn(g, 7, (heads + 2 * kv) * d) * torch.exp(randn(g, (heads + 2 * kv) * d))).to(torch.bfloat16)
+    wq, wk = (None, None) if norm is None else ((1 + 0.3 * randn(g, d)).to(norm) for _ in range(2))
+    cos, sin = rotary(100, rot // 2, g)
+    args = (qkv, heads, kv, d, wq, wk, 1e-6, cos, sin, rot, pos, slot, *rows, table, status)
+    before = [r.codes.clone() for r in rows]
+    assert torch.equal(ops.int4.qk_norm_rope_append(*args, append=False), ops.int4.qk_norm_rope_append(*args))
+    got = ops.int4.qk_norm_rope_append(*args)
+    assert int(status) == 0 and not torch.equal(before[0], rows[0].codes)
+
+    def made(x, w):
+        x = x.double().unflatten(1, (-1, d))
+        if w is not None:
+            x = x * torch.rsqrt(x.square().mean(2, keepdim=True) + 1e-6) * w.double()
+        y, size, h = x.clone(), x.abs(), rot // 2
+        if rot:
+            c, s = (t.double()[pos.long()][:, None] for t in (cos, sin))
+            a, b = x[..., :h], x[..., h:rot]
+            y[..., :h], y[..., h:rot] = a * c - b * s, b * c + a * s
+            size = size.clone()
+            size[..., :h], size[..., h:rot] = (a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs()
+        return y, size * 32 * 2 ** -24
+
+    want, off = made(qkv[:, :heads * d], wq)
+    assert bool(((got.double() - want).abs() <= want.abs() * 2 ** -8 + off + 1e-38).all())
+    live = slot >= 0
+    k = ops.int4.read(rows[0], table, pos, slot, status, torch.float32)
+    want, off = made(qkv[:, heads * d:(heads + kv) * d], wk)
+    at = (table[slot[live].long(), (pos[live] // page).long()].long(), slice(None), (pos[live] % page).long())
+    step = rows[0].meta[at][..., 0].double().repeat_interleave(64, -1)
+    assert bool(((k.double() - want).abs()[live] <= step * (0.5 + 2 ** -18) + off[live] + want.abs()[live] * 2 ** -23).all())
+    assert not bool(k[~live].any())
+    # values, and keys without norm and rotation, as `append` writes them
+    other = [ops.int4.Int4Rows.zeros(60, kv, page, d, DEV) for _ in range(2)]
+    plain_k, plain_v = (qkv[:, a * d:(a + kv) * d].unflatten(1, (kv, d)) for a in (heads, heads + kv))
+    ops.int4.append(plain_k, plain_v, *other, table, pos, slot, status)
+    for i in range(1 if norm is not None or rot else 0, 2):
+        assert torch.equal(rows[i].codes, other[i].codes) and torch.equal(rows[i].meta, other[i].meta)
+
+
+def test_a_step_on_another_stream_and_from_two_graphs(ops):
+    """Projection, append, attention and output projection: on a stream of their own, and recorded twice and replayed in
+    turn, give the bits of the eager run on the default stream."""
+    g = gen(11)
+    heads, kv, d, hidden, lengths = 8, 2, 128, 256, [900, 30, 257]
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [n + 1 for n in lengths], kv, d, 64)
+    w_qkv = ops.int4.quantize_weight(0.05 * randn(g, (heads + 2 * kv) * d, hidden))
+    w_o = ops.int4.quantize_weight(0.05 * randn(g, hidden, heads * d))
+    pos, slot = torch.tensor(lengths, dtype=torch.int32, device=DEV), torch.arange(3, dtype=torch.int32, device=DEV)
+    cos, sin = rotary(1000, d // 2, g)
+    xs = [randn(g, 3, hidden).to(torch.bfloat16) for _ in range(2)]
+
+    def step(x):
+        qkv = ops.linear(x, w_qkv)
+        q = ops.int4.qk_norm_rope_append(qkv, heads, kv, d, None, None, 1e-6, cos, sin, d, pos, slot, k_rows, v_rows, table, status)
+        return ops.linear(ops.int4.attention_decode(q, k_rows, v_rows, table, pos, slot, d ** -0.5, 0, status, n_splits=3), w_o)
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [step(x) for x in xs]
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for x in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(x))
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, out, w in zip(graphs, outs, want):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, w)
+    assert int(status) == 0
+
+
+def test_prompts_of_few_and_of_many_tokens_agree_where_they_meet(ops):
+    """The two ways through the cache give the same result within what each may be off."""
+    g = gen(13)
+    heads, kv, d = 8, 2, 128
+    seqs = [(200, 12), (64, 12), (0, 12)]
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [p + n for p, n in seqs], kv, d, 64)
+    spans = [(s, 12 * s, 12, p) for s, (p, n) in enumerate(seqs)]
+    q = randn(g, 36, heads, d).to(torch.bfloat16)
+    runs, blocks = runs_and_blocks(spans, 0)
+    few = ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, d ** -0.5, 0, status)
+    check_attention(few, *plain.attention(q, k_rows, v_rows, table, spans, d ** -0.5, 0))
+    empty = torch.cat([runs[:1].clone(), runs])              # a run without rows, and one of a slot that is idle
+    empty[0, 2] = 0
+    idle = torch.cat([runs, runs[:1]])
+    idle[0, 0] = -1
+    assert torch.equal(ops.int4.attention_prompt(q, k_rows, v_rows, table, empty, blocks, d ** -0.5, 0, status), few)
+    part = ops.int4.attention_prompt(q, k_rows, v_rows, table, idle[:-1], blocks, d ** -0.5, 0, status)
+    rows = slice(int(idle[0, 1]), int(idle[0, 1]) + 12)
+    assert int(status) == 0 and not bool(part[rows].any())
+    for bad in ([0, -1, 4, 0], [0, 30, 12, 0], [0, 0, 12, 1000], [9, 0, 12, 0]):
+        status.zero_()
+        bad = torch.tensor([bad], dtype=torch.int32, device=DEV)
+        assert not bool(ops.int4.attention_prompt(q[:12], k_rows, v_rows, table, bad, blocks, d ** -0.5, 0, status).any()) and int(status) == 4
+
+
+def test_pages_given_back_behind_the_window_are_not_missed(ops):
+    g = gen(17)
+    heads, kv, d, n, window = 4, 1, 64, 300, 50
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [n], kv, d, 16)
+    q = randn(g, 3, heads, d).to(torch.bfloat16)
+    pos, slot = torch.tensor([n - 1], dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    runs, blocks = runs_and_blocks([(0, 0, 3, n - 3)], window)
+    want = ops.int4.attention_decode(q[:1], k_rows, v_rows, table, pos, slot, 0.125, window, status)
+    want_runs = ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, 0.125, window, status)
+    table[0, :(n - 3 - window + 1) // 16] = -1
+    assert torch.equal(ops.int4.attention_decode(q[:1], k_rows, v_rows, table, pos, slot, 0.125, window, status), want)
+    assert torch.equal(ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, 0.125, window, status), want_runs)
+    assert int(status) == 0
+    table[0, (n - 10) // 16] = -1                            # one that the window holds is
+    ops.int4.attention_decode(q[:1], k_rows, v_rows, table, pos, slot, 0.125, window, status)
+    assert int(status) == 5
+
+
+def test_refusals(ops):
+    KernelError = ops.KernelError
+    i4 = ops.int4
+    rows = [i4.Int4Rows.zeros(4, 2, 16, 64, DEV) for _ in range(2)]
+    table = torch.zeros(2, 2, dtype=torch.int32, device=DEV)
+    pos = slot = torch.zeros(3, dtype=torch.int32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=DEV)
+    w = i4.quantize_weight(torch.zeros(32, 128, device=DEV))
+    y = torch.zeros(3, 128, dtype=torch.bfloat16, device=DEV)
+    runs = torch.zeros(1, 4, dtype=torch.int32, device=DEV)
+    blocks = torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    other = i4.Int4Rows.zeros(4, 2, 16, 128, DEV)
+    on_cpu = i4.Int4Rows.zeros(4, 2, 16, 64, "cpu")
+    calls = [
+        lambda: i4.quantize_weight(torch.zeros(4, 4)), lambda: i4.quantize_weight(torch.zeros(4, 4, device=DEV).t()[:, ::2]),
+        lambda: i4.quantize_weight(torch.zeros(0, 4, device=DEV)), lambda: i4.quantize_weight(torch.zeros(4, 4, device=DEV, dtype=torch.float16)),
+        lambda: i4.quantize_weight(torch.zeros(4, device=DEV)),
+        lambda: i4.dequantize_weight(w, first=1, rows=32), lambda: i4.dequantize_weight(w, first=-1, rows=2), lambda: i4.dequantize_weight(w, torch.float16),
+        lambda: i4.dequantize_weight(w, out=torch.zeros(31, 128, device=DEV, dtype=torch.bfloat16)),
+        lambda: ops.linear(y[:, :64], w), lambda: ops.linear(y[0], w), lambda: ops.linear(y.to(torch.float16), w), lambda: ops.linear(y.cpu(), w),
+        lambda: i4.linear_rows(y[:0], w), lambda: i4.linear_rows(torch.zeros(17, 128, dtype=torch.bfloat16, device=DEV), w), lambda: i4.linear_rows(y, w, torch.float16),
+        lambda: i4.linear_rows(y, w, out=torch.zeros(3, 31, device=DEV, dtype=torch.bfloat16)),
+        lambda: i4.linear_rows(y, w, out=torch.zeros(32, 3, device=DEV, dtype=torch.bfloat16).t()),
+        lambda: ops.swiglu_product(y, i4.quantize_weight(torch.zeros(33, 128, device=DEV))),
+        lambda: i4.append(x, x[:, :1], *rows, table, pos, slot, status), lambda: i4.append(x, x.float(), *rows, table, pos, slot, status),
+        lambda: i4.append(x.transpose(1, 2).contiguous().transpose(1, 2), x, *rows, table, pos, slot, status),
+        lambda: i4.append(x, x, rows[0], other, table, pos, slot, status), lambda: i4.append(x, x, on_cpu, on_cpu, table, pos, slot, status),
+        lambda: i4.append(x, x, rows[0].codes, rows[1], table, pos, slot, status), lambda: i4.append(x, x, *rows, table[0], pos, slot, status),
+        lambda: i4.append(x, x, *rows, table, pos[:2], slot, status), lambda: i4.append(x, x, *rows, table, pos.long(), slot, status),
+        lambda: i4.append(x, x, *rows, table, pos, slot.cpu(), status), lambda: i4.append(x, x, *rows, table.t(), pos, slot, status[:0]),
+        lambda: i4.append(x.to(torch.float16), x.to(torch.float16), *rows, table, pos, slot, status),
+        lambda: i4.read(rows[0], table, pos, slot, status, torch.float16), lambda: i4.read(rows[0], table.float(), pos, slot, status),
+        lambda: i4.attention_decode(q.float(), *rows, table, pos, slot, 1.0, 0, status), lambda: i4.attention_decode(q[:, :3], *rows, table, pos, slot, 1.0, 0, status),
+        lambda: i4.attention_decode(q[:, :, :32], *rows, table, pos, slot, 1.0, 0, status), lambda: i4.attention_decode(q[:, ::2], *rows, table, pos, slot, 1.0, 0, status),
+        lambda: i4.attention_decode(q, *rows, table, pos, slot, 1.0, -1, status), lambda: i4.attention_decode(q, *rows, table, pos, slot, 1.0, 0, status, n_splits=257),
+        lambda: i4.attention_decode(q, rows[0], other, table, pos, slot, 1.0, 0, status),
+        lambda: i4.attention_prompt(q, *rows, table, runs[0], blocks, 1.0, 0, status), lambda: i4.attention_prompt(q, *rows, table, runs.long(), blocks, 1.0, 0, status),
+        lambda: i4.attention_prompt(q, *rows, table, runs, blocks.cpu(), 1.0, 0, status),
+    ]
+    cos = torch.zeros(4, 32, device=DEV)
+    qkv = torch.zeros(3, 8 * 64, dtype=torch.bfloat16, device=DEV)
+    rope = lambda a=qkv, n_q=4, c=cos, s=cos, r=64, wq=None, wk=None: i4.qk_norm_rope_append(a, n_q, 2, 64, wq, wk, 1e-6, c, s, r, pos, slot, *rows, table, status)
+    calls += [lambda: rope(a=qkv.float()), lambda: rope(a=qkv[:, :-64]), lambda: rope(n_q=5), lambda: rope(r=32), lambda: rope(s=cos[:2]),
+              lambda: rope(wq=cos[0]), lambda: rope(wq=cos[0], wk=cos[0]), lambda: rope(c=cos.cpu(), s=cos.cpu())]
+    for i, call in enumerate(calls):
+        with pytest.raises(KernelError):
+            call()
+            raise AssertionError(f"call {i} was taken")
+    assert rope().shape == (3, 4, 64)
+    torch.cuda.synchronize()
+    assert ops.linear(y[:0], w).shape == (0, 32)
+    assert i4.attention_decode(q[:0], *rows, table, pos, slot, 1.0, 0, status).shape == (0, 256)
+    i4.append(x[:0], x[:0], *rows, table, pos[:0], slot[:0], status)
+    assert i4.read(rows[0], table, pos[:0], slot[:0], status).shape == (0, 2, 64)

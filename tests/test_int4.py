@@ -1,0 +1,102 @@
+"""4 bits without a GPU: what the holders of weights and pages refuse, the cache's pages, the options of the entry points."""
+import numpy as np
+import pytest
+import torch
+
+from garlic_inference_b200.cache import CacheError, KVRequirement, PagedCache
+from garlic_inference_b200.cli import build_parser
+from garlic_inference_b200.engine import AutoModel
+from garlic_inference_b200.ops import KernelError, int4
+from garlic_inference_b200.parts import Runtime, StepShape, part_class
+from garlic_inference_b200.parts.attention import key_blocks
+
+
+def test_weights_are_held_in_whole_tiles():
+    good = torch.zeros(3, 2, 1088, dtype=torch.uint8)
+    w = int4.Int4Weight(good, 33, 129)
+    assert w.shape == (33, 129) and w.numel() == 33 * 129 and w.bytes() == 6 * 1088
+    for tiles, n, k in ((good, 49, 129), (good, 32, 129), (good, 33, 257), (good, 0, 129), (good, 33, 0), (good[:, :1], 33, 129),
+                        (good.transpose(0, 1).contiguous().transpose(0, 1), 33, 129), (good.to(torch.int8), 33, 129),
+                        (good.reshape(6, 1088), 33, 129)):
+        with pytest.raises(KernelError, match="tiles"):
+            int4.Int4Weight(tiles, n, k)
+
+
+def test_pages_are_held_dense():
+    codes, meta = torch.zeros(2, 3, 4, 64, dtype=torch.uint8), torch.zeros(2, 3, 4, 2, 2, dtype=torch.bfloat16)
+    assert int4.Int4Rows(codes, meta).shape == (2, 3, 4, 128)
+    for c, m in ((codes, meta[..., :1]), (codes, meta.float()), (codes.short(), meta), (codes[..., :48], meta), (codes[:1], meta),
+                 (codes.transpose(1, 2), meta.transpose(1, 2)), (codes[..., ::2], meta[..., :1, :]), (codes[0], meta[0])):
+        with pytest.raises(KernelError, match="no pages in 4 bits"):
+            int4.Int4Rows(c, m)
+    for d in (0, 32, 96):
+        with pytest.raises(KernelError, match="multiple of 64"):
+            int4.Int4Rows.zeros(1, 1, 4, d, "cpu")
+
+
+def test_slices_of_the_keys():
+    for n in (1, 2, 7, 64, 1000):
+        for heads in (1, 2, 8, 40):
+            for keys in (1, 64, 255, 257, 5000, 1 << 20):
+                s = int4.decode_splits(n, heads, keys)
+                assert 1 <= s <= 74 and (s - 1) * 256 < keys
+    assert int4.decode_splits(1, 8, 131000) == 74 and int4.decode_splits(64, 8, 512) == 1
+
+
+@pytest.mark.parametrize("window", [0, 1, 64, 65, 300])
+def test_blocks_of_keys_that_a_step_sees(window):
+    slots, lens, past = [4, 0, 2, 1], [3, 200, 1, 64], [0, 500, 127, 64]
+    got = key_blocks(StepShape(slots, [0, 3, 203, 204], lens, past, False), window)
+    want = {(s, j // 64) for s, n, p in zip(slots, lens, past) for i in range(p, p + n)
+            for j in range(max(0, i - window + 1) if window else 0, i + 1)}
+    assert got.dtype == np.int32 and len(got) == len(want) and {tuple(r) for r in got.tolist()} == want
+
+
+def test_pages_of_the_cache():
+    reqs = [KVRequirement(2, 128, bits=4), KVRequirement(2, 128), KVRequirement(2, 128, bits=4), KVRequirement(1, 64, window=40, bits=4)]
+    cache = PagedCache(reqs, max_tokens=256, max_positions=256, dtype=torch.bfloat16, device="cpu", page_size=16)
+    a, b, c, d = (cache.kv_view(i) for i in range(4))
+    assert a.block_table is c.block_table and a.block_table is not b.block_table
+    for v, shape in ((a, (16, 2, 16, 128)), (c, (16, 2, 16, 128)), (d, (16, 1, 16, 64))):
+        assert isinstance(v.k_pool, int4.Int4Rows) and v.k_pool.shape == v.v_pool.shape == shape
+    held = {t.data_ptr() for v in (a, c) for r in (v.k_pool, v.v_pool) for t in (r.codes, r.meta)}
+    assert len(held) == 8 and isinstance(b.k_pool, torch.Tensor)
+    # two numbers a byte and four bytes for 64 of them
+    assert cache.bytes_per_token() == 2 * 2 * 2 * (64 + 8) + 2 * 2 * 128 * 2 + 2 * (32 + 4)
+    for bad in (KVRequirement(2, 128, bits=8), KVRequirement(2, 128, planes=1, bits=4), KVRequirement(2, 128, value_dim=64, bits=4),
+                KVRequirement(2, 128, window=64, mean_block=16, bits=4), KVRequirement(2, 128, window=64, keep_first=4, bits=4)):
+        with pytest.raises(CacheError, match="bits"):
+            PagedCache([bad], max_tokens=64, max_positions=64, dtype=torch.bfloat16, device="cpu", page_size=16)
+
+
+class _Load:
+    def __init__(self, shapes):
+        self.shapes = shapes
+
+    def dtype(self, *names):
+        return torch.bfloat16
+
+    def __call__(self, name, out=None):
+        return torch.zeros(self.shapes[name].shape, dtype=torch.bfloat16) if out is None else out.zero_()
+
+
+def test_attention_that_cannot_keep_its_keys_in_4_bits_says_so():
+    cls = part_class("gqa_attention")
+    for dtype, d in ((torch.float32, 128), (torch.bfloat16, 32), (torch.bfloat16, 96)):
+        params = dict(hidden_size=64, n_heads=4, n_kv_heads=2, head_dim=d)
+        with pytest.raises(ValueError, match="4 bits"):
+            cls(params, _Load(cls.wanted(params)), Runtime(dtype, torch.device("cpu"), cache="int4"))
+    params = dict(hidden_size=64, n_heads=4, n_kv_heads=2, head_dim=64)
+    part = cls(params, _Load(cls.wanted(params)), Runtime(torch.bfloat16, torch.device("cpu"), cache="int4"))
+    assert part.cache_requirement() == KVRequirement(2, 64, None, bits=4)
+
+
+@pytest.mark.parametrize("name", ["weights", "cache"])
+def test_options_of_the_entry_points(name, tmp_path):
+    for make in (lambda **k: AutoModel.from_random(None, **k), lambda **k: AutoModel.from_pretrained(tmp_path, **k)):
+        with pytest.raises(ValueError, match=f"{name} must be None or 'int4'"):
+            make(**{name: "int8"})
+    args = build_parser().parse_args(["folder", f"--{name}", "int4"])
+    assert getattr(args, name) == "int4" and getattr(build_parser().parse_args(["folder"]), name) is None
+    with pytest.raises(SystemExit):
+        build_parser().parse_args(["folder", f"--{name}", "int2"])
