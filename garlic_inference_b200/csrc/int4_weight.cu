@@ -48,36 +48,44 @@ int4_quantize_weight_kernel(const T* __restrict__ w, long long ld, unsigned char
     if (lane == 0) *reinterpret_cast<uint32_t*>(tile + I4_TILE_CODES + r * 4) = i4_meta(step, low);
 }
 
-// 32 inputs of an output a thread; out [rows, K] holds outputs n0 .. n0 + rows - 1.
+// Eight inputs of eight outputs (a piece of a tile) a thread, so that a warp writes 512 bytes of a row at once; out [rows, K] holds outputs
+// n0 .. n0 + rows - 1.  Bound by writing.
 template <typename T>
 __global__ void __launch_bounds__(256)
-int4_dequantize_weight_kernel(const unsigned char* __restrict__ tiles, T* __restrict__ out, int n0, int rows, int K, int groups,
-                              long long items, int vec) {
+int4_dequantize_weight_kernel(const unsigned char* __restrict__ tiles, T* __restrict__ out, int n0, int rows, int K, int groups, int vec) {
     gi_pdl_start();
-    const long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (item >= items) return;
-    const int quarters = groups * 4;
-    const int kq = (int)(item % quarters);
-    const int row = (int)(item / quarters), n = n0 + row, r = n & 15, k0 = kq * 32;
+    const int word = blockIdx.x * 256 + threadIdx.x, group = word >> 4, k0 = word * 8;      // eight inputs
     if (k0 >= K) return;
-    const unsigned char* tile = tiles + ((long long)(n >> 4) * groups + (kq >> 2)) * I4_TILE;
-    const uint4 c = __ldg(reinterpret_cast<const uint4*>(tile + (r >> 3) * 512 + ((r & 7) * 4 + (kq & 3)) * 16));
-    const uint32_t meta = __ldg(reinterpret_cast<const uint32_t*>(tile + I4_TILE_CODES + r * 4));
-    const float step = i4_bf16_low(meta), low = i4_bf16_high(meta);
-    T* dst = out + (long long)row * K + k0;
-    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+    const int piece = blockIdx.y + (n0 >> 3);
+    const unsigned char* tile = tiles + ((size_t)(piece >> 1) * groups + group) * I4_TILE;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(tile + (piece & 1) * 512) + (word & 15);
+    const uint32_t* meta = reinterpret_cast<const uint32_t*>(tile + I4_TILE_CODES) + (piece & 1) * 8;
+    uint32_t c[8], m[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {                                        // four numbers at a time
-        const uint32_t h = words[j >> 1] >> (16 * (j & 1));
-        const float4 v = make_float4(fmaf(step, (float)(h & 15), low), fmaf(step, (float)((h >> 4) & 15), low),
-                                     fmaf(step, (float)((h >> 8) & 15), low), fmaf(step, (float)((h >> 12) & 15), low));
-        if (vec) {                                                       // K is a multiple of 4: a whole four, or none
-            if (k0 + 4 * j < K) store4_act(dst + 4 * j, v);
+    for (int r = 0; r < 8; ++r) c[r] = __ldg(codes + r * 16), m[r] = __ldg(meta + r);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const int row = piece * 8 + r - n0;
+        if (row < 0 || row >= rows) continue;
+        const float step = i4_bf16_low(m[r]), low = i4_bf16_high(m[r]);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(step, (float)((c[r] >> (4 * i)) & 15), low);
+        T* dst = out + (size_t)row * K + k0;
+        if (vec) {                                                       // K is a multiple of 8
+            if (sizeof(T) == 2) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<__nv_bfloat162*>(&w[i]) = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+                store4_act(dst, make_float4(v[0], v[1], v[2], v[3]));
+                store4_act(dst + 4, make_float4(v[4], v[5], v[6], v[7]));
+            }
         } else {
-            if (k0 + 4 * j < K) dst[4 * j] = from_f32<T>(v.x);
-            if (k0 + 4 * j + 1 < K) dst[4 * j + 1] = from_f32<T>(v.y);
-            if (k0 + 4 * j + 2 < K) dst[4 * j + 2] = from_f32<T>(v.z);
-            if (k0 + 4 * j + 3 < K) dst[4 * j + 3] = from_f32<T>(v.w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (k0 + i < K) dst[i] = from_f32<T>(v[i]);
         }
     }
 }
@@ -102,14 +110,14 @@ extern "C" int gi_int4_dequantize_weight(const void* tiles, void* out, int dtype
                "gi_int4_dequantize_weight: outputs %d .. %d of a weight of %d x %d", n0, n0 + rows - 1, N, K);
     GI_REQUIRE((uintptr_t)tiles % 16 == 0, "gi_int4_dequantize_weight: the tiles must start on 16 bytes");
     const int groups = (K - 1) / I4_GROUP_W + 1;
-    const long long items = (long long)rows * groups * 4, blocks = (items + 255) / 256;
-    GI_REQUIRE(blocks < 2147483647LL, "gi_int4_dequantize_weight: %lld pieces are too many", items);
-    const int vec = K % 4 == 0 && (uintptr_t)out % 16 == 0;
+    const dim3 grid((K + 2047) / 2048, ((n0 + rows + 7) >> 3) - (n0 >> 3));      // eight rows a block
+    GI_REQUIRE(grid.y <= 65535, "gi_int4_dequantize_weight: %d outputs at a time are too many", rows);
+    const int vec = K % 8 == 0 && (uintptr_t)out % 16 == 0;
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == GI_DTYPE_F32)
-        gi_launch(int4_dequantize_weight_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, s, (const unsigned char*)tiles, (float*)out, n0, rows, K, groups, items, vec);
+        gi_launch(int4_dequantize_weight_kernel<float>, grid, dim3(256), 0, s, (const unsigned char*)tiles, (float*)out, n0, rows, K, groups, vec);
     else if (dtype == GI_DTYPE_BF16)
-        gi_launch(int4_dequantize_weight_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, s, (const unsigned char*)tiles, (bf16*)out, n0, rows, K, groups, items, vec);
+        gi_launch(int4_dequantize_weight_kernel<bf16>, grid, dim3(256), 0, s, (const unsigned char*)tiles, (bf16*)out, n0, rows, K, groups, vec);
     else GI_REQUIRE(false, "gi_int4_dequantize_weight: dtype %d", dtype);
     return gi_check_launch("gi_int4_dequantize_weight");
 }

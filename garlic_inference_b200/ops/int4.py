@@ -147,6 +147,29 @@ def linear_rows(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.b
     """x W^T for 1 to 16 rows of bfloat16 x, reading the weight's codes once; with `unit` (a `kernels.glu_shape` tuple) the gated
     unit of the weight's first half of outputs (a multiple of 16) and its last.  `out` may be columns of a wider matrix.
     `ranks`, `parts`: blocks that share the inputs, and parts of a block's share that its warps take (0: chosen by the entry point)."""
+    l, at, tiles, to, m, ld, flag, dev, out = _product(x, w, out_dtype, unit, out)
+    check(l.gi_int4_linear(at, tiles, to, code(out_dtype), ld, m, w.n, w.k, int(unit is not None), *(unit or _NO_UNIT), ranks, parts,
+                           flag, _stream(dev)), l)
+    return out
+
+
+def linear_rows_takes(rows: int, w: Int4Weight, gated: bool) -> bool:
+    """Whether `linear_rows` has room for so many rows of this weight's inputs."""
+    return bool(require_gpu().gi_int4_linear_takes(rows, w.n, w.k, int(gated)))
+
+
+def linear_wide(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.bfloat16, unit: Optional[tuple] = None,
+                out: Optional[torch.Tensor] = None, ranks: int = 0) -> torch.Tensor:
+    """`linear_rows` for any number of rows (the inner size a multiple of 8, x on 16 bytes): the numbers that the codes stand for are
+    rounded to bfloat16 for the tensor cores, once for 32 or 64 rows.  `ranks`: blocks that share the inputs (0: chosen by the
+    entry point)."""
+    l, at, tiles, to, m, ld, flag, dev, out = _product(x, w, out_dtype, unit, out)
+    check(l.gi_int4_linear_tcgen05(at, tiles, to, code(out_dtype), ld, m, w.n, w.k, int(unit is not None), *(unit or _NO_UNIT), ranks,
+                                   flag, _stream(dev)), l)
+    return out
+
+
+def _product(x, w, out_dtype, unit, out) -> tuple:
     l, dev = _start()
     at, tiles = _check(dev, x, "x", torch.bfloat16), _check(dev, w.tiles, "w")
     if x.dim() != 2 or x.shape[1] != w.k:
@@ -160,9 +183,7 @@ def linear_rows(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.b
     flag = kernels._tcgen05_flag.get(dev)
     if flag is None:
         flag = kernels.tcgen05_error_flag(x.device)
-    check(l.gi_int4_linear(at, tiles, to, code(out_dtype), out.stride(0) if m > 1 else n, m, w.n, w.k, int(unit is not None),
-                           *(unit or _NO_UNIT), ranks, parts, flag.data_ptr(), _stream(dev)), l)
-    return out
+    return l, at, tiles, to, m, out.stride(0) if m > 1 else n, flag.data_ptr(), dev, out
 
 
 # -------------------------------------------------------------------------------------------------------------- cache

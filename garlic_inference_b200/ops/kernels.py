@@ -1400,7 +1400,7 @@ def check_bounded_waits(device) -> None:
         raise WaitRanOut(f"a tcgen05 kernel gave up a bounded wait or what it was asked for (code {code}: 11-13 product, 21-23 "
                          "prompt attention, 24 unmapped page, 25 shared memory that does not start on 1,024 bytes and nothing "
                          "written, 31-33 stream-K product, 34 a partial sum that was never announced, 41-43 decode attention, "
-                         "44 unmapped page, 61-63 experts' product, 71-74 float32 product, 81 delta rule, 91-94 recurrent gates, 95-97 product with a 4-bit weight)")
+                         "44 unmapped page, 61-63 experts' product, 71-74 float32 product, 81 delta rule, 91-94 recurrent gates, 95-99 product with a 4-bit weight)")
 
 
 def streamk_test_unanswered_flags(limit: int) -> None:

@@ -72,6 +72,12 @@ def linear_bound(x, w):
     return (32 + 2 * step.shape[1]) * 2 ** -24 * a + 2 ** -36 * x.double().abs().amax(1, keepdim=True) * sq.sum(1)[None]
 
 
+def wide_bound(x, w):
+    """What rounding each number of the weight to bfloat16 (2^-8 of it) and float32 sums of k products (2^-24 each) leave."""
+    a = x.double().abs() @ plain.values(*plain.unpack_weight(w), 128).abs().t()
+    return a * (2 ** -8 + (w.k + 16) * 2 ** -24)
+
+
 def random_weight(ops, g, n, k):
     codes = torch.randint(0, 16, (n, k), generator=g, device=DEV)
     groups = -(-k // 128)
@@ -94,6 +100,8 @@ def test_linear(ops, m, n, k, out_dtype):
     assert got.shape == (m, n) and got.dtype == out_dtype
     want = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
     bound = linear_bound(x, w) * 1.0 + (2 ** -8 if out_dtype == torch.bfloat16 else 2 ** -24) * want.abs()
+    if m > 16:                                               # the weight's numbers may be rounded to bfloat16: see wide_bound
+        bound += wide_bound(x, w)
     worst = ((got.double() - want).abs() / bound).max()
     assert float(worst) <= 1, float(worst)
     assert torch.equal(got, ops.linear(x, w, out_dtype))
@@ -121,7 +129,7 @@ def test_gated_units(ops, m, inter, k):
     w = random_weight(ops, g, 2 * inter, k)
     x = randn(g, m, k).to(torch.bfloat16)
     y = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
-    off = linear_bound(x, w)
+    off = linear_bound(x, w) + (wide_bound(x, w) if m > 16 else 0)
     gate, up = y[:, :inter], y[:, inter:]
     # |silu'| <= 1.1, |gelu'| <= 1.13
     for unit, act in ((kernels.glu_shape("silu"), lambda z: z * torch.sigmoid(z)),
@@ -165,6 +173,72 @@ def test_linear_of_many_rows_and_of_float32(ops, m, n, k):
         tol = 2 ** -8 * (silu * up).abs() + (1.1 * (off[:, :n // 2] + 2 ** -8 * gate.abs())) * (up.abs() + off[:, n // 2:]) \
             + (silu.abs() + 2 ** -8 * gate.abs()) * (off[:, n // 2:] + 2 ** -8 * up.abs()) + 2 ** -18 * (gate * up).abs() + 2 ** -30
         assert float(((got - silu * up).abs() / tol).max()) <= 1
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 8), (17, 128, 128), (32, 129, 136), (33, 16, 2000), (64, 300, 1024), (65, 777, 904), (128, 1000, 640), (200, 48, 512),
+                                   (385, 260, 256)])
+def test_products_on_tensor_memory(ops, m, n, k, out_dtype):
+    g = gen(m + n + k)
+    w = random_weight(ops, g, n, k)
+    x = (randn(g, m, k) * torch.exp(randn(g, k))).to(torch.bfloat16)
+    want = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    bound = wide_bound(x, w) + (2 ** -8 if out_dtype == torch.bfloat16 else 2 ** -24) * want.abs()
+    for ranks in range(0, min(8, -(-k // 128)) + 1):
+        out = torch.full((m, n + 5), 9.0, dtype=out_dtype, device=DEV)
+        got = ops.int4.linear_wide(x, w, out_dtype, out=out[:, 2:2 + n], ranks=ranks)
+        assert float(((got.double() - want).abs() / bound).max()) <= 1, ranks
+        assert torch.equal(got, ops.int4.linear_wide(x, w, out_dtype, ranks=ranks))
+        assert bool((out[:, :2] == 9).all()) and bool((out[:, 2 + n:] == 9).all())
+
+
+@pytest.mark.parametrize("m,inter,k", [(20, 16, 128), (40, 48, 520), (100, 208, 1024), (150, 64, 384), (64, 1000, 256)])
+def test_gated_units_on_tensor_memory(ops, m, inter, k):
+    from garlic_inference_b200.ops import kernels
+    g = gen(m + inter + k)
+    w = random_weight(ops, g, 2 * inter, k)
+    x = randn(g, m, k).to(torch.bfloat16)
+    y = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    off = wide_bound(x, w)
+    gate, up = y[:, :inter], y[:, inter:]
+    for unit, act in ((kernels.glu_shape("silu"), lambda z: z * torch.sigmoid(z)),
+                      (kernels.glu_shape("gelu_tanh", gate_max=1.0, up_limit=0.5, up_shift=1.0),
+                       lambda z: torch.nn.functional.gelu(z, approximate="tanh"))):
+        gg, uu = (gate, up) if unit[0] == 0 else (gate.clamp(max=1.0), up.clamp(-0.5, 0.5) + 1.0)
+        want = act(gg) * uu
+        bound = 2 ** -24 * want.abs() + 1.13 * off[:, :inter] * (uu.abs() + off[:, inter:]) + act(gg).abs() * off[:, inter:] + 2 ** -19 * (gg * uu).abs() + 2 ** -30
+        if inter % 16:                                       # halves that end inside a tile: `linear`'s business
+            with pytest.raises(ops.KernelError):
+                ops.int4.linear_wide(x, w, torch.float32, unit)
+            continue
+        for ranks in range(0, min(4, -(-k // 128)) + 1):
+            got = ops.int4.linear_wide(x, w, torch.float32, unit, ranks=ranks)
+            assert float(((got.double() - want).abs() / bound).max()) <= 1
+
+
+def test_rows_that_are_not_finite_stay_alone_on_tensor_memory(ops):
+    g = gen(19)
+    w = random_weight(ops, g, 150, 704)
+    x = randn(g, 40, 704).to(torch.bfloat16)
+    clean = ops.int4.linear_wide(x, w, torch.float32)
+    x[3, 5], x[20, 700], x[39, 0] = NAN, INF, -INF
+    got = ops.int4.linear_wide(x, w, torch.float32)
+    rest = [i for i in range(40) if i not in (3, 20, 39)]
+    assert torch.equal(got[rest], clean[rest]) and bool(torch.isnan(got[3]).all()) and not bool(torch.isfinite(got[[20, 39]]).any())
+    w.tiles[2, 1, 1024 + 4 * 5:1024 + 4 * 5 + 4] = torch.tensor([0xC0, 0x7F, 0xC0, 0x7F], dtype=torch.uint8, device=DEV)      # output 37, NaN group
+    got = ops.int4.linear_wide(clean.new_zeros(40, 704).to(torch.bfloat16) + 1, w, torch.float32)
+    assert bool(torch.isnan(got[:, 37]).all()) and int(torch.isnan(got).sum()) == 40
+
+
+def test_weights_with_more_inputs_than_16_rows_have_room_for(ops):
+    g = gen(23)
+    for k, m in ((120000, 16), (120001, 16), (120000, 20)):
+        w = random_weight(ops, g, 32, k)
+        x = randn(g, m, k).to(torch.bfloat16)
+        want = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+        bound = wide_bound(x, w) + 2 ** -24 * want.abs()
+        assert float(((ops.linear(x, w, torch.float32).double() - want).abs() / bound).max()) <= 1
+        assert ops.swiglu_product(x, w).shape == (m, 16)
 
 
 def test_rows_of_x_that_are_not_finite_or_huge_or_tiny(ops):
@@ -564,6 +638,9 @@ def test_refusals(ops):
         lambda: i4.linear_rows(y[:0], w), lambda: i4.linear_rows(torch.zeros(17, 128, dtype=torch.bfloat16, device=DEV), w), lambda: i4.linear_rows(y, w, torch.float16),
         lambda: i4.linear_rows(y, w, out=torch.zeros(3, 31, device=DEV, dtype=torch.bfloat16)),
         lambda: i4.linear_rows(y, w, out=torch.zeros(32, 3, device=DEV, dtype=torch.bfloat16).t()),
+        lambda: i4.linear_wide(y[:0], w), lambda: i4.linear_wide(y[:, :120].contiguous(), i4.quantize_weight(torch.zeros(8, 121, device=DEV))),
+        lambda: i4.linear_wide(torch.zeros(3, 121, dtype=torch.bfloat16, device=DEV), i4.quantize_weight(torch.zeros(8, 121, device=DEV))),
+        lambda: i4.linear_wide(y.flatten()[4:].as_strided((2, 128), (128, 1)), w), lambda: i4.linear_wide(y, w, ranks=2), lambda: i4.linear_wide(y, w, ranks=9),
         lambda: ops.swiglu_product(y, i4.quantize_weight(torch.zeros(33, 128, device=DEV))),
         lambda: i4.append(x, x[:, :1], *rows, table, pos, slot, status), lambda: i4.append(x, x.float(), *rows, table, pos, slot, status),
         lambda: i4.append(x.transpose(1, 2).contiguous().transpose(1, 2), x, *rows, table, pos, slot, status),
