@@ -266,7 +266,8 @@ static int launch_int4_wide(const CUtensorMap& x, const unsigned char* tiles, vo
     return gi_check_launch("gi_int4_linear_tcgen05");
 }
 
-// `ranks`: blocks that share the inputs (0: chosen here)
+// K: the inner size, rounded up to a multiple of 8 (x has zeros there; what the codes have counts for nothing).  `ranks`: blocks that share the
+// inputs (0: chosen here).
 extern "C" int gi_int4_linear_tcgen05(const void* x, const void* tiles, void* out, int out_dtype, long long ld_out, int M, int N, int K,
                                       int glu, int kind, float alpha, float gate_max, float up_limit, float up_shift, int ranks,
                                       int* error_flag, void* stream) {

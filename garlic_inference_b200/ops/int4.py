@@ -74,15 +74,14 @@ class Int4Rows:
             raise KernelError(f"codes {tuple(c.shape)} of {c.dtype} and steps {tuple(m.shape)} of {m.dtype} are no pages in 4 bits: "
                               "dense uint8 [pages, heads, page size, d / 2] and bfloat16 [pages, heads, page size, d / 64, 2], "
                               "d a multiple of 64")
+        self.shape = (*shape[:3], shape[3] * 2)              # [pages, heads, page size, d], as a pool of numbers would have it
+        self.index = c.get_device()                          # -1: not on a GPU
+        if m.get_device() != self.index:
+            raise KernelError(f"codes on {c.device} and steps on {m.device}")
 
     @property
     def head_dim(self) -> int:
-        return self.codes.shape[3] * 2
-
-    @property
-    def shape(self) -> tuple:
-        """[pages, heads, page size, d], as a pool of numbers would have it"""
-        return (*self.codes.shape[:3], self.head_dim)
+        return self.shape[3]
 
     @staticmethod
     def zeros(pages: int, heads: int, page_size: int, head_dim: int, device) -> "Int4Rows":
@@ -147,7 +146,7 @@ def linear_rows(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.b
     """x W^T for 1 to 16 rows of bfloat16 x, reading the weight's codes once; with `unit` (a `kernels.glu_shape` tuple) the gated
     unit of the weight's first half of outputs (a multiple of 16) and its last.  `out` may be columns of a wider matrix.
     `ranks`, `parts`: blocks that share the inputs, and parts of a block's share that its warps take (0: chosen by the entry point)."""
-    l, at, tiles, to, m, ld, flag, dev, out = _product(x, w, out_dtype, unit, out)
+    l, at, tiles, to, m, ld, flag, dev, out = _product(x, w, out_dtype, unit, out, w.k)
     check(l.gi_int4_linear(at, tiles, to, code(out_dtype), ld, m, w.n, w.k, int(unit is not None), *(unit or _NO_UNIT), ranks, parts,
                            flag, _stream(dev)), l)
     return out
@@ -160,20 +159,22 @@ def linear_rows_takes(rows: int, w: Int4Weight, gated: bool) -> bool:
 
 def linear_wide(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.bfloat16, unit: Optional[tuple] = None,
                 out: Optional[torch.Tensor] = None, ranks: int = 0) -> torch.Tensor:
-    """`linear_rows` for any number of rows (the inner size a multiple of 8, x on 16 bytes): the numbers that the codes stand for are
+    """`linear_rows` for any number of rows (their length a multiple of 8, x on 16 bytes; for an odd inner size x has zeros behind it, up to
+    the next multiple of 8): the numbers that the codes stand for are
     rounded to bfloat16 for the tensor cores, once for 32 or 64 rows.  `ranks`: blocks that share the inputs (0: chosen by the
     entry point)."""
-    l, at, tiles, to, m, ld, flag, dev, out = _product(x, w, out_dtype, unit, out)
-    check(l.gi_int4_linear_tcgen05(at, tiles, to, code(out_dtype), ld, m, w.n, w.k, int(unit is not None), *(unit or _NO_UNIT), ranks,
+    k = -(-w.k // 8) * 8
+    l, at, tiles, to, m, ld, flag, dev, out = _product(x, w, out_dtype, unit, out, k)
+    check(l.gi_int4_linear_tcgen05(at, tiles, to, code(out_dtype), ld, m, w.n, k, int(unit is not None), *(unit or _NO_UNIT), ranks,
                                    flag, _stream(dev)), l)
     return out
 
 
-def _product(x, w, out_dtype, unit, out) -> tuple:
+def _product(x, w, out_dtype, unit, out, k: int) -> tuple:
     l, dev = _start()
     at, tiles = _check(dev, x, "x", torch.bfloat16), _check(dev, w.tiles, "w")
-    if x.dim() != 2 or x.shape[1] != w.k:
-        raise KernelError(f"x {tuple(x.shape)} does not fit a weight {w.shape} ([out, in])")
+    if x.dim() != 2 or x.shape[1] != k:
+        raise KernelError(f"x {tuple(x.shape)} does not fit a weight {w.shape} ([out, in]): rows of {k}")
     m, n = x.shape[0], w.n // 2 if unit is not None else w.n
     if out is None:
         out = x.new_empty((m, n), dtype=out_dtype)
@@ -192,10 +193,11 @@ def _pools(dev: int, k_rows: Int4Rows, v_rows: Int4Rows) -> tuple:
     if not isinstance(k_rows, Int4Rows) or not isinstance(v_rows, Int4Rows):
         raise KernelError(f"pages in 4 bits are an Int4Rows, not {type(k_rows).__name__} and {type(v_rows).__name__}")
     shape = k_rows.shape
-    if v_rows is not k_rows and shape != v_rows.shape:
+    if shape != v_rows.shape:
         raise KernelError(f"pages of keys {shape} and of values {v_rows.shape} differ")
-    return shape, (_check(dev, k_rows.codes, "k_rows"), _check(dev, k_rows.meta, "k_rows"), _check(dev, v_rows.codes, "v_rows"),
-                   _check(dev, v_rows.meta, "v_rows"))
+    if k_rows.index != dev or v_rows.index != dev:
+        raise KernelError(f"pages on {k_rows.codes.device} and {v_rows.codes.device}; the kernels run on the current GPU, cuda:{dev}")
+    return shape, (k_rows.codes.data_ptr(), k_rows.meta.data_ptr(), v_rows.codes.data_ptr(), v_rows.meta.data_ptr())
 
 
 def _table(dev: int, block_table: torch.Tensor) -> tuple:

@@ -79,8 +79,7 @@ INT4_SURE_INPUTS = 32768          # up to here the kernel for 16 rows has room f
 def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Optional[tuple] = None,
           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The product with a weight in 4 bits, or (`unit`) the gated unit of its halves.  bfloat16: up to 16 rows `int4.linear_rows`
-    (17 rows of 4,096 x 4,096: 15 us in two pieces, 10 in one of the next), up to INT4_CODES_MAX_ROWS `int4.linear_wide`; rows of an odd
-    length or start in pieces of 16.  More, or float32: the weight is made wide, some outputs at a time, for the products that
+    (17 rows of 4,096 x 4,096: 15 us in two pieces, 10 in one of the next), up to INT4_CODES_MAX_ROWS `int4.linear_wide`.  More, or float32: the weight is made wide, some outputs at a time, for the products that
     `linear` has for that type.  Beyond 16 rows bfloat16 rounds each number of the weight once on the way (by half a step of
     2^-8, a hundredth of what 4 bits leave of it)."""
     if x.dim() != 2 or x.shape[1] != w.k:
@@ -89,8 +88,7 @@ def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Opt
         raise KernelError(f"linear: {w.n} outputs cannot be a gate and an up half")
     m, n = x.shape[0], w.n if unit is None else w.n // 2
     fits = x.dtype is torch.bfloat16 and (unit is None or n % 16 == 0)
-    rows = fits and (w.k <= INT4_SURE_INPUTS or int4.linear_rows_takes(min(m, int4.LINEAR_MAX_ROWS), w, unit is not None))
-    if rows and 0 < m <= int4.LINEAR_MAX_ROWS:
+    if fits and 0 < m <= int4.LINEAR_MAX_ROWS and (w.k <= INT4_SURE_INPUTS or int4.linear_rows_takes(m, w, unit is not None)):
         return int4.linear_rows(x, w, out_dtype, unit, out)
     aligned = w.k % 8 == 0 and x.data_ptr() % 16 == 0
     if fits and aligned and 0 < m <= INT4_CODES_MAX_ROWS:
@@ -102,13 +100,12 @@ def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Opt
     if unit is not None and not fits:
         return kernels.glu(_int4(x, w, torch.float32), unit, out=out) if out_dtype == torch.float32 else \
             _narrow(kernels.glu(_int4(x, w, torch.float32), unit), out)
-    if rows and not aligned:
-        for r in range(0, m, int4.LINEAR_MAX_ROWS):
-            int4.linear_rows(x[r:r + int4.LINEAR_MAX_ROWS], w, out_dtype, unit, out[r:r + int4.LINEAR_MAX_ROWS])
+    if fits and not aligned:                                 # rows of an odd length or start: a copy that is aligned
+        even = x.new_zeros((m, -(-w.k // 8) * 8))
+        even[:, :w.k].copy_(x)
+        for r in range(0, m, INT4_CODES_MAX_ROWS):
+            int4.linear_wide(even[r:r + INT4_CODES_MAX_ROWS], w, out_dtype, unit, out[r:r + INT4_CODES_MAX_ROWS])
         return out
-    if fits and not aligned:                                 # too long for pieces of 16 rows
-        y = _int4(kernels.cast(x, torch.float32), w, torch.float32)
-        return _narrow(y if unit is None else kernels.glu(y, unit), out)
     if unit is not None:
         return kernels.gemm_tcgen05_glu_bf16(x, int4.dequantize_weight(w), unit, out=out)
     per = max(256, INT4_WIDE_BYTES // (w.k * x.element_size()) // 256 * 256)

@@ -192,6 +192,24 @@ def test_products_on_tensor_memory(ops, m, n, k, out_dtype):
         assert bool((out[:, :2] == 9).all()) and bool((out[:, 2 + n:] == 9).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(17, 40, 65), (111, 78, 65), (400, 32, 333), (30, 300, 1021)])
+def test_rows_of_odd_lengths_and_starts(ops, m, n, k):
+    g = gen(m + n + k)
+    w = random_weight(ops, g, n, k)
+    filled = plain.pack_weight(torch.nn.functional.pad(plain.unpack_weight(w)[0], (0, -k % 128), value=15.0), *plain.unpack_weight(w)[1:])
+    w = ops.int4.Int4Weight(filled, n, k)                    # beyond k the codes are not zeros
+    x = randn(g, m, k).to(torch.bfloat16)
+    want = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    bound = wide_bound(x, w) + 2 ** -24 * want.abs()
+    got = ops.linear(x, w, torch.float32)
+    assert float(((got.double() - want).abs() / bound).max()) <= 1
+    flat = torch.zeros(m * 128 + 3, dtype=torch.bfloat16, device=DEV)
+    odd = flat[3:].view(m, 128)                              # even rows that start on 6 bytes
+    odd.copy_(randn(g, m, 128))
+    v = random_weight(ops, g, n, 128)
+    assert torch.equal(ops.linear(odd, v, torch.float32), ops.linear(odd.clone(), v, torch.float32))
+
+
 @pytest.mark.parametrize("m,inter,k", [(20, 16, 128), (40, 48, 520), (100, 208, 1024), (150, 64, 384), (64, 1000, 256)])
 def test_gated_units_on_tensor_memory(ops, m, inter, k):
     from garlic_inference_b200.ops import kernels
@@ -639,6 +657,7 @@ def test_refusals(ops):
         lambda: i4.linear_rows(y, w, out=torch.zeros(3, 31, device=DEV, dtype=torch.bfloat16)),
         lambda: i4.linear_rows(y, w, out=torch.zeros(32, 3, device=DEV, dtype=torch.bfloat16).t()),
         lambda: i4.linear_wide(y[:0], w), lambda: i4.linear_wide(y[:, :120].contiguous(), i4.quantize_weight(torch.zeros(8, 121, device=DEV))),
+        lambda: i4.linear_wide(torch.zeros(3, 136, dtype=torch.bfloat16, device=DEV), i4.quantize_weight(torch.zeros(8, 121, device=DEV))),
         lambda: i4.linear_wide(torch.zeros(3, 121, dtype=torch.bfloat16, device=DEV), i4.quantize_weight(torch.zeros(8, 121, device=DEV))),
         lambda: i4.linear_wide(y.flatten()[4:].as_strided((2, 128), (128, 1)), w), lambda: i4.linear_wide(y, w, ranks=2), lambda: i4.linear_wide(y, w, ranks=9),
         lambda: ops.swiglu_product(y, i4.quantize_weight(torch.zeros(33, 128, device=DEV))),
