@@ -79,6 +79,56 @@ __device__ __forceinline__ void i4a_matrix_trans(uint32_t (&r)[4], uint32_t at) 
 #define I4A_SLACK 8.f              // a score may lie this far (in powers of two) above the reference
 #define I4A_STEP_TOP 6             // the largest step so far is scaled to [2^6, 2^7): times 2^8 it stays below f16's largest number
 
+// Where the warps of a block meet: [warp][column][D + 4] sums, [warp][column] maximum and weight, then the block's own maximum and weight of a
+// column; its sums lie in the first warp's place.
+template <int D, int NT> struct Int4Meet {
+    static constexpr int COLS = 8 * NT, LD = D + 4, ML = I4A_WARPS * COLS * LD, OWN = ML + I4A_WARPS * COLS * 2, FLOATS = OWN + COLS * 2;
+};
+__device__ __forceinline__ uint32_t i4a_remote(const void* p, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void i4a_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Slices whose blocks are a cluster: each adds up its share of the columns' numbers, in the order of the slices, out of the others' shared memory
+template <int D, int NT, typename Row>
+__device__ __forceinline__ void i4a_join(bf16* __restrict__ out, int n_cols, int split, int n_splits, Row result_row) {
+    typedef Int4Meet<D, NT> M;
+    extern __shared__ __align__(16) unsigned char i4a_smem[];
+    const float* const meet = reinterpret_cast<const float*>(i4a_smem);
+    __syncwarp();
+    i4a_cluster_sync();                                                        // the blocks' sums are there
+    const int items = n_cols * (D / 4);
+#pragma unroll 1
+    for (int i = items * split / n_splits + threadIdx.x; i < items * (split + 1) / n_splits; i += I4A_THREADS) {
+        const int cc = i / (D / 4), d4 = (i % (D / 4)) * 4;
+        float m[8], l[8], most = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            m[r] = -INFINITY;
+            if (r < n_splits) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[r]), "=f"(l[r]) : "r"(i4a_remote(meet + M::OWN + cc * 2, r)) : "memory");
+            most = fmaxf(most, m[r]);
+        }
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float L = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            if (m[r] == -INFINITY) continue;                                   // no such slice, or it saw no key
+            float4 v;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(i4a_remote(meet + cc * M::LD + d4, r)) : "memory");
+            const float f = i4a_exp2(m[r] - most);
+            acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+            L = fmaf(f, l[r], L);
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        store4_act(out + result_row(cc) * D + d4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    }
+    __syncwarp();
+    i4a_cluster_sync();                                                        // the others have read this block's
+}
+
 // Columns col0 .. of a run (rows row0 .. row0 + rows - 1 of q, at positions pos0 ..) over slice `split` of its keys, by a whole block.
 template <int D, int NT>
 __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const Int4Cache& cache, const int* __restrict__ table, bf16* __restrict__ out,
@@ -113,7 +163,10 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
     const int per = max((n_chunks + n_splits - 1) / n_splits, 2 * I4A_WARPS);   // fewer chunks do not pay for a block's start
     const int c_begin = chunk0 + split * per, c_end = chunk0 + min(n_chunks, (split + 1) * per);
     if (!ok || c_begin >= c_end) {
-        if (n_splits > 1) {
+        if (n_splits > 1 && !part_ml) {
+            if (threadIdx.x < n_cols) *reinterpret_cast<float2*>(reinterpret_cast<float*>(i4a_smem) + Int4Meet<D, NT>::OWN + threadIdx.x * 2) = make_float2(-INFINITY, 0.f);
+            i4a_join<D, NT>(out, n_cols, split, n_splits, result_row);
+        } else if (n_splits > 1) {
             for (int i = threadIdx.x; i < n_cols; i += I4A_THREADS) {
                 float* ml = part_ml + (result_row(i) * n_splits + split) * 2;
                 ml[0] = -INFINITY, ml[1] = 0.f;
@@ -130,17 +183,19 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
     constexpr int ROWS = 32 / C::PIECES;                                       // rows that a copy of the warp takes
     const int my_r = lane / C::PIECES, my_dst = i4a_piece<D>(my_r, lane % C::PIECES);      // of the first copy; others lie ROWS rows on
     int next = c_begin + warp, slot_in = 0;
+    int page_next = whole >= 0 && next < c_end ? __ldg(bt + (next * I4A_KEYS >> whole)) : -1;      // asked for one chunk ahead
     bool unmapped = false;
     auto issue = [&]() {
         if (next < c_end) {
             const int j0 = next * I4A_KEYS, here = hi - j0 + 1;                // rows of the chunk that exist
             unsigned char* dst = ring + slot_in * C::BYTES;
-            if (whole) {                                                       // a chunk lies in one page: its rows are contiguous
-                const int lp = j0 / page_size, page = __ldg(bt + lp);
+            if (whole >= 0) {                                                  // a chunk lies in one page: its rows are contiguous
+                const int page = page_next;
+                if (next + I4A_WARPS < c_end) page_next = __ldg(bt + (j0 + I4A_WARPS * I4A_KEYS >> whole));
                 const bool mapped = page >= 0 && page < n_pages;
                 unmapped |= !mapped;
                 const int rows_here = mapped ? here : 0;
-                const size_t row = mapped ? ((size_t)page * n_kv + kvh) * page_size + (j0 - lp * page_size) : 0;
+                const size_t row = mapped ? ((size_t)page * n_kv + kvh) * page_size + (j0 & (page_size - 1)) : 0;
                 const unsigned char *k = cache.k + row * C::ROW + lane * 16, *v = cache.v + row * C::ROW + lane * 16;
                 const unsigned char *km = cache.km + (row + lane) * (G * 4), *vm = cache.vm + (row + lane) * (G * 4);
                 unsigned char *to = dst + my_dst, *mto = dst + 2 * C::CODES + lane * G * 4;
@@ -417,12 +472,13 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
     }
     if (unmapped) atomicExch(status, 5);
 
-    // ---- the warps meet: [warp][column][D + 4] outputs, then [warp][column] maximum and sum
+    // ---- the warps meet
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     __syncthreads();
-    constexpr int LD = D + 4;
+    typedef Int4Meet<D, NT> M;
+    constexpr int LD = M::LD;
     float* so = reinterpret_cast<float*>(i4a_smem);
-    float* sml = so + I4A_WARPS * COLS * LD;
+    float* sml = so + M::ML;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -455,16 +511,16 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
 #pragma unroll 1
     for (int i = threadIdx.x; i < n_cols * (D / 4); i += I4A_THREADS) {
         const int cc = i / (D / 4), d4 = (i % (D / 4)) * 4;
-        float M = -INFINITY;
+        float most = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < I4A_WARPS; ++w) M = fmaxf(M, sml[(w * COLS + cc) * 2]);
+        for (int w = 0; w < I4A_WARPS; ++w) most = fmaxf(most, sml[(w * COLS + cc) * 2]);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float L = 0.f;
 #pragma unroll 1
         for (int w = 0; w < I4A_WARPS; ++w) {
             const float mw = sml[(w * COLS + cc) * 2];
             if (mw == -INFINITY) continue;                                     // saw no key
-            const float f = i4a_exp2(mw - M);
+            const float f = i4a_exp2(mw - most);
             const float4 v = *reinterpret_cast<const float4*>(so + (w * COLS + cc) * LD + d4);
             acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
             L = fmaf(f, sml[(w * COLS + cc) * 2 + 1], L);
@@ -473,14 +529,15 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
         if (n_splits == 1) {
             const float inv = L == 0.f ? 0.f : 1.f / L;
             store4_act(out + row * D + d4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        } else if (!part_ml) {
+            *reinterpret_cast<float4*>(so + cc * LD + d4) = acc;               // the first warp's, read by this thread alone
+            if (d4 == 0) *reinterpret_cast<float2*>(so + M::OWN + cc * 2) = make_float2(most, L);
         } else {
             *reinterpret_cast<float4*>(part_o + (row * n_splits + split) * D + d4) = acc;
-            if (d4 == 0) {
-                part_ml[(row * n_splits + split) * 2] = M;
-                part_ml[(row * n_splits + split) * 2 + 1] = L == L ? L : 1.f;       // then the sums are NaN, and stay so
-            }
+            if (d4 == 0) *reinterpret_cast<float2*>(part_ml + (row * n_splits + split) * 2) = make_float2(most, L);
         }
     }
+    if (n_splits > 1 && !part_ml) i4a_join<D, NT>(out, n_cols, split, n_splits, result_row);
 }
 
 // The run of a block: slot, first row, rows, position of the first row; without runs, run i is the single token i.  False: there is none.
@@ -573,7 +630,8 @@ int4_attention_join_kernel(const float* __restrict__ part_o, const float* __rest
 }
 
 // runs [n_runs, 4], or none: every token is a sequence of its own.  With n_splits > 1 the
-// slices lie in part_o [tokens, n_q, n_splits, d] and part_ml [tokens, n_q, n_splits, 2], and a second kernel joins them.
+// up to 8 slices without part_o and part_ml are a cluster and join
+// themselves; otherwise they lie in part_o [tokens, n_q, n_splits, d] and part_ml [tokens, n_q, n_splits, 2], and a second kernel joins them.
 extern "C" int gi_int4_attention(const void* q, const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta,
                                  const int* table, const int* runs, int n_runs, int n_rows, const int* tok_pos, const int* tok_slot,
                                  void* out, float* part_o, float* part_ml, int n_q, int n_kv, int d, int n_slots, int max_pages,
@@ -583,12 +641,14 @@ extern "C" int gi_int4_attention(const void* q, const void* k_codes, const void*
     GI_REQUIRE(n_runs >= 0 && n_runs <= 65535 && n_rows >= (runs ? 0 : n_runs) && n_rows <= 1 << 24,
                "gi_int4_attention: %d runs of %d rows", n_runs, n_rows);
     GI_REQUIRE(page_size > 0 && max_pages > 0 && n_slots > 0 && window >= 0, "gi_int4_attention: page and table sizes must be positive");
-    GI_REQUIRE(n_splits >= 1 && n_splits <= 256 && (n_splits == 1 || (part_o && part_ml)), "gi_int4_attention: %d slices", n_splits);
+    GI_REQUIRE(n_splits >= 1 && n_splits <= 256 && (part_o != nullptr) == (part_ml != nullptr) && (n_splits <= 8 || part_o), "gi_int4_attention: %d slices", n_splits);
     GI_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_meta % 8 == 0 &&
                (uintptr_t)v_meta % 8 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)part_o % 16 == 0 && (uintptr_t)runs % 16 == 0,
                "gi_int4_attention: operands must start on 16 bytes");
     if (n_runs == 0 || n_rows == 0) return 0;
     const Int4Cache cache = {(const unsigned char*)k_codes, (const unsigned char*)v_codes, (const unsigned char*)k_meta, (const unsigned char*)v_meta};
+    int whole = -1;                                                            // pages of 2^whole rows, chunks within a page; -1: any other
+    for (int i = 5; i < 31; ++i) if (page_size == 1 << i) whole = i;
     const int group = n_q / n_kv;
     const long long cols = ((long long)n_rows * group + n_runs - 1) / n_runs;   // of a run, on average
     const int nt = cols > 8 ? 2 : 1;
@@ -597,19 +657,27 @@ extern "C" int gi_int4_attention(const void* q, const void* k_codes, const void*
 #define GI_I4A(DD, NN)                                                                                                               \
     {                                                                                                                                \
         size_t smem = (size_t)I4A_WARPS * I4A_STAGES * Int4Chunk<DD>::BYTES;                                                         \
-        const size_t meet = (size_t)I4A_WARPS * 8 * NN * (DD + 4 + 2) * 4;                                                           \
+        const size_t meet = (size_t)Int4Meet<DD, NN>::FLOATS * 4;                                                                     \
         if (meet > smem) smem = meet;                                                                                                \
         if (int rc = gi_reserve_smem((const void*)int4_attention_kernel<DD, NN>, smem, "gi_int4_attention")) return rc;              \
-        gi_launch(int4_attention_kernel<DD, NN>, dim3((unsigned)(col_tiles * n_splits), n_kv, n_runs), dim3(I4A_THREADS), smem,      \
-                  (cudaStream_t)stream, (const bf16*)q, cache, table, (const int4*)runs, tok_pos, tok_slot, (bf16*)out, part_o,      \
-                  part_ml, n_rows, n_q, n_kv, n_slots, max_pages, page_size, n_pages, window, scale * I4A_LOG2E, n_splits, group,    \
-                  page_size % I4A_KEYS == 0, status);                                                                                \
+        cudaLaunchConfig_t cfg = {};                                                                                                 \
+        cfg.gridDim = dim3((unsigned)(col_tiles * n_splits), n_kv, n_runs), cfg.blockDim = dim3(I4A_THREADS);                        \
+        cfg.dynamicSmemBytes = smem, cfg.stream = (cudaStream_t)stream;                                                              \
+        cudaLaunchAttribute attr[2];                                                                                                 \
+        attr[0].id = cudaLaunchAttributeClusterDimension;                                                                            \
+        attr[0].val.clusterDim.x = part_o ? 1 : n_splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;                   \
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;                                                             \
+        attr[1].val.programmaticStreamSerializationAllowed = 1;                                                                      \
+        cfg.attrs = attr, cfg.numAttrs = gi_pdl_enabled() ? 2 : 1;                                                                   \
+        cudaLaunchKernelEx(&cfg, int4_attention_kernel<DD, NN>, (const bf16*)q, cache, table, (const int4*)runs, tok_pos, tok_slot,  \
+                           (bf16*)out, part_o, part_ml, n_rows, n_q, n_kv, n_slots, max_pages, page_size, n_pages, window,           \
+                           scale * I4A_LOG2E, n_splits, group, whole, status);                                                       \
     }
     if (d == 64) { if (nt == 1) GI_I4A(64, 1) else GI_I4A(64, 2) }
     else { if (nt == 1) GI_I4A(128, 1) else GI_I4A(128, 2) }
 #undef GI_I4A
     if (int rc = gi_check_launch("gi_int4_attention")) return rc;
-    if (n_splits == 1) return 0;
+    if (!part_o || n_splits == 1) return 0;
     const int per = runs ? (n_rows + n_runs - 1) / n_runs : 1;
     const dim3 joins(n_q, per < 65535 ? per : 65535, n_runs);
     if (d == 64) gi_launch(int4_attention_join_kernel<64>, joins, dim3(128), 0, (cudaStream_t)stream, part_o, part_ml, (const int4*)runs, (bf16*)out, n_rows, n_q, n_splits);

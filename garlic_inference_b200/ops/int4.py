@@ -26,6 +26,8 @@ GROUP_WEIGHT = 128          # inputs that share a step
 GROUP_ROWS = 64             # numbers of a head that share a step
 TILE_BYTES = 1088           # 16 outputs x 128 inputs: 1,024 bytes of codes, then (step, low) of the 16 outputs
 _NO_UNIT = (0, 1.0, float("inf"), float("inf"), 0.0)
+MAX_CLUSTER = 8             # slices of the keys that join themselves
+PLACES = 592                # blocks of the attention kernel for up to 8 columns that 148 SMs hold; 444 for up to 16
 LINEAR_MAX_ROWS = 16        # rows of x that the kernel reading a weight's codes takes
 
 
@@ -297,31 +299,36 @@ def _queries(dev: int, q: torch.Tensor, shape: tuple) -> int:
 
 
 def _few(l, dev: int, q: torch.Tensor, at: int, shape: tuple, pools: tuple, table: tuple, runs, n_runs: int, pos, slot, scale: float,
-         window: int, status: torch.Tensor, out: torch.Tensor, n_splits: int) -> torch.Tensor:
+         window: int, status: torch.Tensor, out: torch.Tensor, n_splits: int, blocks: int) -> torch.Tensor:
+    """`blocks`: of the kernel, without slices.  Up to 8 slices are a cluster and join themselves where all blocks have a place at
+    once (8 runs of 2,048 keys, 6 slices: 12.7 us, 14.0 with a second kernel); where they wait for places, a cluster waits for
+    as many as it has blocks (64 runs of 500 keys, 4 slices: 35.7 against 24.3)."""
     n_pages, heads, page_size, d = shape
     n, n_q, _ = q.shape
     part_o = part_ml = None
-    if n_splits > 1:                                         # one workspace: the slices' sums, then their maxima and weights
+    if n_splits > MAX_CLUSTER or n_splits > 1 and n_splits * blocks > PLACES:      # one workspace: the slices' sums, then their maxima and weights
         room = q.new_empty((n * n_q * n_splits * (d + 2),), dtype=torch.float32)
         part_o = room.data_ptr()
         part_ml = part_o + n * n_q * n_splits * d * 4
+        kernels.counters.launches += 1                       # the kernel that joins the slices
     check(l.gi_int4_attention(at, *pools, table[0], runs, n_runs, n, pos, slot, out.data_ptr(), part_o, part_ml, n_q, heads, d, table[1],
                               table[2], page_size, n_pages, window, scale, n_splits, _status(dev, status), _stream(dev)), l)
-    if n_splits > 1:
-        kernels.counters.launches += 1                       # the kernel that joins the slices
     return out
 
 
-def decode_splits(n_runs: int, heads: int, keys: int, slots: int = 592, uneven: int = 1024) -> int:
-    """Slices of the keys per (run, key/value head): as many as fill the 148 SMs with 4 blocks each (`slots`), a run of many keys among
-    others one for every `uneven` keys up to 8 (lengths may differ, and are not known here), none of fewer than 256 keys.
-    `keys`: what the table's width or the window lets a run see.  Heads of 128, in us by slices:
-      8 runs of 2,048 keys, 8 heads    1: 25.0   4: 13.8   9: 13.7   14: 13.9   74: 21.9        (9 taken)
-      1 run of 131,000 keys, 8 heads   37: 51.1   55: 45.8   74: 43.0   111: 51.9               (74)
-      48 runs of 1 .. 8,000, 8 heads   1: 99   4: 64.4   7: 61.2   9: 62.9   14: 68.7           (7)
-      64 runs of 500 keys, 8 heads     1: 16.2   4: 23.7   9: 27.7                              (1)
-      1 run of 100 keys, 8 heads       1: 4.4   4: 7.0   74: 9.1                                (1)"""
-    return max(1, min(max(slots // max(1, n_runs * heads), min(8, keys // uneven)), -(-keys // 256), 74))
+def decode_splits(n_runs: int, heads: int, keys: int, places: int = PLACES, uneven: int = 1024) -> int:
+    """Slices of the keys per (run, key/value head): as many as fill the 148 SMs with 4 blocks each (`places`), a run of many keys among
+    others one for every `uneven` keys up to 8 (lengths may differ, and are not known here), none of fewer than 256 keys, 8
+    instead of a few more (they join themselves).  `keys`: what the table's width or the window lets a run see.  Heads of 128, in us
+    by slices:
+      8 runs of 2,048 keys, 8 heads    1: 24.3   4: 13.4   6: 12.7   8: 13.6   14: 14.2   74: 23.0      (8 taken)
+      1 run of 131,000 keys, 8 heads   37: 51.1   55: 45.8   74: 43.0   111: 51.9                       (74)
+      1 run of 4,000 keys, 8 heads     1: 40.0   4: 14.3   8: 9.7   16: 8.4                             (16)
+      48 runs of 1 .. 8,000, 8 heads   1: 93.8   4: 64.5   7: 60.9   9: 63.1   14: 69.3                 (7)
+      64 runs of 500 keys, 8 heads     1: 16.4   2: 22.3   9: 29.0                                      (1)
+      1 run of 100 keys, 8 heads       1: 4.9   4: 6.1   74: 10.0                                       (1)"""
+    n = max(1, min(max(places // max(1, n_runs * heads), min(8, keys // uneven)), -(-keys // 256), 74))
+    return 8 if 8 < n < 12 else n
 
 
 # Up to how many columns (tokens x query heads of a key/value head) of a run, on average, `attention_prompt` reads the codes.  12 runs of
@@ -346,7 +353,9 @@ def attention_decode(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
     if not n_splits:
         keys = table[2] * shape[2]
         n_splits = decode_splits(n, shape[1], min(keys, window) if window else keys)
-    return _few(l, dev, q, at, shape, pools, table, None, n, pos, slot, scale, window, status, q.new_empty((n, n_q * d)), n_splits)
+    group = n_q // shape[1]
+    return _few(l, dev, q, at, shape, pools, table, None, n, pos, slot, scale, window, status, q.new_empty((n, n_q * d)), n_splits,
+                n * shape[1] * (1 if group <= 8 else -(-group // 16)))
 
 
 def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor, runs: torch.Tensor,
@@ -371,9 +380,9 @@ def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
         return q.new_zeros((n, n_q * d))
     columns = -(-n * (n_q // heads) // n_runs)
     if columns <= FEW_COLUMNS:
-        tiles, slots = (1, 592) if columns <= 8 else (-(-columns // 16), 444)      # wider columns: 3 blocks an SM
+        tiles, places = (1, PLACES) if columns <= 8 else (-(-columns // 16), 444)
         return _few(l, dev, q, at, shape, pools, table, runs_at, n_runs, None, None, scale, window, status, q.new_zeros((n, n_q * d)),
-                    decode_splits(n_runs * tiles, heads, 64 * n_blocks // n_runs, slots, 2048))
+                    decode_splits(n_runs * tiles, heads, 64 * n_blocks // n_runs, places, 2048), n_runs * heads * tiles)
     max_blocks = -(-width * page_size // 64)
     pages = q.new_empty((2, n_blocks, heads, 64, d))
     new_table = block_table.new_full((n_slots, max_blocks), -1)

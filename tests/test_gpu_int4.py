@@ -421,6 +421,23 @@ def test_decode(ops, heads, kv, d, page, lengths, window, splits):
     assert torch.equal(got, ops.int4.attention_decode(q, k_rows, v_rows, table, pos, slot, d ** -0.5, window, status, n_splits=splits))
 
 
+@pytest.mark.parametrize("splits", [2, 5, 8, 9, 12, 74, 256])
+@pytest.mark.parametrize("heads,kv,d,n,least,most", [(4, 1, 128, 5, 1, 700), (16, 8, 64, 60, 1, 400), (6, 6, 128, 3, 800, 1000)])
+def test_slices_join_in_either_way(ops, heads, kv, d, n, least, most, splits):
+    """Few blocks join in clusters, many (60 sequences of 8 heads) and more than 8 slices by a second kernel; most slices are empty."""
+    rnd = random.Random(n)
+    lengths = [rnd.randint(least, most) for _ in range(n)]
+    g = gen(n + splits)
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, lengths, kv, d, 64)
+    q = randn(g, n, heads, d).to(torch.bfloat16)
+    pos, slot = torch.tensor(lengths, dtype=torch.int32, device=DEV) - 1, torch.arange(n, dtype=torch.int32, device=DEV)
+    slot[n // 2] = -1
+    got = ops.int4.attention_decode(q, k_rows, v_rows, table, pos, slot, d ** -0.5, 0, status, n_splits=splits)
+    spans = [(i, i, 1, lengths[i] - 1) for i in range(n) if i != n // 2]
+    check_attention(got, *plain.attention(q, k_rows, v_rows, table, spans, d ** -0.5, 0))
+    assert int(status) == 0 and not bool(got[n // 2].any())
+
+
 def runs_and_blocks(spans, window):
     runs = sorted(((s, r + a, min(128, n - a), p + a) for s, r, n, p in spans for a in range(0, n, 128)), key=lambda t: -(t[2] + t[3]))
     blocks = [(s, b) for s, r, n, p in spans for b in range((max(0, p - window + 1) if window else 0) // 64, -(-(p + n) // 64))]
