@@ -3,20 +3,21 @@
 //
 // A block takes 128 outputs (with a gated unit 64 of the gate's and the 64 of the up half that meet them), a block of rows of x and, as
 // one of the blocks of a cluster, a slice of K.  For each group of 128 inputs of its slice:
-//   warp 8       asks for codes and steps, four groups of a row of tiles a copy, into a ring of shared memory (a copy costs its warp 90 cycles:
-//                pieces of 512 bytes came at 1,100 ns a group, five times too late).  W is nobody's output: in
-//                a recorded step the ring fills before the kernel waits for the one that makes x.
+//   warp 8       asks for codes and steps, two groups of a row of tiles a copy, into a ring of shared memory (a copy costs 90 cycles: in pieces
+//                of 512 bytes W came at 1.1 us a group).  W is nobody's output: in a recorded step the ring fills before the kernel
+//                waits for the one that makes x.
 //   warps 0-7    make it wide, two groups of four warps in turn: step * q + low in bfloat16 (one rounding, by fma), a thread an output, into
-//                tensor memory: the 128-row operand never passes through shared memory again (32 KB a group, a
-//                quarter of the time that W takes to arrive).
+//                tensor memory: the 128-row operand never passes through shared memory again, 32 KB a group.
 //   warp 9       brings the rows of x.
 //   warp 10      products, 128 x BN x 16, accumulated in float32 in tensor memory over the whole slice.
 // Then the sums go to shared memory, the blocks of the cluster add up a share of the rows each, in the order of the ranks (the same bits from
 // run to run), and write.
 //
-// Bound by reading W (8,704 bytes a group: 366 cycles of an SM's share of the memory rate) next to unpacking it: 17 instructions for 8
-// numbers, 1,150 of a warp a group (two of them keep the numbers in their order, so that x can come by tensor copies: with the order that a shift
-// and a mask leave, other warps had to reorder x, 880 more a group).
+// Reading W is 8,704 bytes a group, 0.2 us of an SM's share of the memory rate.  Measured 0.5 us a group and SM, with one block or two: without the
+// arithmetic of unpacking (17 instructions for 8 numbers, 1,150 of a warp a group) 0.3, without the products 0.48; more warps that unpack,
+// deeper rings and waits that sleep change nothing.  (Two of the 17 keep the numbers in their order, so that x can come by tensor copies: four
+// warps that reordered x instead took 880 instructions a group.)  32 rows, us: 4,096 x 4,096 10.8, 5,120 x 17,408 28.4, 24,576 x 4,096 31.6;
+// 64 rows 12.9, -, 34.8; 128 rows 24,576 x 4,096 53.
 #include "int4.cuh"
 #include "glu.cuh"
 #include "tcgen05.cuh"
@@ -281,10 +282,20 @@ extern "C" int gi_int4_linear_tcgen05(const void* x, const void* tiles, void* ou
     GI_REQUIRE(error_flag != nullptr, "gi_int4_linear_tcgen05: an error flag on the device is required");
     const int groups = (K + I4_GROUP_W - 1) / I4_GROUP_W, bn = M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const long long blocks = (long long)((glu ? N / 2 + 63 : N + 127) / (glu ? 64 : 128)) * ((M + bn - 1) / bn);
-    // As many as leave no block waiting for a place: 148 SMs hold 48 clusters of 3 and 33 of 4, and rarely all of them at once.  32 rows, us by
-    // ranks: 40 tiles x 136 groups 1: 69, 2: 38, 3: 29, 4: 37; 32 x 96 2: 30, 3: 23, 4: 19, 5: 25; 48 x 32 1: 21, 2: 14, 3: 16
-    if (ranks == 0)
-        for (ranks = 1; ranks < 8 && blocks * (ranks + 1) <= 132 && groups >= 4 * (ranks + 1);) ++ranks;
+    // In ns: 500 a group of 128 inputs, 450 where two blocks share an SM, 1,000 a block and 800 more for each of a cluster (128 rows: 2,000 and
+    // 3,000, their sums being larger); the SMs hold 148 blocks at once, 74 clusters of 2, 33 of 4 and rarely more than 44 of 3.  us by ranks:
+    //    32 rows, 40 rows of tiles x 136 groups   1: 69   2: 38   3: 29   4: 36      128 rows, 32 x 96    1: 59   2: 38   3: 30   4: 27
+    //    32 rows, 48 x 32                         1: 21   2: 14   3: 16   4: 14      128 rows, 192 x 32   1: 53   2: 57   3: 79
+    //    32 rows, 192 x 32                        1: 35   2: 32   3: 38   4: 40      384 rows, 32 x 96    1: 59   2: 74   4: 76
+    if (ranks == 0) {
+        const int held[4] = {148, 74, 44, 33};
+        long long best = 0;
+        for (int r = 1; r <= 4 && r <= groups; ++r) {
+            const long long load = (blocks + held[r - 1] - 1) / held[r - 1], each = (groups + r - 1) / r;
+            const long long ns = bn <= 64 ? load * each * (load > 1 ? 450 : 500) + (load + 1) / 2 * (1000 + 800 * r) : load * (each * 500 + 2000 + 3000 * r);
+            if (ranks == 0 || ns < best) best = ns, ranks = r;
+        }
+    }
     GI_REQUIRE(ranks >= 1 && ranks <= 8 && ranks <= groups, "gi_int4_linear_tcgen05: a cluster of %d blocks; 1 to 8 are possible, with a group of inputs each", ranks);
     const GluShape unit = {kind, alpha, gate_max, up_limit, up_shift};
     CUtensorMap xp;
