@@ -383,9 +383,12 @@ def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
         tiles, places = (1, PLACES) if columns <= 8 else (-(-columns // 16), 444)
         return _few(l, dev, q, at, shape, pools, table, runs_at, n_runs, None, None, scale, window, status, q.new_zeros((n, n_q * d)),
                     decode_splits(n_runs * tiles, heads, 64 * n_blocks // n_runs, places, 2048), n_runs * heads * tiles)
+    if n_blocks == 0:
+        raise KernelError(f"{n_runs} runs that see no block of the cache")
     max_blocks = -(-width * page_size // 64)
+    kept = torch.empty_like(runs)
     pages = q.new_empty((2, n_blocks, heads, 64, d))
     new_table = block_table.new_full((n_slots, max_blocks), -1)
-    check(l.gi_int4_gather(*pools, pages[0].data_ptr(), pages[1].data_ptr(), new_table.data_ptr(), blocks_at, n_blocks, table[0], heads, d,
-                           n_slots, width, max_blocks, page_size, n_pages, _status(dev, status), _stream(dev)), l)
-    return kernels.attention_prefill_tcgen05(q, pages[0], pages[1], new_table, runs, scale, window)
+    check(l.gi_int4_gather(*pools, pages[0].data_ptr(), pages[1].data_ptr(), new_table.data_ptr(), blocks_at, n_blocks, runs_at,
+                           kept.data_ptr(), n_runs, n, table[0], heads, d, n_slots, width, max_blocks, page_size, n_pages, _status(dev, status), _stream(dev)), l)
+    return kernels.attention_prefill_tcgen05(q, pages[0], pages[1], new_table, kept, scale, window)

@@ -630,6 +630,27 @@ def test_prompts_of_few_and_of_many_tokens_agree_where_they_meet(ops):
         assert not bool(ops.int4.attention_prompt(q[:12], k_rows, v_rows, table, bad, blocks, d ** -0.5, 0, status).any()) and int(status) == 4
 
 
+def test_long_runs_that_do_not_exist_are_left_out(ops):
+    """Runs of more columns than are read as single tokens: a slot, rows or positions that do not exist are reported, the others stay right."""
+    g = gen(29)
+    heads, kv, d, n = 8, 1, 64, 40
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [100, 60], kv, d, 16)
+    q = randn(g, 2 * n, heads, d).to(torch.bfloat16)
+    runs, blocks = runs_and_blocks([(0, 0, n, 60), (1, n, n, 20)], 0)
+    assert 2 * n * heads > ops.int4.FEW_COLUMNS * 2
+    want = ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, 0.125, 0, status)
+    assert int(status) == 0 and torch.equal(runs[0].cpu(), torch.tensor([0, 0, n, 60], dtype=torch.int32))
+    for bad, code in (([-1, 0, n, 60], 0), ([0, 0, 0, 60], 0), ([2, 0, n, 60], 4), ([0, -1, n, 60], 4), ([0, n + 1, n, 60], 4), ([0, 0, n, -1], 4),
+                      ([0, 0, n, 100000], 4), ([0, 0, 129, 0], 4), ([0, 0, n, 2147483647], 4)):
+        status.zero_()
+        some = runs.clone()
+        some[0] = torch.tensor(bad, dtype=torch.int32)
+        got = ops.int4.attention_prompt(q, k_rows, v_rows, table, some, blocks, 0.125, 0, status)
+        assert int(status) == code and torch.equal(got[n:], want[n:]) and not bool(got[:n].any()), bad
+    with pytest.raises(ops.KernelError):
+        ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks[:0], 0.125, 0, status)
+
+
 def test_pages_given_back_behind_the_window_are_not_missed(ops):
     g = gen(17)
     heads, kv, d, n, window = 4, 1, 64, 300, 50
