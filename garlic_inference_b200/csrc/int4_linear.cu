@@ -347,26 +347,20 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------ host
-#include <mutex>
-#include <vector>
-namespace {
-struct Residency { const void* kernel; int device, ranks; size_t smem; int clusters; };
-std::mutex g_residency_mutex;
-std::vector<Residency> g_residency;
-}
-// How many clusters of `ranks` CTAs of this kernel the current device holds at once (looked up once).
-static int resident_clusters(const void* kernel, cudaLaunchConfig_t* cfg, int ranks, size_t smem, int* clusters) {
+#include <atomic>
+// How many clusters of `ranks` blocks of this kernel the current device holds at once: `seen` [device][ranks], 0 where it was not asked for yet.
+#define I4L_DEVICES 64
+static int resident_clusters(const void* kernel, cudaLaunchConfig_t* cfg, int ranks, std::atomic<int> (*seen)[9], int* clusters) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) { gi_set_error("gi_int4_linear: %s", cudaGetErrorString(e)); return (int)e; }
-    std::lock_guard<std::mutex> lock(g_residency_mutex);
-    for (const Residency& r : g_residency)
-        if (r.kernel == kernel && r.device == dev && r.ranks == ranks && r.smem == smem) { *clusters = r.clusters; return 0; }
+    *clusters = dev < I4L_DEVICES ? seen[dev][ranks].load(std::memory_order_relaxed) : 0;
+    if (*clusters > 0) return 0;
     cfg->gridDim = dim3(1, ranks);
     e = cudaOccupancyMaxActiveClusters(clusters, kernel, cfg);
     if (e != cudaSuccess) { gi_set_error("gi_int4_linear: clusters of %d: %s", ranks, cudaGetErrorString(e)); return (int)e; }
-    if (*clusters < 1) { gi_set_error("gi_int4_linear: no cluster of %d blocks with %zu bytes of shared memory fits this GPU", ranks, smem); return GI_ERR_ARGUMENT; }
-    g_residency.push_back({kernel, dev, ranks, smem, *clusters});
+    if (*clusters < 1) { gi_set_error("gi_int4_linear: no cluster of %d blocks fits this GPU", ranks); return GI_ERR_ARGUMENT; }
+    if (dev < I4L_DEVICES) seen[dev][ranks].store(*clusters, std::memory_order_relaxed);
     return 0;
 }
 
@@ -380,8 +374,8 @@ static size_t smem_of(int ranks, int parts, int sg, int groups, int units, int c
 // Clusters of so many blocks, one to an SM, that a B200 was seen to hold at once.
 static int resident(int ranks) { const int n[9] = {0, 148, 74, 48, 33, 28, 21, 18, 15}; return n[ranks]; }
 // The cut whose busiest warp has the least to do: tiles to multiply, rows of tiles to hand over (as long as a tile), pairs of rows of x to
-// convert (two tiles), sums of a row to add up (an eighth); an even number of blocks, or one (clusters of 3 or 5 left a recorded step's SMs idle: 28 us where 4 took 16).  Best and chosen,
-// us: 8 x 4096 x 4096 6.9 in 4 blocks and 2 parts, chosen; 8 x 12288 x 4096 11.8 in 6 and 1, chosen; 8 x 4096 x 24576 gated 16.1 in 4 and 1, chosen.
+// convert (two tiles), sums of a row to add up (an eighth); an even number of blocks, or one (clusters of 3 or 5 left a recorded step's SMs idle: 28 us where
+// 4 took 16).  Best and chosen, us: 8 x 4096 x 4096 6.9 in 4 blocks and 2 parts, chosen; 8 x 12288 x 4096 11.8 in 6 and 1, chosen; 8 x 4096 x 24576 gated 16.1 in 4 and 1, chosen.
 static Int4Cut cut_of(int M, int N, int K, int glu, int ranks, int parts) {
     const int groups = (K - 1) / I4_GROUP_W + 1, row_tiles = (N + 15) / 16, units = glu ? row_tiles / 2 : row_tiles, nt = M > 8 ? 2 : 1, R = glu ? 2 : 1;
     Int4Cut cut = {0, 0, 0};
@@ -426,8 +420,9 @@ static int launch_int4_linear(const bf16* x, const unsigned char* tiles, void* o
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    static std::atomic<int> seen[I4L_DEVICES][9];
     int clusters = 0;
-    if (int rc = resident_clusters((const void*)kernel, &cfg, pick, cfg.dynamicSmemBytes, &clusters)) return rc;
+    if (int rc = resident_clusters((const void*)kernel, &cfg, pick, seen, &clusters)) return rc;
     if (clusters > units) clusters = units;
     const size_t smem = smem_of(pick, pick_parts, cut.sg, groups, units, clusters, NT, R);
     GI_REQUIRE(smem <= 224 * 1024, "gi_int4_linear: %d x %d is too large for %d rows on %d clusters of %d blocks", N, K, M, clusters, pick);

@@ -208,6 +208,7 @@ def test_rows_of_odd_lengths_and_starts(ops, m, n, k):
     odd.copy_(randn(g, m, 128))
     v = random_weight(ops, g, n, 128)
     assert torch.equal(ops.linear(odd, v, torch.float32), ops.linear(odd.clone(), v, torch.float32))
+    assert torch.equal(ops.linear(odd[:11], v, torch.float32), ops.linear(odd[:11].clone(), v, torch.float32))
 
 
 @pytest.mark.parametrize("m,inter,k", [(20, 16, 128), (40, 48, 520), (100, 208, 1024), (150, 64, 384), (64, 1000, 256)])
@@ -667,6 +668,40 @@ def test_pages_given_back_behind_the_window_are_not_missed(ops):
     table[0, (n - 10) // 16] = -1                            # one that the window holds is
     ops.int4.attention_decode(q[:1], k_rows, v_rows, table, pos, slot, 0.125, window, status)
     assert int(status) == 5
+
+
+def test_pages_and_tiles_beyond_32_bits(ops):
+    """Codes that lie further than 2^32 bytes into their tensors."""
+    g = gen(31)
+    heads, kv, d, page = 4, 8, 128, 64
+    n_pages = (1 << 32) // (kv * page * d // 2) + 40
+    k_rows, v_rows = (ops.int4.Int4Rows.zeros(n_pages, kv, page, d, DEV) for _ in range(2))
+    table = torch.tensor([[n_pages - 1, n_pages - 7, 3, n_pages - 30]], dtype=torch.int32, device=DEV)
+    near = torch.tensor([[3, 2, 0, 1]], dtype=torch.int32, device=DEV)
+    small = [ops.int4.Int4Rows.zeros(4, kv, page, d, DEV) for _ in range(2)]
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    pos, slot = torch.arange(240, dtype=torch.int32, device=DEV), torch.zeros(240, dtype=torch.int32, device=DEV)
+    k, v = (randn(g, 240, kv, d).to(torch.bfloat16) for _ in range(2))
+    q = randn(g, 240, 2 * kv, d).to(torch.bfloat16)
+    runs, blocks = runs_and_blocks([(0, 0, 240, 0)], 0)
+    out = []
+    for rows, t in (((k_rows, v_rows), table), (small, near)):
+        ops.int4.append(k, v, *rows, t, pos, slot, status)
+        out.append([ops.int4.read(rows[0], t, pos, slot, status), ops.int4.attention_decode(q[:1], *rows, t, pos[239:], slot, 0.09, 0, status),
+                    ops.int4.attention_prompt(q, *rows, t, runs, blocks, 0.09, 0, status),
+                    ops.int4.attention_prompt(q[:3], *rows, t, torch.tensor([[0, 0, 3, 237]], dtype=torch.int32, device=DEV), blocks, 0.09, 0, status)])
+    assert int(status) == 0 and all(torch.equal(a, b) for a, b in zip(*out)) and bool(out[0][0].any())
+    del k_rows, v_rows, out
+    n, ins = 140000, 65536                                   # 8,750 x 512 tiles, 4.9 GB
+    tiles = torch.randint(0, 256, (n // 16, ins // 128, 1088), dtype=torch.uint8, device=DEV, generator=g)
+    tiles[..., 1024:] = torch.tensor([0.01, -0.08], dtype=torch.bfloat16, device=DEV).view(torch.uint8).repeat(16)
+    w, last = ops.int4.Int4Weight(tiles, n, ins), ops.int4.Int4Weight(tiles[-2:].clone(), 32, ins)
+    for m in (2, 20):
+        x = randn(g, m, ins).to(torch.bfloat16)
+        want = x.double() @ plain.values(*plain.unpack_weight(last), 128).t()
+        got = ops.linear(x, w, torch.float32)[:, -32:].double()
+        assert float(((got - want).abs() / (wide_bound(x, last) + 2 ** -24 * want.abs())).max()) <= 1
+    assert torch.equal(ops.int4.dequantize_weight(w, torch.float32, n - 32, 32), ops.int4.dequantize_weight(last, torch.float32))
 
 
 def test_refusals(ops):

@@ -137,6 +137,30 @@ def test_generation_is_repeatable_and_gives_its_pages_back(model_dirs):
     assert cache.slots.n_free == cache.max_slots and all(g.host.pool.n_free == g.host.pool.n_pages for g in cache.groups)
 
 
+@pytest.mark.parametrize("module,name", [("tiny_fivitar", "mix"), ("tiny_kenovik", None), ("tiny_dugopel", None), ("tiny_zogulorn", None),
+                                         ("tiny_nezolorn", None), ("tiny_netolorn", None)])
+def test_other_architectures_pack_their_feed_forwards_or_say_that_they_pack_nothing(module, name, tmp_path):
+    """Every model either runs with what it packs, graphs included, or refuses; none has keys and values for 4 bits."""
+    import importlib
+    tiny_of = importlib.import_module(module)
+    ran = 0
+    for n in [name] if name else list(tiny_of.TINY):
+        folder = tmp_path / n
+        folder.mkdir()
+        folder = tiny_of.write_model(n, folder)
+        try:
+            model = load(folder, max_tokens=256, weights="int4")
+        except ValueError as e:
+            assert "none of this model's parts" in str(e)
+            continue
+        out = model.generate([[1, 2, 3, 4, 5], [7, 8]], max_new_tokens=6)
+        assert [len(o) for o in out] == [6, 6] and out == model.generate([[1, 2, 3, 4, 5], [7, 8]], max_new_tokens=6)
+        ran += 1
+        with pytest.raises(ValueError, match="none of this model's mixers"):
+            load(folder, max_tokens=256, cache="int4")
+    assert ran
+
+
 def test_float32_activations_take_weights_in_4_bits_and_no_such_cache(model_dirs):
     model = load(model_dirs("D"), max_tokens=256, dtype="float32", weights="int4")
     assert len(model.generate([[1, 2, 3]], max_new_tokens=5)[0]) == 5
