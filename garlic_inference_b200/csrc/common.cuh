@@ -96,6 +96,13 @@ __device__ __forceinline__ void gi_pdl_wait() {
     gi_tl_mark(1);
 }
 
+// For kernels whose result a later kernel may take for "nobody's output" and ask for before its own wait (weights): the next kernel
+// is not let start early, so it is launched when this grid has finished and its writes are visible.
+__device__ __forceinline__ void gi_pdl_start_alone() {
+    gi_tl_mark(0);
+    gi_pdl_wait();
+}
+
 // kernel<<<grid, block, smem, stream>>>(args...), with the attribute that allows the overlap above when
 // gi_pdl_enabled().
 bool gi_pdl_enabled();

@@ -5,7 +5,8 @@
 // and 8-15), in each 8 outputs x 4 quarters of 32 inputs x 16 bytes, which is the order in which the 32 lanes of a warp hold the
 // product's first operand, 16 bytes each; then (step, low) of the 16 outputs.  What a tile holds beyond N or K is zeros.
 //
-// Both kernels are bound by the 16- or 32-bit side: 2 or 4 bytes a number against 0.53.
+// Both kernels are bound by the 16- or 32-bit side: 2 or 4 bytes a number against 0.53.  Neither lets its successor start early: products ask
+// for their weight before they wait for the kernel in front, and here that kernel writes it.
 #include "int4.cuh"
 
 // A warp per (output, group of 128): 4 consecutive inputs a lane.
@@ -13,7 +14,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 int4_quantize_weight_kernel(const T* __restrict__ w, long long ld, unsigned char* __restrict__ tiles, int N, int K, long long items,
                             int groups) {
-    gi_pdl_start();
+    gi_pdl_start_alone();
     const long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     if (item >= items) return;
     const int lane = threadIdx.x & 31;
@@ -53,7 +54,7 @@ int4_quantize_weight_kernel(const T* __restrict__ w, long long ld, unsigned char
 template <typename T>
 __global__ void __launch_bounds__(256)
 int4_dequantize_weight_kernel(const unsigned char* __restrict__ tiles, T* __restrict__ out, int n0, int rows, int K, int groups, int vec) {
-    gi_pdl_start();
+    gi_pdl_start_alone();
     const int word = blockIdx.x * 256 + threadIdx.x, group = word >> 4, k0 = word * 8;      // eight inputs
     if (k0 >= K) return;
     const int piece = blockIdx.y + (n0 >> 3);

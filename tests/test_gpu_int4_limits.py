@@ -1,0 +1,83 @@
+"""4 bits at the limits of what the entry points take: float32 activations in recorded steps, sizes beyond one kernel's room, steps of unlike
+runs, numbers far apart."""
+import shutil
+
+import pytest
+import torch
+
+import plain_int4 as plain
+import tiny
+from test_gpu_int4 import gen, random_weight, randn
+from test_gpu_int4_model import HELD, load
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from garlic_inference_b200 import ops
+    return ops
+
+
+def held_folder(folder, to):
+    """The model of `folder` with the numbers that its weights' codes stand for as float32 weights."""
+    from garlic_inference_b200.ops import int4
+    from garlic_inference_b200.weights import Checkpoint
+    from garlic_inference_b200.weights.safetensors_io import write_safetensors
+    ckpt = Checkpoint(folder)
+    tensors = {}
+    for n in ckpt.names():
+        t = ckpt.tensor(n).clone()
+        if any(f"{p}.weight" in n for p in HELD):
+            t = int4.dequantize_weight(int4.quantize_weight(t.cuda()), torch.float32).cpu()
+        tensors[n] = t
+    shutil.copy(folder / "config.json", to / "config.json")
+    write_safetensors(to / "model.safetensors", tensors)
+    return to
+
+
+# ------------------------------------------------------------------------------------------------ weights made wide
+@pytest.mark.parametrize("name", ["D", "E"])
+def test_float32_steps_recorded_and_eager(name, model_dirs, tmp_path):
+    """Every layer's weight is made wide right in front of its product: recorded steps, whose kernels start early, give the bits
+    of eager ones, and both the logits of the codes' numbers."""
+    reqs = tiny.random_requests(tiny.TINY[name]["cfg"]["vocab_size"], [90, 41, 7], seed=6)
+    want = tiny.plain_logits(held_folder(model_dirs(name), tmp_path), reqs)
+    traces = (tiny.trace_tail_by_one(reqs, tail=24), tiny.trace_batched(reqs, [["r0", "r1", "r2"]], prompt_frac=0.5))
+    for trace in traces:
+        got = []
+        for graphs in (True, False):
+            model = load(model_dirs(name), max_tokens=384, dtype="float32", weights="int4", use_graphs=graphs)
+            got.append(tiny.run_trace_in_process(model, trace))
+            tiny.compare(got[-1], want, tiny.TOL["float32"], f"{name} graphs={graphs}")
+        for rid in got[0]:
+            for p in got[0][rid]:
+                assert (got[0][rid][p] == got[1][rid][p]).all(), (rid, p)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 256, 192), (3, 100, 384), (9, 64, 130), (1, 1024, 2048), (40, 2048, 1024)])
+def test_products_right_behind_the_kernel_that_makes_their_weight(ops, m, n, k):
+    """With launches that let the next kernel start early: weights of one size in turn, so that what the memory held before is another
+    weight; float32 rows over 4-bit weights, and weights that are quantised in front of their product."""
+    g = gen(m + n + k)
+    ws = [randn(g, n, k) for _ in range(4)]
+    held = [ops.int4.quantize_weight(w) for w in ws]
+    x = randn(g, m, k)
+    xb = x.to(torch.bfloat16)
+    want = [(ops.linear(x, h), ops.linear(xb, h, torch.float32)) for h in held]
+    torch.cuda.synchronize()
+    from garlic_inference_b200.ops import kernels
+    kernels.set_dependent_launch(True)
+    try:
+        for _ in range(5):
+            got = []
+            for w, h in zip(ws, held):
+                a = ops.linear(x, h)
+                fresh = ops.int4.quantize_weight(w)
+                got.append((a, ops.linear(xb, fresh, torch.float32)))
+                del fresh
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q))
+    finally:
+        kernels.set_dependent_launch(False)
