@@ -154,9 +154,19 @@ def linear_rows(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.b
     return out
 
 
+_rows_take: dict = {}
+
+
 def linear_rows_takes(rows: int, w: Int4Weight, gated: bool) -> bool:
-    """Whether `linear_rows` has room for so many rows of this weight's inputs."""
-    return bool(require_gpu().gi_int4_linear_takes(rows, w.n, w.k, int(gated)))
+    """Whether `linear_rows` has room in shared memory for so many rows of x and their sums, which grow with the weight's inputs and
+    outputs.  The answer is the same for 1 to 8 and for 9 to 16 rows, and is kept."""
+    if not 1 <= rows <= LINEAR_MAX_ROWS:
+        return False
+    key = (rows > 8, w.n, w.k, gated, w.tiles.get_device())
+    takes = _rows_take.get(key)
+    if takes is None:
+        takes = _rows_take[key] = bool(require_gpu().gi_int4_linear_takes(rows, w.n, w.k, int(gated)))
+    return takes
 
 
 def linear_wide(x: torch.Tensor, w: Int4Weight, out_dtype: torch.dtype = torch.bfloat16, unit: Optional[tuple] = None,

@@ -73,14 +73,13 @@ def _streamk_min_bytes(m: int) -> int:
 # 24,576 x 4,096 105 / 122, 6,144 x 4,096 28 / 39; 512 rows 155 / 126, 53 / 40, 4,096 x 12,288 60 / 84.
 INT4_CODES_MAX_ROWS = 384
 INT4_WIDE_BYTES = 64 << 20        # of a weight made wide at a time: it stays in L2 between the two kernels
-INT4_SURE_INPUTS = 32768          # up to here the kernel for 16 rows has room for its slice of x, whatever the cut
 
 
 def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Optional[tuple] = None,
           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The product with a weight in 4 bits, or (`unit`) the gated unit of its halves.  bfloat16: up to 16 rows `int4.linear_rows`
-    (17 rows of 4,096 x 4,096: 15 us in two pieces, 10 in one of the next), up to INT4_CODES_MAX_ROWS `int4.linear_wide`.  More, or float32: the weight is made wide, some outputs at a time, for the products that
-    `linear` has for that type.  Beyond 16 rows bfloat16 rounds each number of the weight once on the way (by half a step of
+    where it has room (17 rows of 4,096 x 4,096: 15 us in two pieces, 10 in one of the next), up to INT4_CODES_MAX_ROWS `int4.linear_wide`.  More, or float32: the weight is made wide, some outputs at a time, for the products that
+    `linear` has for that type.  Beyond `linear_rows` bfloat16 rounds each number of the weight once on the way (by half a step of
     2^-8, a hundredth of what 4 bits leave of it)."""
     if x.dim() != 2 or x.shape[1] != w.k:
         raise KernelError(f"linear: x {tuple(x.shape)} does not fit a weight {w.shape} ([out, in])")
@@ -88,7 +87,7 @@ def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Opt
         raise KernelError(f"linear: {w.n} outputs cannot be a gate and an up half")
     m, n = x.shape[0], w.n if unit is None else w.n // 2
     fits = x.dtype is torch.bfloat16 and (unit is None or n % 16 == 0)
-    if fits and 0 < m <= int4.LINEAR_MAX_ROWS and (w.k <= INT4_SURE_INPUTS or int4.linear_rows_takes(m, w, unit is not None)):
+    if fits and int4.linear_rows_takes(m, w, unit is not None):
         return int4.linear_rows(x, w, out_dtype, unit, out)
     aligned = w.k % 8 == 0 and x.data_ptr() % 16 == 0
     if fits and aligned and 0 < m <= INT4_CODES_MAX_ROWS:

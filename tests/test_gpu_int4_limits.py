@@ -7,7 +7,7 @@ import torch
 
 import plain_int4 as plain
 import tiny
-from test_gpu_int4 import gen, random_weight, randn
+from test_gpu_int4 import gen, randn, wide_bound
 from test_gpu_int4_model import HELD, load
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +81,29 @@ def test_products_right_behind_the_kernel_that_makes_their_weight(ops, m, n, k):
             assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q))
     finally:
         kernels.set_dependent_launch(False)
+
+
+# -------------------------------------------------------------------------------------------- sizes beyond a kernel's room
+@pytest.mark.parametrize("m,n,k,gated", [(16, 2048, 32768, False), (9, 2048, 32768, False), (16, 32, 32768, True), (12, 152064, 4096, False),
+                                         (10, 57344, 8192, True), (9, 8192, 28672, False), (1, 106496, 16384, True)])
+def test_steps_of_few_rows_whose_sums_have_no_room_beside_them(ops, m, n, k, gated):
+    g = gen(m + n + k)
+    tile = torch.randint(0, 256, (n // 16, k // 128, 1088), dtype=torch.uint8, device=DEV, generator=g)
+    tile[..., 1024:] = torch.tensor([0.01, -0.08], dtype=torch.bfloat16, device=DEV).view(torch.uint8).repeat(16)
+    w = ops.int4.Int4Weight(tile, n, k)
+    assert not ops.int4.linear_rows_takes(m, w, gated)
+    x = randn(g, m, k).to(torch.bfloat16)
+    got = ops.swiglu_product(x, w) if gated else ops.linear(x, w, torch.float32)
+    half = n // 2 if gated else n
+    assert got.shape == (m, half)
+    # 16 outputs at either end (of both halves), each against 64 bits; bounds: test_gpu_int4.wide_bound, and a bfloat16 result of a unit
+    for a in {0, half - 16}:
+        parts = [ops.int4.Int4Weight(tile[i // 16:i // 16 + 1].clone(), 16, k) for i in ((a, half + a) if gated else (a,))]
+        y = [x.double() @ plain.values(*plain.unpack_weight(p), 128).t() for p in parts]
+        off = [wide_bound(x, p) for p in parts]
+        if gated:
+            want = y[0] * torch.sigmoid(y[0]) * y[1]
+            bound = 2 ** -8 * want.abs() + 1.1 * off[0] * (y[1].abs() + off[1]) + y[0].abs() * off[1] + 2 ** -19 * (y[0] * y[1]).abs() + 2 ** -30
+        else:
+            want, bound = y[0], off[0] + 2 ** -24 * y[0].abs()
+        assert float(((got[:, a:a + 16].double() - want).abs() / bound).max()) <= 1

@@ -100,3 +100,25 @@ def test_options_of_the_entry_points(name, tmp_path):
     assert getattr(args, name) == "int4" and getattr(build_parser().parse_args(["folder"]), name) is None
     with pytest.raises(SystemExit):
         build_parser().parse_args(["folder", f"--{name}", "int2"])
+
+
+def test_products_go_where_there_is_room(monkeypatch):
+    """The choice of product against the capacity that the kernel for up to 16 rows states, over sizes on both sides of it."""
+    from garlic_inference_b200.ops import lib, linear as entry, swiglu_product
+    taken = []
+    for name in ("linear_rows", "linear_wide"):
+        monkeypatch.setattr(int4, name, lambda x, w, *a, name=name, **k: taken.append(name))
+    monkeypatch.setattr(int4, "require_gpu", lib)
+    monkeypatch.setattr(int4, "_rows_take", {})
+    both = set()
+    for k in (128, 1024, 4096, 8192, 16384, 28672, 32768, 120000):
+        for n in (32, 2048, 8192, 57344, 106496, 152064):
+            w = int4.Int4Weight(torch.empty(n // 16, -(-k // 128), 1088, dtype=torch.uint8, device="meta"), n, k)
+            for m in (1, 8, 9, 12, 16, 17):
+                x = torch.empty((m, k), dtype=torch.bfloat16, device="meta")
+                for product, gated in ((entry, 0), (swiglu_product, 1)):
+                    product(x, w)
+                    takes = lib().gi_int4_linear_takes(m, n, k, gated)
+                    both.add((takes, m <= 16))
+                    assert taken.pop() == ("linear_rows" if takes else "linear_wide"), (m, n, k, gated)
+    assert both == {(0, True), (1, True), (0, False)}
