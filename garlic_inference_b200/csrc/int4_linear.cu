@@ -348,46 +348,68 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
 
 // ------------------------------------------------------------------------------------------------ host
 #include <atomic>
-// How many clusters of `ranks` blocks of this kernel the current device holds at once: `seen` [device][ranks], 0 where it was not asked for yet.
 #define I4L_DEVICES 64
-static int resident_clusters(const void* kernel, cudaLaunchConfig_t* cfg, int ranks, std::atomic<int> (*seen)[9], int* clusters) {
+#define I4L_WARPS 16
+#define I4L_SMEM (214 * 1024)      // of an SM's 227 KB: what a product may take
+// Clusters of 1 to 8 blocks, one to an SM, that a B200 was seen to hold at once.  They differ a little from device to device (45 of 3, 26
+// of 5, 22 of 6, 15 of 7 on another): the cut, and so the order of the sums, is chosen with these, that a result has the same bits on all.
+static const int i4l_b200[9] = {0, 148, 74, 48, 33, 28, 21, 18, 15};
+// What the current device holds, asked for once a device: how many are launched, and so what a product's sums take in shared memory.  Where
+// there is no device to ask (sizes worked out on a host), the numbers above.
+struct Int4Held { int clusters[9]; };
+static int clusters_held(Int4Held* held) {
+    static std::atomic<int> seen[I4L_DEVICES][9];
     int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) { gi_set_error("gi_int4_linear: %s", cudaGetErrorString(e)); return (int)e; }
-    *clusters = dev < I4L_DEVICES ? seen[dev][ranks].load(std::memory_order_relaxed) : 0;
-    if (*clusters > 0) return 0;
-    cfg->gridDim = dim3(1, ranks);
-    e = cudaOccupancyMaxActiveClusters(clusters, kernel, cfg);
-    if (e != cudaSuccess) { gi_set_error("gi_int4_linear: clusters of %d: %s", ranks, cudaGetErrorString(e)); return (int)e; }
-    if (*clusters < 1) { gi_set_error("gi_int4_linear: no cluster of %d blocks fits this GPU", ranks); return GI_ERR_ARGUMENT; }
-    if (dev < I4L_DEVICES) seen[dev][ranks].store(*clusters, std::memory_order_relaxed);
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        for (int r = 0; r <= 8; ++r) held->clusters[r] = i4l_b200[r];
+        return 0;
+    }
+    // every instance of the kernel has the same threads, and takes more than half an SM's shared memory: one stands for all
+    auto kernel = int4_linear_kernel<1, I4L_WARPS, false>;
+    held->clusters[0] = 0;
+    for (int r = 1; r <= 8; ++r) {
+        int n = dev < I4L_DEVICES ? seen[dev][r].load(std::memory_order_relaxed) : 0;
+        if (n == 0) {
+            if (int rc = gi_reserve_smem((const void*)kernel, 224 * 1024, "gi_int4_linear")) return rc;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1, r), cfg.blockDim = dim3((I4L_WARPS + I4L_COPIERS) * 32), cfg.dynamicSmemBytes = I4L_SMEM;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1, attr[0].val.clusterDim.y = r, attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr, cfg.numAttrs = 1;
+            const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, (const void*)kernel, &cfg);
+            if (e != cudaSuccess) { gi_set_error("gi_int4_linear: clusters of %d: %s", r, cudaGetErrorString(e)); return (int)e; }
+            if (n < 1) n = -1;                                           // none fits: that number of blocks is not taken
+            if (dev < I4L_DEVICES) seen[dev][r].store(n, std::memory_order_relaxed);
+        }
+        held->clusters[r] = n;
+    }
     return 0;
 }
 
 // How a product is cut: blocks that share K, parts that a block's warps take of its slice, groups of a copy; ranks 0: it does not fit.
 struct Int4Cut { int ranks, parts, sg; };
-#define I4L_WARPS 16
 static size_t smem_of(int ranks, int parts, int sg, int groups, int units, int clusters, int nt, int rows_of_unit) {
     return (size_t)I4L_WARPS * I4L_STAGES * sg * I4_TILE + (size_t)((groups + ranks - 1) / ranks) * nt * (2048 + 64) +
            (size_t)(((units + clusters - 1) / clusters + ranks - 1) / ranks) * rows_of_unit * ranks * parts * nt * 512;
 }
-// Clusters of so many blocks, one to an SM, that a B200 was seen to hold at once.
-static int resident(int ranks) { const int n[9] = {0, 148, 74, 48, 33, 28, 21, 18, 15}; return n[ranks]; }
 // The cut whose busiest warp has the least to do: tiles to multiply, rows of tiles to hand over (as long as a tile), pairs of rows of x to
 // convert (two tiles), sums of a row to add up (an eighth); an even number of blocks, or one (clusters of 3 or 5 left a recorded step's SMs idle: 28 us where
 // 4 took 16).  Best and chosen, us: 8 x 4096 x 4096 6.9 in 4 blocks and 2 parts, chosen; 8 x 12288 x 4096 11.8 in 6 and 1, chosen; 8 x 4096 x 24576 gated 16.1 in 4 and 1, chosen.
-static Int4Cut cut_of(int M, int N, int K, int glu, int ranks, int parts) {
+static Int4Cut cut_of(int M, int N, int K, int glu, int ranks, int parts, const Int4Held& held) {
     const int groups = (K - 1) / I4_GROUP_W + 1, row_tiles = (N + 15) / 16, units = glu ? row_tiles / 2 : row_tiles, nt = M > 8 ? 2 : 1, R = glu ? 2 : 1;
     Int4Cut cut = {0, 0, 0};
     long long best = -1;
     for (int r = 1; r <= 8; ++r) {
         if (ranks ? r != ranks : (r > 1 && r % 2)) continue;
-        if (r > groups) continue;
-        const int slice = (groups + r - 1) / r, clusters = units < resident(r) ? units : resident(r), rows = R * ((units + clusters - 1) / clusters);
+        if (r > groups || held.clusters[r] < 1) continue;
+        const int slice = (groups + r - 1) / r, clusters = units < held.clusters[r] ? units : held.clusters[r],
+                  rows = R * ((units + i4l_b200[r] - 1) / i4l_b200[r]);
         for (int p = 1; p <= 16 && p <= slice; p *= 2) {
             if (parts && p != parts) continue;
-            const int sg = smem_of(r, p, 4, groups, units, clusters, nt, R) <= 214 * 1024 && nt == 1 ? 4 : 2;
-            if (smem_of(r, p, sg, groups, units, clusters, nt, R) > 214 * 1024) continue;
+            const int sg = smem_of(r, p, 4, groups, units, clusters, nt, R) <= I4L_SMEM && nt == 1 ? 4 : 2;
+            if (smem_of(r, p, sg, groups, units, clusters, nt, R) > I4L_SMEM) continue;
             const int stride = I4L_WARPS / p;
             const long long turns = (rows + stride - 1) / stride;
             const long long cost = 8 * (turns * ((slice + p - 1) / p + 1) + 2 * ((slice * 4 * nt + I4L_WARPS - 1) / I4L_WARPS)) + r * p;
@@ -399,7 +421,7 @@ static Int4Cut cut_of(int M, int N, int K, int glu, int ranks, int parts) {
 
 template <int NT, bool GLU>
 static int launch_int4_linear(const bf16* x, const unsigned char* tiles, void* out, int out_f32, int M, int N, int K, Int4Cut cut,
-                              GluShape act, long long ld_out, int* error_flag, cudaStream_t stream) {
+                              const Int4Held& held, GluShape act, long long ld_out, int* error_flag, cudaStream_t stream) {
     const int groups = (K - 1) / I4_GROUP_W + 1, row_tiles = (N + 15) / 16, units = GLU ? row_tiles / 2 : row_tiles;
     auto kernel = int4_linear_kernel<NT, I4L_WARPS, GLU>;
     constexpr int WARPS = I4L_WARPS, R = GLU ? 2 : 1;
@@ -420,12 +442,8 @@ static int launch_int4_linear(const bf16* x, const unsigned char* tiles, void* o
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    static std::atomic<int> seen[I4L_DEVICES][9];
-    int clusters = 0;
-    if (int rc = resident_clusters((const void*)kernel, &cfg, pick, seen, &clusters)) return rc;
-    if (clusters > units) clusters = units;
+    const int clusters = units < held.clusters[pick] ? units : held.clusters[pick];
     const size_t smem = smem_of(pick, pick_parts, cut.sg, groups, units, clusters, NT, R);
-    GI_REQUIRE(smem <= 224 * 1024, "gi_int4_linear: %d x %d is too large for %d rows on %d clusters of %d blocks", N, K, M, clusters, pick);
     if (smem > cfg.dynamicSmemBytes) cfg.dynamicSmemBytes = smem;
     cfg.gridDim = dim3(clusters, pick);
     cfg.numAttrs = gi_pdl_enabled() ? 2 : 1;
@@ -459,15 +477,24 @@ extern "C" int gi_int4_linear(const void* x, const void* tiles, void* out, int o
     const unsigned char* tp = (const unsigned char*)tiles;
     const int f32 = out_dtype == GI_DTYPE_F32;
     cudaStream_t s = (cudaStream_t)stream;
-    const Int4Cut cut = cut_of(M, N, K, glu, ranks, parts);
+    Int4Held held;
+    if (int rc = clusters_held(&held)) return rc;
+    const Int4Cut cut = cut_of(M, N, K, glu, ranks, parts, held);
     GI_REQUIRE(cut.ranks > 0, "gi_int4_linear: %d x %d is too large for %d rows (in %d blocks, %d parts)", N, K, M, ranks, parts);
-#define GI_I4(NT, GLU) launch_int4_linear<NT, GLU>(xp, tp, out, f32, M, N, K, cut, unit, ld_out, error_flag, s)
+#define GI_I4(NT, GLU) launch_int4_linear<NT, GLU>(xp, tp, out, f32, M, N, K, cut, held, unit, ld_out, error_flag, s)
     if (M <= 8) return glu ? GI_I4(1, true) : GI_I4(1, false);
     return glu ? GI_I4(2, true) : GI_I4(2, false);
 #undef GI_I4
 }
 
-// Whether gi_int4_linear takes a product of these sizes: 1 or 0.
+// Whether gi_int4_linear takes a product of these sizes on the current device: 1 or 0, or -1 if the device could not be asked.
 extern "C" int gi_int4_linear_takes(int M, int N, int K, int glu) {
-    return M >= 1 && M <= 16 && N > 0 && K > 0 && N < (1 << 30) && K < (1 << 30) && (!glu || N % 32 == 0) && cut_of(M, N, K, glu, 0, 0).ranks > 0;
+    Int4Held held;
+    if (clusters_held(&held)) return -1;
+    return M >= 1 && M <= 16 && N > 0 && K > 0 && N < (1 << 30) && K < (1 << 30) && (!glu || N % 32 == 0) && cut_of(M, N, K, glu, 0, 0, held).ranks > 0;
+}
+// What gi_int4_linear counts on: clusters of 1 to 8 blocks that the current device holds at once.
+extern "C" int gi_int4_linear_held(int ranks) {
+    Int4Held held;
+    return ranks < 1 || ranks > 8 || clusters_held(&held) ? -1 : held.clusters[ranks];
 }

@@ -116,6 +116,7 @@ _SIGNATURES = {
     "gi_int4_dequantize_weight": ([P, P, I, I, I, I, I, P], I),
     "gi_int4_linear": ([P, P, P, I, L, I, I, I, I, I, F, F, F, F, I, I, P, P], I),
     "gi_int4_linear_takes": ([I, I, I, I], I),
+    "gi_int4_linear_held": ([I], I),
     "gi_int4_append": ([P, L, L, P, L, L, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, P], I),
     "gi_int4_read": ([P, P, P, I, P, P, P, I, I, I, I, I, I, I, P, P], I),
     "gi_int4_gather": ([P, P, P, P, P, P, P, P, I, P, P, I, I, P, I, I, I, I, I, I, I, P, P], I),

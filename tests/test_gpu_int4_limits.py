@@ -107,3 +107,27 @@ def test_steps_of_few_rows_whose_sums_have_no_room_beside_them(ops, m, n, k, gat
         else:
             want, bound = y[0], off[0] + 2 ** -24 * y[0].abs()
         assert float(((got[:, a:a + 16].double() - want).abs() / bound).max()) <= 1
+
+
+def test_room_is_counted_with_the_clusters_that_the_device_holds(ops):
+    """What the choice of product counts on is what the launch is made with: whatever is stated to fit runs, at the edges of the room."""
+    l = ops.lib()
+    held = [l.gi_int4_linear_held(r) for r in range(1, 9)]
+    assert held[0] == torch.cuda.get_device_properties(0).multi_processor_count and all(0 < b * r <= held[0] for r, b in enumerate(held, 1))
+    assert l.gi_int4_linear_held(0) == l.gi_int4_linear_held(9) == -1
+    for m, k, gated in ((1, 16384, 1), (8, 16384, 1), (16, 4096, 0), (16, 8192, 1), (9, 28672, 0)):
+        unit = 32
+        low, high = 1, 8192                                  # outputs in units of 32: the last that fit, to within an eighth
+        assert l.gi_int4_linear_takes(m, low * unit, k, gated) == 1
+        while high - low > max(1, low // 8):
+            mid = (low + high) // 2
+            low, high = (mid, high) if l.gi_int4_linear_takes(m, mid * unit, k, gated) == 1 else (low, mid)
+        n = low * unit
+        tiles = torch.zeros(n // 16, k // 128, 1088, dtype=torch.uint8, device=DEV)
+        tiles[..., 1024:] = torch.tensor([0.01, 0.5], dtype=torch.bfloat16, device=DEV).view(torch.uint8).repeat(16)
+        w = ops.int4.Int4Weight(tiles, n, k)
+        x = torch.ones((m, k), dtype=torch.bfloat16, device=DEV)
+        unit_of = ops.kernels.glu_shape("silu") if gated else None
+        got = ops.int4.linear_rows(x, w, torch.float32, unit_of)
+        y = 0.5 * k                                          # every code is 0: sums of halves, exact in float32
+        assert torch.equal(got, torch.full_like(got, y * y if gated else y))
