@@ -61,6 +61,23 @@ __device__ __forceinline__ void i4l_wait(void* bar, uint32_t parity, volatile in
     __syncwarp();
 }
 
+// The end of a warp that gave up a wait: what is on its way into the block's shared memory lands before the block leaves (again with a limit).
+// First its ring's copies; the copying lane leaves 1 + their number in `left`.  Then other blocks' sums: those blocks' waits are bounded
+// too, and the barrier of the cluster counts who has left, so behind it all sums are under way and the count of bytes says when they are here.
+__device__ __noinline__ void i4l_leave(volatile int* left, uint64_t* full, uint64_t* arrived, bool owned, bool cluster) {
+    const bool first = (threadIdx.x & 31) == 0;
+    int never = 0;
+    if (first) {
+        int n = 0;
+        for (int i = 0; i < I4L_POLLS && n == 0; ++i) n = *left;
+        for (int j = max(0, n - 1 - I4L_STAGES); j < n - 1; ++j) t5_bar_wait(&full[j % I4L_STAGES], (j / I4L_STAGES) & 1, &never);
+    }
+    __syncwarp();
+    if (cluster) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    if (first && owned) t5_bar_wait(arrived, 0, &never);
+    __syncwarp();
+}
+
 // Eight consecutive inputs of a row of x from k on, zeros beyond K.  vec: K is a multiple of 8 and x starts on 16 bytes.
 __device__ __noinline__ uint4 i4l_load8_plain(const bf16* row, int k, int K) {
     uint32_t w[4];
@@ -100,7 +117,7 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
     extern __shared__ __align__(16) unsigned char i4_smem[];
     __shared__ __align__(8) uint64_t s_full[WARPS][I4L_STAGES], s_room[WARPS][I4L_STAGES], s_arrived, s_x;
     __shared__ uint32_t s_odd;                                           // rows of x that are summed the long way
-    __shared__ int s_abort;
+    __shared__ int s_abort, s_left[WARPS];                               // 1 + the copies of a ring, when its lane has left
     constexpr int R = GLU ? 2 : 1;                                       // rows of tiles of a unit
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     // blocks of a cluster lie along y and share K; cluster cl has units cl, cl + n_cl, ..: units_each, and one more of the first units_left
@@ -129,6 +146,7 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
     if (x_first && warp < WARPS) raw = load_x(warp);                     // no kernel before this one is still to write x
     if (warp == WARPS) {
         if (lane < WARPS) {
+            s_left[lane] = 0;
 #pragma unroll
             for (int i = 0; i < I4L_STAGES; ++i) t5_bar_init(&s_full[lane][i], 1), t5_bar_init(&s_room[lane][i], 1);
         }
@@ -178,6 +196,7 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
                 break;
             }
         }
+        if (w < WARPS) *(volatile int*)&s_left[w] = 1 + round * I4L_STAGES + slot;
         return;
     }
     gi_pdl_wait();
@@ -344,6 +363,7 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
             }
         }
     }
+    if (*(volatile int*)&s_abort) i4l_leave(&s_left[warp], s_full[warp], &s_arrived, owned > 0, ranks > 1);
 }
 
 // ------------------------------------------------------------------------------------------------ host

@@ -99,6 +99,7 @@ int4_linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const unsi
     __syncthreads();
     t5_fence_after();
     const uint32_t tmem = ctl->tmem;
+    int sent = 0;                                                              // copies, or groups multiplied, of this warp's role
 
     if (warp == 8) {
         // lane l asks for row l of the block's eight rows of tiles
@@ -109,8 +110,7 @@ int4_linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const unsi
         const int total = GLU ? 2 * min(4, have - first) : min(8, have - first);
         const unsigned char* src = tiles + ((size_t)(row + (GLU && lane >= 4 ? half : 0)) * groups + ga) * I4_TILE;
         const int copies = (n + I4W_SG - 1) / I4W_SG;
-        int i = 0;
-        for (; i < copies; ++i, src += I4W_SG * I4_TILE) {
+        for (int i = 0; i < copies; ++i, src += I4W_SG * I4_TILE, sent = i) {
             const int s = i % I4W_RING;
             const uint32_t bytes = min(I4W_SG, n - i * I4W_SG) * I4_TILE;
             if (i >= I4W_RING && !i4w_wait(&ctl->w_empty[s], (i / I4W_RING - 1) & 1, abort, error_flag, I4W_ERR_COPY)) break;
@@ -118,14 +118,9 @@ int4_linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const unsi
             __syncwarp();
             if (mine) i4w_copy(t5_smem(ring + s * I4W_STAGE + lane * I4W_ROW), src, bytes, t5_smem(&ctl->w_full[s]));
         }
-        if (i < copies && lane == 0) {                                         // gave up: the copies in flight land before the block leaves
-            int never = 0;
-            for (int j = max(0, i - I4W_RING); j < i; ++j) t5_bar_wait(&ctl->w_full[j % I4W_RING], (j / I4W_RING) & 1, &never);
-        }
     } else if (warp == 9) {
         gi_pdl_wait();
-        int i = 0;
-        for (; i < n; ++i) {
+        for (int i = 0; i < n; sent = ++i) {
             const int s = i % I4W_A;
             if (i >= I4W_A && !i4w_wait(&ctl->done[s], (i / I4W_A - 1) & 1, abort, error_flag, I4W_ERR_PRODUCT)) break;
             if (lane == 0) {
@@ -134,16 +129,11 @@ int4_linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const unsi
                 t5_load_2d(smem + s * X_BYTES + X_BYTES / 2, &map_x, (ga + i) * I4_GROUP_W + 64, m0, &ctl->x_full[s]);
             }
         }
-        if ((i < n || *abort) && lane == 0) {                                  // gave up: the copies in flight land before the block leaves
-            int never = 0;
-            for (int j = max(0, i - I4W_A); j < i; ++j) t5_bar_wait(&ctl->x_full[j % I4W_A], (j / I4W_A) & 1, &never);
-        }
     } else if (warp == 10) {
         // whole, so that the operands' addresses are known to be alike: issued by one lane of a divided warp, eight products took 650 cycles
         constexpr uint32_t idesc = t5_idesc(128, BN);
         const uint64_t xd = t5_desc<128>(t5_smem(smem));
-        int i = 0;
-        for (; i < n; ++i) {
+        for (int i = 0; i < n; sent = ++i) {
             const int s = i % I4W_A;
             if (!i4w_wait(&ctl->x_full[s], (i / I4W_A) & 1, abort, error_flag, I4W_ERR_PRODUCT)) break;
             if (!i4w_wait(&ctl->ready[s], (i / I4W_A) & 1, abort, error_flag, I4W_ERR_PRODUCT)) break;
@@ -239,6 +229,17 @@ int4_linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const unsi
     }
     if (ranks > 1) i4w_cluster_sync();                                         // the others have read this block's sums
     else __syncthreads();
+    if (*abort && warp >= 8) {
+        // some role gave up, perhaps when others had left theirs: copies in flight land, and products end, before the block leaves and its
+        // tensor memory is freed.  Warp 8's copies are counted by w_full, warp 9's by x_full, warp 10's products by done
+        if (lane == 0) {
+            int never = 0;
+            const int ring = warp == 8 ? I4W_RING : I4W_A;
+            unsigned long long* const bars = warp == 8 ? ctl->w_full : warp == 9 ? ctl->x_full : ctl->done;
+            for (int j = max(0, sent - ring); j < sent; ++j) t5_bar_wait(&bars[j % ring], (j / ring) & 1, &never);
+        }
+        __syncwarp();
+    }
     if (warp == 10) {
         t5_fence_after();
         t5_free(tmem, TMEM);
