@@ -325,10 +325,11 @@ int4_linear_kernel(const bf16* __restrict__ x, const unsigned char* __restrict__
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const float4 xm = *reinterpret_cast<const float4*>(xmeta + ((two ? gi + r : gi) * NT + nt) * 8 + 2 * t4);
-                    y[nt][0] = fmaf(l, xm.y, fmaf(s * xm.x, z[r][nt][0], y[nt][0]));
-                    y[nt][1] = fmaf(l, xm.w, fmaf(s * xm.z, z[r][nt][1], y[nt][1]));
-                    y[nt][2] = fmaf(l8, xm.y, fmaf(s8 * xm.x, z[r][nt][2], y[nt][2]));
-                    y[nt][3] = fmaf(l8, xm.w, fmaf(s8 * xm.z, z[r][nt][3], y[nt][3]));
+                    // z < 4 and xm.x < 2^126: their product is finite, a step times xm.x need not be
+                    y[nt][0] = fmaf(l, xm.y, fmaf(s, xm.x * z[r][nt][0], y[nt][0]));
+                    y[nt][1] = fmaf(l, xm.w, fmaf(s, xm.z * z[r][nt][1], y[nt][1]));
+                    y[nt][2] = fmaf(l8, xm.y, fmaf(s8, xm.x * z[r][nt][2], y[nt][2]));
+                    y[nt][3] = fmaf(l8, xm.w, fmaf(s8, xm.z * z[r][nt][3], y[nt][3]));
                 }
             }
         }

@@ -7,7 +7,7 @@ import torch
 
 import plain_int4 as plain
 import tiny
-from test_gpu_int4 import gen, randn, wide_bound
+from test_gpu_int4 import gen, linear_bound, randn, wide_bound
 from test_gpu_int4_model import HELD, load
 
 pytestmark = pytest.mark.gpu
@@ -131,3 +131,32 @@ def test_room_is_counted_with_the_clusters_that_the_device_holds(ops):
         got = ops.int4.linear_rows(x, w, torch.float32, unit_of)
         y = 0.5 * k                                          # every code is 0: sums of halves, exact in float32
         assert torch.equal(got, torch.full_like(got, y * y if gated else y))
+
+
+@pytest.mark.parametrize("m", [1, 8, 11])
+def test_large_inputs_and_steps_whose_product_is_no_number(ops, m):
+    """x up to 2^115, steps up to 2^20: what an output's codes leave of them is finite, and zero where they all are.  Bound: the
+    kernel's of test_gpu_int4.linear_bound, 8 roundings a group and the ends of sums whose numbers add up to A."""
+    g = gen(m)
+    n, k = 40, 300
+    codes = torch.zeros(n, k, dtype=torch.long, device=DEV)
+    codes[1::4, 3] = 1                                       # one input of one group
+    codes[2::4, 200:210] = 15
+    groups = 3
+    step = torch.full((n, groups), 2.0 ** 20, device=DEV)
+    step[2::4] = 2.0 ** 4
+    low = torch.zeros(n, groups, device=DEV)
+    low[3::4] = 1.0
+    w = ops.int4.Int4Weight(plain.pack_weight(codes, step, low), n, k)
+    x = torch.zeros(m, k, device=DEV)
+    x[:, 100] = 2.0 ** 115                                   # meets codes of 0, or the low value 1
+    x[:, 3] = randn(g, m) * 2.0 ** 100
+    x[:, 200:210] = (1 + torch.rand(m, 10, generator=g, device=DEV)) * 2.0 ** 114
+    x = x.to(torch.bfloat16)
+    wide = plain.values(*plain.unpack_weight(w), 128)
+    want = x.double() @ wide.t()
+    assert bool((want[:, 0::4] == 0).all()) and bool((want.abs() < 2.0 ** 126).all())
+    assert bool((want[:, 1::4] != 0).all()) and float(want[:, 2::4].abs().min()) > 2.0 ** 120
+    got = ops.linear(x, w, torch.float32).double()
+    assert bool(torch.isfinite(got).all()) and bool((got[:, 0::4] == 0).all())
+    assert float(((got - want).abs() / (linear_bound(x, w) + 2 ** -24 * want.abs() + 2.0 ** -126)).max()) <= 1
