@@ -11,7 +11,9 @@
 //   out^T [16 numbers x 8] += codes of V^T [16 x 16 keys] . (p_j * step_j)^T,   and  sum_j p_j * low_j beside it
 //
 // q goes in exactly (a scaled f16), p_j * step_j rounded to the 11 significant bits of an f16, scaled by a power of two that
-// follows the largest step so far; a probability of 2^-20 of the largest still has all of them.  Everything else is float32.
+// follows the largest step so far; a probability of 2^-20 of the largest still has all of them, 2^-10 with a step 2^10 below the
+// largest.  Steps further apart go in as several products of one range each, so that no key, seen or not, takes bits from others.
+// Everything else is float32.
 // The transposition that the second product needs of V (its 16-wide side runs along a row of the cache) is ldmatrix's, on half words of
 // four numbers; that of the probabilities is movmatrix.
 //
@@ -81,6 +83,8 @@ __device__ __forceinline__ void i4a_matrix_trans(uint32_t (&r)[4], uint32_t at) 
 }
 #define I4A_SLACK 8.f              // a score may lie this far (in powers of two) above the reference
 #define I4A_STEP_TOP 6             // the largest step so far is scaled to [2^6, 2^7): times 2^8 it stays below f16's largest number
+#define I4A_STEP_RANGE 10          // steps down to 2^-10 of it share its scale
+#define I4A_STEP_MOST 30           // the scale follows steps up to 2^31, so that sums of larger ones and of those near 1 are both float32 numbers
 
 // Where the warps of a block meet: [warp][column][D + 4] sums, [warp][column] maximum and weight, then the block's own maximum and weight of a
 // column; its sums lie in the first warp's place.
@@ -300,10 +304,15 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
     }
-    int vexp[G];                                                               // exponent of the largest step so far
-    float vscale[G], vlimit[G];                                                // what scales it to [2^6, 2^7); steps from here on outgrow it
+    // What scales the largest step so far (of those below 2^31) to [2^6, 2^7): 2^(6 - e), e its exponent; 0 while there is none.  A step
+    // shares this scale if it lies in [2^(e - 10), 2^(e + 1)).
+    float vscale[G];
+    auto step_exp = [&](int gr) { return vscale[gr] == 0.f ? -113 : I4A_STEP_TOP + 127 - (int)(__float_as_uint(vscale[gr]) >> 23); };
+    auto outside = [&](int gr, uint32_t step) {
+        return step + __float_as_uint(vscale[gr]) - ((uint32_t)(I4A_STEP_TOP - I4A_STEP_RANGE + 254) << 23) >= (uint32_t)(I4A_STEP_RANGE + 1) << 23;
+    };
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) vexp[gr] = -113, vscale[gr] = 0.f, vlimit[gr] = -1.f;
+    for (int gr = 0; gr < G; ++gr) vscale[gr] = 0.f;
 
     uint32_t matrix[G];                                                        // this lane's row of the four matrices of a group, K's and V's
 #pragma unroll
@@ -367,7 +376,6 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
                 for (int gr = 0; gr < G; ++gr) {
                     vs[gr][half] = i4_bf16_low(vm[gr]);
                     vo[gr][half] = i4_bf16_high(vm[gr]);
-                    moved |= vs[gr][half] >= vlimit[gr];
                 }
             }
             // ---- keys that a column does not see, and values there that are not finite
@@ -382,6 +390,13 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
                         if (j > p || (window > 0 && j <= p - window)) s[nt][e] = -INFINITY;
                     }
 #pragma unroll
+                for (int half = 0; half < 2; ++half) {                         // what no column sees has no value
+                    const int j = j0 + g + half * 8;
+                    if (j > hi || (window > 0 && j <= first - window))
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) vs[gr][half] = vo[gr][half] = 0.f;
+                }
+#pragma unroll
                 for (int gr = 0; gr < G; ++gr) odd |= !(vs[gr][0] <= 3.4e38f) || !(vs[gr][1] <= 3.4e38f) || !(fabsf(vo[gr][0]) <= 3.4e38f) || !(fabsf(vo[gr][1]) <= 3.4e38f);
                 odd = __any_sync(0xffffffffu, odd);
             }
@@ -389,17 +404,21 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) moved |= s[nt][e] > limit[nt][e & 1];
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+                moved |= !(fabsf(vs[gr][0] * vscale[gr] - 64.f) <= 63.9375f) || !(fabsf(vs[gr][1] * vscale[gr] - 64.f) <= 63.9375f);      // [2^-4, 2^7)
             // ---- a new reference for the columns' sums, or a new scale for the steps
+            uint32_t apart = 0;                                                // groups with steps of several ranges
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
                     const uint32_t b0 = __float_as_uint(vs[gr][0]), b1 = __float_as_uint(vs[gr][1]);      // never negative; NaN and infinities aside
                     const uint32_t most = __reduce_max_sync(0xffffffffu, max(b0 < 0x7F800000u ? b0 : 0u, b1 < 0x7F800000u ? b1 : 0u));
-                    const int e = max(max((int)(most >> 23) - 127, -112), vexp[gr]);
-                    const float grow = vexp[gr] < -112 ? 0.f : i4a_exp2((float)(vexp[gr] - e));      // nothing summed up yet: 0 times 0
-                    vexp[gr] = e;
+                    const int before = step_exp(gr), e = max(max(min((int)(most >> 23) - 127, I4A_STEP_MOST), -112), before);
+                    const float grow = before < -112 ? 0.f : i4a_exp2((float)(before - e));      // nothing summed up yet: 0 times 0
                     vscale[gr] = i4_pow2(I4A_STEP_TOP - e);
-                    vlimit[gr] = e < 127 ? i4_pow2(e + 1) : INFINITY;
+                    const bool far = (b0 != 0 && b0 < 0x7F800000u && outside(gr, b0)) || (b1 != 0 && b1 < 0x7F800000u && outside(gr, b1));
+                    apart |= __any_sync(0xffffffffu, far) ? 1u << gr : 0u;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -426,15 +445,65 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
                         for (int i = 0; i < G * 4; ++i) o[i][nt][e] *= corr, o[i][nt][e + 2] *= corr;
                     }
             }
-            // ---- probabilities
+            auto probabilities = [&]() {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    s[nt][e] = i4a_exp2(s[nt][e]);
-                    s[nt][e + 2] = i4a_exp2(s[nt][e + 2]);
-                    l[nt][e] += s[nt][e] + s[nt][e + 2];
-                }
+                    for (int e = 0; e < 2; ++e) {
+                        s[nt][e] = i4a_exp2(s[nt][e]);
+                        s[nt][e + 2] = i4a_exp2(s[nt][e + 2]);
+                        l[nt][e] += s[nt][e] + s[nt][e + 2];
+                    }
+            };
+            // a half's second operand, keys of its 8 rows, with their step scaled; what a column does not see stays out of it
+            auto operand = [&](int nt, int half, float step) {
+                const float p0 = s[nt][half * 2], p1 = s[nt][half * 2 + 1];
+                return i4a_transpose(i4_f16x2(p0 == 0.f ? 0.f : p0 * step, p1 == 0.f ? 0.f : p1 * step));
+            };
+            auto offsets = [&](int gr, int half, int nt) {
+                const float p0 = s[nt][half * 2], p1 = s[nt][half * 2 + 1];
+                off_sum[nt][gr][0] += p0 == 0.f ? 0.f : p0 * vo[gr][half];
+                off_sum[nt][gr][1] += p1 == 0.f ? 0.f : p1 * vo[gr][half];
+            };
+            // ---- steps of several ranges: one product for each, the largest first, brought to the sums' scale afterwards
+            if (apart || odd) {
+                probabilities();
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) offsets(gr, 0, nt), offsets(gr, 1, nt);
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr)
+#pragma unroll 1
+                    while (__any_sync(0xffffffffu, vs[gr][0] != 0.f || vs[gr][1] != 0.f)) {      // a step that has had its turn becomes 0
+                        const uint32_t b0 = __float_as_uint(vs[gr][0]), b1 = __float_as_uint(vs[gr][1]);
+                        const uint32_t most = __reduce_max_sync(0xffffffffu, max(b0 < 0x7F800000u ? b0 : 0u, b1 < 0x7F800000u ? b1 : 0u));
+                        const int e = max((int)(most >> 23) - 127, -112);
+                        const uint32_t from = e > -112 ? (uint32_t)(e - I4A_STEP_RANGE + 127) << 23 : 1u;
+                        const float scale = i4_pow2(I4A_STEP_TOP - e), up = i4a_exp2((float)(e - step_exp(gr)));
+                        uint32_t w[4], b[NT][2];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            b[nt][0] = operand(nt, 0, b0 >= from ? vs[gr][0] * scale : 0.f);      // NaN with the first
+                            b[nt][1] = operand(nt, 1, b1 >= from ? vs[gr][1] * scale : 0.f);
+                        }
+                        vs[gr][0] = b0 >= from ? 0.f : vs[gr][0], vs[gr][1] = b1 >= from ? 0.f : vs[gr][1];
+                        i4a_matrix_trans(w, sK + C::CODES + matrix[gr]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t a = w[i & 2] >> (i & 1) * 8, d = w[(i & 2) + 1] >> (i & 1) * 8;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                float z[4];
+                                i4_mma_first(z, a & I4_NEAR, a & I4_FAR, d & I4_NEAR, d & I4_FAR, b[nt][0], b[nt][1]);
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) o[gr * 4 + i][nt][x] = fmaf(z[x], up, o[gr * 4 + i][nt][x]);
+                            }
+                        }
+                    }
+                continue;
+            }
+            probabilities();
             // ---- out^T += codes of V^T . (p step)^T
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
@@ -445,16 +514,9 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const float p0 = s[nt][half * 2], p1 = s[nt][half * 2 + 1];
-                        float x0 = p0 * step, x1 = p1 * step;
-                        if (odd) {                                             // not to the columns that do not see it
-                            x0 = p0 == 0.f ? 0.f : x0, x1 = p1 == 0.f ? 0.f : x1;
-                            off_sum[nt][gr][0] += p0 == 0.f ? 0.f : p0 * vo[gr][half];
-                            off_sum[nt][gr][1] += p1 == 0.f ? 0.f : p1 * vo[gr][half];
-                        } else {
-                            off_sum[nt][gr][0] = fmaf(p0, vo[gr][half], off_sum[nt][gr][0]);
-                            off_sum[nt][gr][1] = fmaf(p1, vo[gr][half], off_sum[nt][gr][1]);
-                        }
-                        b[nt][half] = i4a_transpose(i4_f16x2(x0, x1));
+                        off_sum[nt][gr][0] = fmaf(p0, vo[gr][half], off_sum[nt][gr][0]);
+                        off_sum[nt][gr][1] = fmaf(p1, vo[gr][half], off_sum[nt][gr][1]);
+                        b[nt][half] = i4a_transpose(i4_f16x2(p0 * step, p1 * step));
                     }
                 }
                 // half words of numbers 4 g .. of keys 2 t, 2 t + 1; of keys 8 on; of numbers 32 + 4 g ..
@@ -495,8 +557,8 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
                 float f = off_sum[nt][gr][e];
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) f += __shfl_xor_sync(0xffffffffu, f, x);
-                // 2^(vexp - 6) for the steps' scale, 2^24 for the codes', in two factors of which neither overflows
-                const float back = vexp[gr] < -112 ? 0.f : i4_pow2(vexp[gr]);
+                // 2^(e - 6) for the steps' scale, 2^24 for the codes', in two factors of which neither overflows
+                const float back = vscale[gr] == 0.f ? 0.f : i4_pow2(step_exp(gr));
                 float* dst = so + (warp * COLS + cc) * LD + gr * 64 + 4 * g;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {                                  // numbers four bits up count 16 times

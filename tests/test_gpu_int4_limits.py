@@ -7,7 +7,7 @@ import torch
 
 import plain_int4 as plain
 import tiny
-from test_gpu_int4 import gen, linear_bound, randn, wide_bound
+from test_gpu_int4 import check_attention, gen, linear_bound, make_cache, randn, runs_and_blocks, wide_bound
 from test_gpu_int4_model import HELD, load
 
 pytestmark = pytest.mark.gpu
@@ -160,3 +160,82 @@ def test_large_inputs_and_steps_whose_product_is_no_number(ops, m):
     got = ops.linear(x, w, torch.float32).double()
     assert bool(torch.isfinite(got).all()) and bool((got[:, 0::4] == 0).all())
     assert float(((got - want).abs() / (linear_bound(x, w) + 2 ** -24 * want.abs() + 2.0 ** -126)).max()) <= 1
+
+
+# ------------------------------------------------------------------------------------------------ steps far apart
+def far_apart(ops, heads, kv, d, page, lengths, seed, huge, where):
+    """A filled cache whose values at the given (sequence, position) are `huge` times as large as the others."""
+    g = gen(seed)
+    k_rows, v_rows, table, status, k, v, pos, slot = make_cache(ops, g, lengths, kv, d, page)
+    starts = [sum(lengths[:s]) for s in range(len(lengths))]
+    for s, p in where:
+        v[starts[s] + p] *= huge
+    ops.int4.append(k, v, k_rows, v_rows, table, pos, slot, status)
+    return g, k_rows, v_rows, table, status
+
+
+@pytest.mark.parametrize("huge", [2.0 ** 20, 2.0 ** 40, 2.0 ** 100])
+@pytest.mark.parametrize("heads,d,page", [(4, 128, 64), (2, 64, 64), (12, 128, 16)])
+def test_large_values_behind_the_window_leave_no_trace(ops, heads, d, page, huge):
+    """Keys in front of the window lie in the first chunk of keys that is read: whatever their values' size, a token's result is as exact as
+    without them."""
+    window, n = 70, 300
+    first = n - window
+    g, k_rows, v_rows, table, status = far_apart(ops, heads, 1, d, page, [n, n], 41, huge, [(0, p) for p in range(first - 20, first)])
+    q = randn(g, 2, heads, d).to(torch.bfloat16)
+    pos, slot = torch.full((2,), n - 1, dtype=torch.int32, device=DEV), torch.arange(2, dtype=torch.int32, device=DEV)
+    for splits in (None, 1):
+        got = ops.int4.attention_decode(q, k_rows, v_rows, table, pos, slot, d ** -0.5, window, status, n_splits=splits)
+        check_attention(got, *plain.attention(q, k_rows, v_rows, table, [(0, 0, 1, n - 1), (1, 1, 1, n - 1)], d ** -0.5, window))
+
+
+@pytest.mark.parametrize("huge", [2.0 ** 20, 2.0 ** 40, 2.0 ** 100])
+@pytest.mark.parametrize("heads,kv,d,seqs", [(4, 1, 128, [(200, 4), (33, 2)]), (4, 2, 64, [(64, 3), (0, 5)]), (8, 1, 128, [(90, 6)])])
+def test_large_values_of_later_tokens_leave_no_trace(ops, heads, kv, d, seqs, huge):
+    """The tokens of a run in front of one with large values do not see it: their results are as exact as without it."""
+    where = [(s, p + n - 2 if n > 2 else p + n - 1) for s, (p, n) in enumerate(seqs)]
+    g, k_rows, v_rows, table, status = far_apart(ops, heads, kv, d, 64, [p + n for p, n in seqs], 43, huge, where)
+    spans, row = [], 0
+    for s, (p, n) in enumerate(seqs):
+        spans.append((s, row, n, p))
+        row += n
+    q = randn(g, row, heads, d).to(torch.bfloat16)
+    runs, blocks = runs_and_blocks(spans, 0)
+    got = ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, d ** -0.5, 0, status)
+    check_attention(got, *plain.attention(q, k_rows, v_rows, table, spans, d ** -0.5, 0))
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 30, 2.0 ** 60])
+@pytest.mark.parametrize("heads,d,at", [(4, 128, 3), (2, 64, 40), (16, 128, 255)])
+def test_a_large_value_with_hardly_any_weight_costs_the_others_nothing(ops, heads, d, at, ratio):
+    """One key's probability is 2^-69 or so of the others' and its values are `ratio` times as large: the others keep their bits."""
+    n = 256
+    g = gen(47)
+    k_rows, v_rows, table, status, k, v, pos, slot = make_cache(ops, g, [n], 1, d, 64)
+    q = torch.ones(1, heads, d, device=DEV).to(torch.bfloat16)
+    k *= 0.1
+    k[at] = -48.0 / d ** 0.5                                 # its score is 48 below the others'
+    v[at] *= ratio
+    ops.int4.append(k, v, k_rows, v_rows, table, pos, slot, status)
+    spans = [(0, 0, 1, n - 1)]
+    for splits in (None, 1):
+        got = ops.int4.attention_decode(q, k_rows, v_rows, table, pos[-1:], slot[:1], d ** -0.5, 0, status, n_splits=splits)
+        check_attention(got, *plain.attention(q, k_rows, v_rows, table, spans, d ** -0.5, 0))
+
+
+def test_values_of_all_sizes(ops):
+    """Every token's values are a power of two of their own, up and down over 2^40, seen by single tokens, short runs and their heads."""
+    heads, kv, d, n = 6, 2, 128, 400
+    g = gen(53)
+    k_rows, v_rows, table, status, k, v, pos, slot = make_cache(ops, g, [n, n], kv, d, 64)
+    v *= torch.exp2(torch.randint(-20, 21, (2 * n, 1, 1), generator=g, device=DEV).float()).to(torch.bfloat16)
+    ops.int4.append(k, v, k_rows, v_rows, table, pos, slot, status)
+    q = randn(g, 7, heads, d).to(torch.bfloat16)
+    spans = [(0, 0, 1, n - 1), (1, 1, 6, n - 6)]
+    at = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+    got = ops.int4.attention_decode(q[:1], k_rows, v_rows, table, at, slot[:1], d ** -0.5, 0, status)
+    check_attention(got, *plain.attention(q[:1], k_rows, v_rows, table, spans[:1], d ** -0.5, 0))
+    runs, blocks = runs_and_blocks(spans, 0)
+    got = ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, d ** -0.5, 0, status)
+    check_attention(got, *plain.attention(q, k_rows, v_rows, table, spans, d ** -0.5, 0))
+    assert int(status) == 0
