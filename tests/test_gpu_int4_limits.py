@@ -239,3 +239,79 @@ def test_values_of_all_sizes(ops):
     got = ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, d ** -0.5, 0, status)
     check_attention(got, *plain.attention(q, k_rows, v_rows, table, spans, d ** -0.5, 0))
     assert int(status) == 0
+
+
+# ------------------------------------------------------------------------------------------------ prompts, held tightly
+def wide_attention(q, k_rows, v_rows, table, spans, scale, window):
+    """What the gathered path computes: softmax over keys and values rounded to bfloat16, and how far it may be off.
+
+    The bound, per number: 2^-8 of it (its own rounding); 2^-8 of sum p |v| / sum p (probabilities rounded to bfloat16); float32 sums
+    over n keys, 2^-24 of sum p |v| / sum p for each of n / 16 products in turn and 64 at the ends; scores: d / 16 + 8 roundings of
+    2^-24 of sum |q| |k| and 2^-22 of exp2, which the result sees twice."""
+    n, n_q, d = q.shape
+    out = torch.zeros(n, n_q * d, dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(out)
+    for slot, row, count, past in spans:
+        k, v = (plain.values(*plain.sequence(rows, table[slot], past + count), 64).to(torch.bfloat16).double() for rows in (k_rows, v_rows))
+        i, j = torch.arange(past, past + count, device=q.device)[:, None], torch.arange(past + count, device=q.device)[None]
+        hidden = (j > i) | ((j <= i - window) if window else torch.zeros_like(j > i))
+        for h in range(n_q):
+            e = h // (n_q // k.shape[0])
+            x = q[row:row + count, h].double()
+            p = torch.softmax((x @ k[e].t() * scale).masked_fill(hidden, -float("inf")), dim=1)
+            cols = slice(h * d, (h + 1) * d)
+            o, size = p @ v[e], p @ v[e].abs()
+            off = ((d / 16 + 8) * 2 ** -24 * 1.4427 * scale * (x.abs() @ k[e].abs().t()).masked_fill(hidden, 0.0)).amax(1, keepdim=True) + 2 ** -22
+            out[row:row + count, cols] = o
+            bound[row:row + count, cols] = 2 ** -8 * o.abs() + (2 ** -8 + ((past + count) / 16 + 64) * 2 ** -24 + 2 * off) * size
+    return out, bound
+
+
+TIGHT = [
+    # heads, kv heads, d, page, (cached, new), window
+    (4, 2, 128, 64, [(0, 1)], 0),
+    (4, 1, 64, 16, [(0, 5), (30, 1), (100, 3)], 0),
+    (8, 2, 128, 64, [(500, 4), (64, 4), (0, 2)], 0),
+    (5, 1, 128, 32, [(700, 5), (0, 17)], 40),
+    (6, 2, 64, 7, [(90, 9), (333, 3), (5, 20)], 0),
+    (16, 1, 128, 128, [(250, 5), (129, 2)], 100),
+    (24, 2, 64, 64, [(1000, 3), (33, 8), (64, 1)], 64),
+    (3, 1, 64, 1, [(70, 31)], 1),
+    (32, 8, 128, 64, [(0, 300), (200, 130)], 0),
+    (6, 3, 64, 64, [(0, 129), (1000, 64), (60, 70)], 0),
+    (4, 2, 128, 16, [(300, 200), (0, 40)], 100),
+    (16, 1, 64, 7, [(90, 33), (0, 64)], 0),
+    (8, 1, 128, 64, [(127, 200), (64, 64)], 65),
+    (4, 1, 64, 32, [(0, 128), (511, 140)], 300),
+]
+
+
+@pytest.mark.parametrize("heads,kv,d,page,seqs,window", TIGHT)
+def test_prompts_are_held_to_their_own_path(ops, heads, kv, d, page, seqs, window):
+    """Runs that read codes are held to the codes' numbers, gathered ones to these rounded to bfloat16; an oracle with a key too many, a
+    key too few, queries one position early or a scale of 0.95 is told apart by the same bounds."""
+    g = gen(heads + 3 * d + page + len(seqs))
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [p + n for p, n in seqs], kv, d, page)
+    spans, row = [], 0
+    for s, (p, n) in enumerate(seqs):
+        spans.append((s, row, n, p))
+        row += n
+    q = (1.5 * randn(g, row, heads, d)).to(torch.bfloat16)
+    runs, blocks = runs_and_blocks(spans, window)
+    got = ops.int4.attention_prompt(q, k_rows, v_rows, table, runs, blocks, d ** -0.5, window, status).double()
+    few = -(-row * (heads // kv) // len(runs)) <= ops.int4.FEW_COLUMNS
+    oracle = plain.attention if few else wide_attention
+    worst = lambda **other: float(((got - (w := oracle(**{**dict(q=q, k_rows=k_rows, v_rows=v_rows, table=table, spans=spans, scale=d ** -0.5,
+                                                                 window=window), **other}))[0]).abs() / (w[1] + 1e-30)).max())
+    assert int(status) == 0 and worst() <= 1
+    if max(p + n for p, n in seqs) > 1:
+        assert worst(scale=0.95 * d ** -0.5) > 1 or window == 1
+        early = [(s, r, n, p - 1) for s, r, n, p in spans if p]
+        if early:
+            only = torch.zeros_like(got, dtype=torch.bool)
+            for s, r, n, p in early:
+                only[r:r + n] = True
+            o, b = oracle(q, k_rows, v_rows, table, early, d ** -0.5, window)
+            assert float(((got - o).abs() / (b + 1e-30))[only].max()) > 1
+    if window:
+        assert worst(window=window + 1) > 1 and (window == 1 or worst(window=window - 1) > 1)
