@@ -220,19 +220,22 @@ int4_read_kernel(Int4Pool pool, T* __restrict__ out, const int* __restrict__ tab
 
 // Blocks of 64 positions of the step's sequences as bfloat16 pages of their own, [blocks, n_kv, 64, d], for the prompt kernel on
 // tensor memory, and their block table [n_slots, max_blocks]: block i holds positions 64 b .. of the slot that blocks[i] =
-// {slot, b} names.  Positions without a page are zeros, as are those behind the table's last column.  runs_out: the runs, those that name a slot, rows or
-// positions that do not exist as empty ones (the prompt kernel takes them as they are).
+// {slot, b} names.  Positions without a page are zeros, as are those behind the table's last column; one that a run sees is reported.  runs_out: the
+// runs, those that name a slot, rows or positions that do not exist as empty ones (the prompt kernel takes them as they are).
 __global__ void __launch_bounds__(I4R_THREADS)
 int4_gather_kernel(Int4Pool kp, Int4Pool vp, bf16* __restrict__ k_out, bf16* __restrict__ v_out, int* __restrict__ out_table,
                    const int2* __restrict__ blocks, const int4* __restrict__ runs, int4* __restrict__ runs_out, int n_runs, int n_rows,
                    const int* __restrict__ table, int n_kv, int groups, int n_slots, int max_pages, int max_blocks, int page_size,
-                   int n_pages, int* __restrict__ status) {
+                   int n_pages, int window, int* __restrict__ status) {
     gi_pdl_start();
+    auto run_there = [&](int4 r) {
+        return r.x < n_slots && r.y >= 0 && r.z <= 128 && r.z <= n_rows && r.y <= n_rows - r.z && r.w >= 0 && r.w <= 2147483647 - 128 &&
+               (r.w + r.z - 1) / page_size < max_pages;
+    };
     if (blockIdx.x == 0 && blockIdx.y == 0)
         for (int i = threadIdx.x; i < n_runs; i += I4R_THREADS) {
             int4 r = runs[i];
-            const bool there = r.x < n_slots && r.y >= 0 && r.z <= 128 && r.z <= n_rows && r.y <= n_rows - r.z && r.w >= 0 &&
-                               r.w <= 2147483647 - 128 && (r.w + r.z - 1) / 64 < max_blocks;
+            const bool there = run_there(r);
             if (r.x >= 0 && r.z > 0 && !there) atomicExch(status, 4);
             if (r.x < 0 || r.z <= 0 || !there) r = make_int4(-1, 0, 0, 0);
             runs_out[i] = r;
@@ -257,6 +260,14 @@ int4_gather_kernel(Int4Pool kp, Int4Pool vp, bf16* __restrict__ k_out, bf16* __r
                 const size_t at = (((size_t)page * n_kv + head) * page_size + (pos - lp * page_size)) * groups + grp;
                 bits = reinterpret_cast<const uint2*>(pool.codes)[at * 4 + l];
                 meta = pool.meta[at];
+            } else if (blockIdx.y == 0 && l == 0 && grp == 0) {                // of the first head's keys: is it one that a run sees?
+                for (int j = 0; j < n_runs; ++j) {
+                    const int4 r = runs[j];
+                    if (r.x == b.x && r.z > 0 && run_there(r) && pos < r.w + r.z && (window == 0 || pos > r.w - window)) {
+                        atomicExch(status, 5);
+                        break;
+                    }
+                }
             }
         }
         i4r_unpack(out + (size_t)i * 16, bits, meta);
@@ -343,16 +354,17 @@ extern "C" int gi_int4_read(const void* codes, const void* meta, void* out, int 
 
 extern "C" int gi_int4_gather(const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, void* k_out, void* v_out,
                               int* out_table, const int* blocks, int n_blocks, const int* runs, int* runs_out, int n_runs, int n_rows, const int* table, int n_kv, int d, int n_slots,
-                              int max_pages, int max_blocks, int page_size, int n_pages, int* status, void* stream) {
+                              int max_pages, int max_blocks, int page_size, int n_pages, int window, int* status, void* stream) {
     if (int rc = check_pool("gi_int4_gather", k_codes, k_meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
     if (int rc = check_pool("gi_int4_gather", v_codes, v_meta, n_kv, d, page_size, max_pages, n_slots)) return rc;
     GI_REQUIRE(n_blocks >= 0 && max_blocks > 0 && n_kv <= 32767 && (uintptr_t)blocks % 8 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                "gi_int4_gather: %d blocks of %d heads; blocks must start on 8 bytes, the pages on 16", n_blocks, n_kv);
+    GI_REQUIRE(window >= 0, "gi_int4_gather: a window of %d", window);
     GI_REQUIRE(n_blocks > 0 && n_runs >= 0 && n_rows >= 0 && (uintptr_t)runs % 16 == 0 && (uintptr_t)runs_out % 16 == 0,
                "gi_int4_gather: %d runs over %d blocks; runs must start on 16 bytes", n_runs, n_blocks);
     const Int4Pool kp = {(unsigned char*)k_codes, (uint32_t*)k_meta}, vp = {(unsigned char*)v_codes, (uint32_t*)v_meta};
     gi_launch(int4_gather_kernel, dim3((unsigned)n_blocks, (unsigned)(2 * n_kv)), dim3(I4R_THREADS), 0, (cudaStream_t)stream, kp, vp, (bf16*)k_out,
               (bf16*)v_out, out_table, (const int2*)blocks, (const int4*)runs, (int4*)runs_out, n_runs, n_rows, table, n_kv, d / I4_GROUP_KV, n_slots, max_pages, max_blocks, page_size,
-              n_pages, status);
+              n_pages, window, status);
     return gi_check_launch("gi_int4_gather");
 }

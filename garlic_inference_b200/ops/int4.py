@@ -400,5 +400,6 @@ def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
     pages = q.new_empty((2, n_blocks, heads, 64, d))
     new_table = block_table.new_full((n_slots, max_blocks), -1)
     check(l.gi_int4_gather(*pools, pages[0].data_ptr(), pages[1].data_ptr(), new_table.data_ptr(), blocks_at, n_blocks, runs_at,
-                           kept.data_ptr(), n_runs, n, table[0], heads, d, n_slots, width, max_blocks, page_size, n_pages, _status(dev, status), _stream(dev)), l)
+                           kept.data_ptr(), n_runs, n, table[0], heads, d, n_slots, width, max_blocks, page_size, n_pages, window,
+                           _status(dev, status), _stream(dev)), l)
     return kernels.attention_prefill_tcgen05(q, pages[0], pages[1], new_table, kept, scale, window)

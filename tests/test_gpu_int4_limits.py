@@ -315,3 +315,39 @@ def test_prompts_are_held_to_their_own_path(ops, heads, kv, d, page, seqs, windo
             assert float(((got - o).abs() / (b + 1e-30))[only].max()) > 1
     if window:
         assert worst(window=window + 1) > 1 and (window == 1 or worst(window=window - 1) > 1)
+
+
+@pytest.mark.parametrize("window", [0, 90])
+def test_long_runs_report_pages_that_are_missing(ops, window):
+    """Gathered prompts say what those that read codes say: a page missing that some row sees is reported; in front of the window and
+    behind the end there need be none, and a run that goes beyond the table is left out."""
+    g = gen(61)
+    heads, kv, d, page, n = 8, 1, 64, 16, 40
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [230, 60], kv, d, page)
+    q = randn(g, 2 * n, heads, d).to(torch.bfloat16)
+    spans = [(0, 0, n, 190), (1, n, n, 20)]
+    runs, blocks = runs_and_blocks(spans, window)
+    call = lambda t, r=runs: ops.int4.attention_prompt(q, k_rows, v_rows, t, r, blocks, d ** -0.5, window, status)
+    want = call(table)
+    assert 2 * n * heads // 2 > ops.int4.FEW_COLUMNS and int(status) == 0
+    unseen = table.clone()
+    if window:
+        unseen[0, :(190 - window + 1) // page] = -1
+        assert torch.equal(call(unseen), want) and int(status) == 0
+    first = (190 - window + 1) // page if window else 0
+    for slot, p in ((0, first), (0, 229 // page), (0, 160 // page), (1, 0), (1, 59 // page)):
+        for value in (-1, 100000):
+            missing = unseen.clone()
+            missing[slot, p] = value
+            got = call(missing)
+            assert int(status) == 5, (slot, p)
+            status.zero_()
+            rows = slice(n, 2 * n) if slot == 0 else slice(0, n)
+            assert torch.equal(got[rows], want[rows])
+    # a table of 15 pages of 16: position 240 lies beyond it, though in its last block of 64
+    beyond = runs.clone()
+    at = int((runs[:, 0] == 0).nonzero()[0])
+    beyond[at, 3] = 240 - n + 1
+    narrow = table[:, :15].contiguous()
+    got = call(narrow, beyond)
+    assert int(status) == 4 and not bool(got[:n].any()) and torch.equal(got[n:], want[n:])
