@@ -137,8 +137,9 @@ __device__ __forceinline__ void tg_store_row(void* out, const uint32_t (&r)[32],
     }
 }
 
-// 32 columns of silu(gate) * up of one row: both factors rounded to bfloat16 as a stored product would be,
+// 32 columns of silu(gate) * up of one row: both factors rounded to bfloat16 as a stored product would be (or, KEEP, left in float32),
 // then the SwiGLU kernel's float32 arithmetic, rounded once
+template <bool KEEP>
 __device__ __forceinline__ void tg_store_swiglu(bf16* out, const uint32_t (&g)[32], const uint32_t (&u)[32], int row, int col,
                                                 int M, int inter, const GluShape& unit, long long ld_out) {
     if (row >= M || col >= inter) return;
@@ -152,8 +153,9 @@ __device__ __forceinline__ void tg_store_swiglu(bf16* out, const uint32_t (&g)[3
             float v[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float gf = __bfloat162float(__float2bfloat16_rn(__uint_as_float(g[j + e + h])));
-                const float uf = __bfloat162float(__float2bfloat16_rn(__uint_as_float(u[j + e + h])));
+                const float gr = __uint_as_float(g[j + e + h]), ur = __uint_as_float(u[j + e + h]);
+                const float gf = KEEP ? gr : __bfloat162float(__float2bfloat16_rn(gr));
+                const float uf = KEEP ? ur : __bfloat162float(__float2bfloat16_rn(ur));
                 v[h] = glu_unit(gf, uf, unit);
             }
             __nv_bfloat162 p = __floats2bfloat162_rn(v[0], v[1]);
@@ -468,7 +470,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                     uint32_t g[32], u[32];
                     tg_ld32(acc + c * 32, g);
                     tg_ld32(acc + TP_BN_HALF + c * 32, u);
-                    tg_store_swiglu(reinterpret_cast<bf16*>(out), g, u, row, col0 + c * 32, M, inter, unit, ld_out);
+                    tg_store_swiglu<SWIGLU == 2>(reinterpret_cast<bf16*>(out), g, u, row, col0 + c * 32, M, inter, unit, ld_out);
                 }
             } else {
                 const int n0 = (t / m_tiles) * TG_BN;
@@ -608,7 +610,7 @@ extern "C" int gi_gemm_tcgen05_bf16(const void* x, const void* W, void* out, int
 // out[M, I] = silu(x . Wg^T) * (x . Wu^T) for W = [Wg; Wu] of 2 I rows: the gate/up product of a SwiGLU
 // feed-forward with the activation in its epilogue, on pairs of CTAs.  bfloat16 in and out.
 static int tcgen05_glu_entry(const void* x, const void* W, void* out, int M, int two_inter, int K, int* error_flag,
-                             void* stream, GluShape unit, long long ld_out) {
+                             void* stream, GluShape unit, long long ld_out, bool keep = false) {
     GI_REQUIRE(M > 0 && two_inter > 0 && K > 0, "gi_gemm_tcgen05_swiglu_bf16: sizes must be positive");
     GI_REQUIRE(two_inter % 2 == 0, "gi_gemm_tcgen05_swiglu_bf16: W has %d rows, which cannot be a gate and an up half", two_inter);
     GI_REQUIRE(K % 8 == 0, "gi_gemm_tcgen05_swiglu_bf16: inner size %d is no multiple of 8 (rows must be a multiple of 16 bytes for TMA)", K);
@@ -629,12 +631,8 @@ static int tcgen05_glu_entry(const void* x, const void* W, void* out, int M, int
     if (int rc = tg_make_map(&map_x, x, M, K, TG_BM)) return rc;
     if (int rc = tg_make_map(&map_w, W, two_inter, K, TP_BN_HALF)) return rc;
     const size_t smem = (size_t)TP_STAGES * (TG_A_BYTES + TP_B_BYTES) + sizeof(TpControl) + 1024;
-    static bool attr_done = false;
-    if (!attr_done) {
-        cudaError_t e = cudaFuncSetAttribute((const void*)gemm_tcgen05_pair_kernel<0, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) { gi_set_error("gi_gemm_tcgen05_swiglu_bf16: shared memory: %s", cudaGetErrorString(e)); return (int)e; }
-        attr_done = true;
-    }
+    const auto kernel = keep ? gemm_tcgen05_pair_kernel<0, 2> : gemm_tcgen05_pair_kernel<0, 1>;
+    if (int rc = gi_reserve_smem((const void*)kernel, smem, "gi_gemm_tcgen05_swiglu_bf16")) return rc;
     const long long pairs = tiles < n_sm / 2 ? tiles : n_sm / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
@@ -650,7 +648,7 @@ static int tcgen05_glu_entry(const void* x, const void* W, void* out, int M, int
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = gi_pdl_enabled() ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_tcgen05_pair_kernel<0, 1>, map_x, map_w, out, M, two_inter, K, error_flag, unit, ld_out);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, out, M, two_inter, K, error_flag, unit, ld_out);
     if (e != cudaSuccess) { gi_set_error("gi_gemm_tcgen05_swiglu_bf16: launch: %s", cudaGetErrorString(e)); return (int)e; }
     return gi_check_launch("gi_gemm_tcgen05_swiglu_bf16");
 }
@@ -661,11 +659,12 @@ extern "C" int gi_gemm_tcgen05_swiglu_bf16(const void* x, const void* W, void* o
                              two_inter / 2);
 }
 
-// The same with any gated unit of glu.cuh (activation `kind`, limits, shift) and output rows `ld_out` apart.
+// The same with any gated unit of glu.cuh (activation `kind`, limits, shift) and output rows `ld_out` apart.  keep: gate and up are
+// not rounded to bfloat16 in front of the unit.
 extern "C" int gi_gemm_tcgen05_glu_bf16(const void* x, const void* W, void* out, long long ld_out, int M, int two_inter, int K,
-                                        int kind, float alpha, float gate_max, float up_limit, float up_shift,
+                                        int kind, float alpha, float gate_max, float up_limit, float up_shift, int keep,
                                         int* error_flag, void* stream) {
     GI_REQUIRE(kind >= 0 && kind <= 2 && up_limit >= 0.f, "gi_gemm_tcgen05_glu_bf16: gated unit %d", kind);
     return tcgen05_glu_entry(x, W, out, M, two_inter, K, error_flag, stream, GluShape{kind, alpha, gate_max, up_limit, up_shift},
-                             ld_out);
+                             ld_out, keep != 0);
 }

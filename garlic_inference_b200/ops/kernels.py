@@ -1360,13 +1360,13 @@ def gemm_skinny_glu_bf16(x: torch.Tensor, w_gate_up: torch.Tensor, unit: tuple, 
 
 
 def gemm_tcgen05_glu_bf16(x: torch.Tensor, w_gate_up: torch.Tensor, unit: tuple,
-                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                          out: Optional[torch.Tensor] = None, keep: bool = False) -> torch.Tensor:
     """unit(x . Wg^T, x . Wu^T) with the gated unit (a `glu_shape` tuple) in the epilogue of the tcgen05 product
     (pairs of CTAs); `out` may be columns of a wider matrix that start on 16 bytes.  The bits of
-    `glu(gemm_tcgen05_bf16(x, w_gate_up), unit)`."""
+    `glu(gemm_tcgen05_bf16(x, w_gate_up), unit)`, whose product is rounded to bfloat16; `keep`: it stays in float32."""
     l = require_gpu()
     m, n2, k, out = _glu_out(x, w_gate_up, out)
-    check(l.gi_gemm_tcgen05_glu_bf16(_ptr(x), _ptr(w_gate_up), _ptr(out), out.stride(0), m, n2, k, *unit,
+    check(l.gi_gemm_tcgen05_glu_bf16(_ptr(x), _ptr(w_gate_up), _ptr(out), out.stride(0), m, n2, k, *unit, int(keep),
                                      _ptr(tcgen05_error_flag(x.device)), _stream()), l)
     return out
 

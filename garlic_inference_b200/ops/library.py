@@ -101,7 +101,7 @@ _SIGNATURES = {
     "gi_gemv_swiglu_bf16": ([P, P, P, I, I, P], I),
     "gi_gemm_skinny_swiglu_bf16": ([P, P, P, I, I, I, I, I, P], I),
     "gi_gemm_skinny_glu_bf16": ([P, P, P, L, I, I, I, I, F, F, F, F, I, I, P], I),
-    "gi_gemm_tcgen05_glu_bf16": ([P, P, P, L, I, I, I, I, F, F, F, F, P, P], I),
+    "gi_gemm_tcgen05_glu_bf16": ([P, P, P, L, I, I, I, I, F, F, F, F, I, P, P], I),
     "gi_gemm_tcgen05_swiglu_bf16": ([P, P, P, I, I, I, P, P], I),
     "gi_gemm_streamk_bf16": ([P, P, P, I, I, I, I, P, P, P, P], I),
     "gi_gemm_streamk_workspace_floats": ([], L),

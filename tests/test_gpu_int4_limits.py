@@ -351,3 +351,32 @@ def test_long_runs_report_pages_that_are_missing(ops, window):
     narrow = table[:, :15].contiguous()
     got = call(narrow, beyond)
     assert int(status) == 4 and not bool(got[:n].any()) and torch.equal(got[n:], want[n:])
+
+
+# ------------------------------------------------------------------------------------------------ gated units of long prompts
+def unit_bound(x, w, want, gate, up):
+    """A unit of long prompts: the weight's numbers rounded to bfloat16 (wide_bound), the unit in float32 (|silu'| <= 1.1, silu within 2^-19 of
+    itself), its result rounded to bfloat16.  No rounding of gate and up in between."""
+    off, inter = wide_bound(x, w), gate.shape[1]
+    return 2 ** -8 * want.abs() + 1.1 * off[:, :inter] * (up.abs() + off[:, inter:]) + gate.abs() * off[:, inter:] + 2 ** -19 * (gate * up).abs() + 2 ** -30
+
+
+def test_gate_and_up_of_a_long_prompt_are_not_rounded(ops):
+    """Weights of whole numbers, exact in bfloat16, and inputs of whole numbers: every product is exact, and the unit's result the bfloat16
+    next to its 64-bit value (or one step off where float32 lies on the other side of a half)."""
+    g = gen(71)
+    m, inter, k = 400, 96, 256
+    codes = torch.randint(0, 16, (2 * inter, k), generator=g, device=DEV)
+    step, low = torch.ones(2 * inter, 2, device=DEV), torch.full((2 * inter, 2), -7.0, device=DEV)
+    w = ops.int4.Int4Weight(plain.pack_weight(codes, step, low), 2 * inter, k)
+    x = torch.randint(-15, 16, (m, k), generator=g, device=DEV).to(torch.bfloat16)
+    y = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    gate, up = y.chunk(2, 1)
+    assert float((gate.to(torch.bfloat16).double() != gate).double().mean()) > 0 and float(y.abs().max()) < 2 ** 24
+    want = gate * torch.sigmoid(gate) * up
+    got = ops.swiglu_product(x, w).double()
+    assert float(((got - want).abs() / (2 ** -8 * want.abs() * (1 + 2 ** -10) + 2 ** -30)).max()) <= 1
+    # rounding both factors first would be told apart
+    gate, up = (t.to(torch.bfloat16).double() for t in (gate, up))
+    other = (gate * torch.sigmoid(gate) * up).to(torch.bfloat16).double()      # as such a kernel would give it
+    assert float(((other - want).abs() / (2 ** -8 * want.abs() + 2 ** -30)).max()) > 1
