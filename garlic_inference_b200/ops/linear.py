@@ -106,7 +106,9 @@ def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Opt
             int4.linear_wide(even[r:r + INT4_CODES_MAX_ROWS], w, out_dtype, unit, out[r:r + INT4_CODES_MAX_ROWS])
         return out
     if unit is not None:
-        return kernels.gemm_tcgen05_glu_bf16(x, int4.dequantize_weight(w), unit, out=out, keep=True)
+        straight = out.data_ptr() % 16 == 0                  # the product stores from 16 bytes on; other columns get a copy
+        y = kernels.gemm_tcgen05_glu_bf16(x, int4.dequantize_weight(w), unit, out=out if straight else None, keep=True)
+        return out if straight else out.copy_(y)
     per = max(256, INT4_WIDE_BYTES // (w.k * x.element_size()) // 256 * 256)
     for a in range(0, w.n, per):
         b = min(per, w.n - a)

@@ -380,3 +380,21 @@ def test_gate_and_up_of_a_long_prompt_are_not_rounded(ops):
     gate, up = (t.to(torch.bfloat16).double() for t in (gate, up))
     other = (gate * torch.sigmoid(gate) * up).to(torch.bfloat16).double()      # as such a kernel would give it
     assert float(((other - want).abs() / (2 ** -8 * want.abs() + 2 ** -30)).max()) > 1
+
+
+@pytest.mark.parametrize("first,more", [(1, 5), (8, 0), (3, 13), (0, 7)])
+@pytest.mark.parametrize("m", [5, 40, 385, 600])
+def test_units_into_columns_that_start_anywhere(ops, m, first, more):
+    """`out` may be any columns of a wider matrix, whatever the rows: the numbers of a result of its own, and nothing beside them."""
+    g = gen(m + first)
+    inter, k = 208, 256
+    w = ops.int4.quantize_weight(randn(g, 2 * inter, k) * 0.06)
+    x = randn(g, m, k).to(torch.bfloat16)
+    wide = torch.full((m, first + inter + more), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = ops.glu_product(x, w, ops.kernels.glu_shape("silu"), out=wide[:, first:first + inter])
+    assert got.data_ptr() == wide[:, first:].data_ptr() and torch.equal(got, ops.swiglu_product(x, w))
+    assert bool((wide[:, :first] == 7).all()) and bool((wide[:, first + inter:] == 7).all())
+    y = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    gate, up = y.chunk(2, 1)
+    want = gate * torch.sigmoid(gate) * up
+    assert float(((got.double() - want).abs() / unit_bound(x, w, want, gate, up)).max()) <= 1
