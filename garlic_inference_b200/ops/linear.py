@@ -73,6 +73,10 @@ def _streamk_min_bytes(m: int) -> int:
 # 24,576 x 4,096 105 / 122, 6,144 x 4,096 28 / 39; 512 rows 155 / 126, 53 / 40, 4,096 x 12,288 60 / 84.
 INT4_CODES_MAX_ROWS = 384
 INT4_WIDE_BYTES = 64 << 20        # of a weight made wide at a time: it stays in L2 between the two kernels
+# The same of a gate and an up half, a bound on the work space alone: pieces that stay in L2 lose more in launches and in products' last tiles
+# than they save (2,048 rows of 2 x 12,288 x 4,096 whole 345 us, in pieces of 64 MB 365; 512 rows 137 and 186; 512 rows of 2 x 28,672 x 8,192
+# whole 580, in two pieces 650).
+INT4_GATED_BYTES = 1 << 30
 
 
 def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Optional[tuple] = None,
@@ -107,8 +111,15 @@ def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Opt
         return out
     if unit is not None:
         straight = out.data_ptr() % 16 == 0                  # the product stores from 16 bytes on; other columns get a copy
-        y = kernels.gemm_tcgen05_glu_bf16(x, int4.dequantize_weight(w), unit, out=out if straight else None, keep=True)
-        return out if straight else out.copy_(y)
+        to = out if straight else torch.empty((m, n), dtype=x.dtype, device=x.device)
+        per = _gated_columns(n, w.k)
+        wide = torch.empty((2 * min(per, n), w.k), dtype=x.dtype, device=x.device)
+        for a in range(0, n, per):                           # a gate's outputs and the up half's that meet them
+            b = min(per, n - a)
+            int4.dequantize_weight(w, x.dtype, a, b, out=wide[:b])
+            int4.dequantize_weight(w, x.dtype, n + a, b, out=wide[b:2 * b])
+            kernels.gemm_tcgen05_glu_bf16(x, wide[:2 * b], unit, out=to[:, a:a + b], keep=True)
+        return out if straight else out.copy_(to)
     per = max(256, INT4_WIDE_BYTES // (w.k * x.element_size()) // 256 * 256)
     for a in range(0, w.n, per):
         b = min(per, w.n - a)
@@ -120,6 +131,13 @@ def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Opt
         else:
             out[:, a:a + b] = kernels.gemm_tcgen05_bf16(x, wide, out_dtype)
     return out
+
+
+def _gated_columns(n: int, k: int) -> int:
+    """How many of a gated unit's n outputs are made wide at a time: whole tiles of 128, INT4_GATED_BYTES of gate and up at most (or one tile),
+    in pieces as equal as that lets them be."""
+    most = max(1, INT4_GATED_BYTES // (4 * k * 128)) * 128
+    return n if n <= most else min(most, -(-n // (-(-n // most) * 128)) * 128)
 
 
 def _narrow(y: torch.Tensor, out: torch.Tensor) -> torch.Tensor:

@@ -7,7 +7,7 @@ import torch
 
 import plain_int4 as plain
 import tiny
-from test_gpu_int4 import check_attention, gen, linear_bound, make_cache, randn, runs_and_blocks, wide_bound
+from test_gpu_int4 import check_attention, gen, linear_bound, make_cache, random_weight, randn, runs_and_blocks, wide_bound
 from test_gpu_int4_model import HELD, load
 
 pytestmark = pytest.mark.gpu
@@ -394,6 +394,32 @@ def test_units_into_columns_that_start_anywhere(ops, m, first, more):
     got = ops.glu_product(x, w, ops.kernels.glu_shape("silu"), out=wide[:, first:first + inter])
     assert got.data_ptr() == wide[:, first:].data_ptr() and torch.equal(got, ops.swiglu_product(x, w))
     assert bool((wide[:, :first] == 7).all()) and bool((wide[:, first + inter:] == 7).all())
+    y = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+    gate, up = y.chunk(2, 1)
+    want = gate * torch.sigmoid(gate) * up
+    assert float(((got.double() - want).abs() / unit_bound(x, w, want, gate, up)).max()) <= 1
+
+
+@pytest.mark.parametrize("m,inter,k", [(400, 6000, 4096), (700, 2064, 16384)])
+def test_wide_units_of_long_prompts_take_a_bounded_work_space(ops, m, inter, k, monkeypatch):
+    """Several pieces of the weight, the last a short one: the bits of the weight as a whole, results against 64 bits, and what the call holds
+    beside its result."""
+    import sys
+    limit = 32 << 20
+    monkeypatch.setattr(sys.modules["garlic_inference_b200.ops.linear"], "INT4_GATED_BYTES", limit)
+    g = gen(m)
+    w = random_weight(ops, g, 2 * inter, k)
+    x = (randn(g, m, k) * 0.2).to(torch.bfloat16)
+    assert 4 * inter * k > 2 * limit
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = ops.swiglu_product(x, w)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before <= limit + 2 * m * inter + (1 << 20)
+    monkeypatch.undo()
+    assert torch.equal(got, ops.swiglu_product(x, w))
     y = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
     gate, up = y.chunk(2, 1)
     want = gate * torch.sigmoid(gate) * up

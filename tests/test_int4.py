@@ -122,3 +122,13 @@ def test_products_go_where_there_is_room(monkeypatch):
                     both.add((takes, m <= 16))
                     assert taken.pop() == ("linear_rows" if takes else "linear_wide"), (m, n, k, gated)
     assert both == {(0, True), (1, True), (0, False)}
+
+
+def test_gated_units_are_made_wide_in_bounded_pieces():
+    from garlic_inference_b200.ops.linear import INT4_GATED_BYTES, _gated_columns
+    for n in (16, 128, 4096, 12288, 57344, 700000):
+        for k in (128, 4096, 8192, 120000, 2000000):
+            c = _gated_columns(n, k)
+            assert c == n if 4 * n * k <= INT4_GATED_BYTES // 2 else c == n or c < n and c % 128 == 0
+            assert 4 * min(c, n) * k <= max(INT4_GATED_BYTES, 4 * 128 * k)
+            assert -(-n // c) <= -(-4 * n * k // INT4_GATED_BYTES) * 2
