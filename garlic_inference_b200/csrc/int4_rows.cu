@@ -274,6 +274,23 @@ int4_gather_kernel(Int4Pool kp, Int4Pool vp, bf16* __restrict__ k_out, bf16* __r
     }
 }
 
+// Listed rows of a matrix, 16 bytes a piece, into a dense one (put: from it), for the short sequences of a step.  A row that does not exist is reported:
+// zeros are taken for it, and it is put nowhere.
+__global__ void __launch_bounds__(I4R_THREADS)
+int4_move_rows_kernel(uint4* __restrict__ matrix, uint4* __restrict__ some, const int* __restrict__ rows, int n, int pieces, int put,
+                      int* __restrict__ status) {
+    gi_pdl_start();
+    const int row = rows[blockIdx.x];
+    const bool there = row >= 0 && row < n;
+    if (!there && threadIdx.x == 0) atomicExch(status, 4);
+    uint4* const at = matrix + (size_t)(there ? row : 0) * pieces;
+    uint4* const to = some + (size_t)blockIdx.x * pieces;
+    for (int i = threadIdx.x; i < pieces; i += I4R_THREADS) {
+        if (!put) to[i] = there ? at[i] : make_uint4(0, 0, 0, 0);
+        else if (there) at[i] = to[i];
+    }
+}
+
 static int check_pool(const char* who, const void* codes, const void* meta, int n_kv, int d, int page_size, int max_pages, int n_slots) {
     GI_REQUIRE(n_kv > 0 && d > 0 && d % I4_GROUP_KV == 0 && d <= 1024, "%s: %d heads of %d; heads are multiples of 64 numbers", who, n_kv, d);
     GI_REQUIRE(page_size > 0 && max_pages > 0 && n_slots > 0, "%s: page and table sizes must be positive", who);
@@ -350,6 +367,16 @@ extern "C" int gi_int4_read(const void* codes, const void* meta, void* out, int 
         gi_launch(int4_read_kernel<bf16>, dim3(blocks), dim3(I4R_THREADS), 0, s, pool, (bf16*)out, table, tok_pos, tok_slot, n_kv, groups, n_slots, max_pages, page_size, n_pages, items, status);
     else GI_REQUIRE(false, "gi_int4_read: dtype %d", dtype);
     return gi_check_launch("gi_int4_read");
+}
+
+extern "C" int gi_int4_move_rows(void* matrix, void* some, const int* rows, int n_some, int n, long long row_bytes, int put, int* status,
+                                 void* stream) {
+    GI_REQUIRE(n_some >= 0 && n >= 0 && row_bytes > 0 && row_bytes % 16 == 0 && row_bytes / 16 < (1 << 30) && (uintptr_t)matrix % 16 == 0 &&
+               (uintptr_t)some % 16 == 0, "gi_int4_move_rows: %d of %d rows of %lld bytes; rows must start on 16", n_some, n, row_bytes);
+    if (n_some == 0) return 0;
+    gi_launch(int4_move_rows_kernel, dim3((unsigned)n_some), dim3(I4R_THREADS), 0, (cudaStream_t)stream, (uint4*)matrix, (uint4*)some, rows, n,
+              (int)(row_bytes / 16), put, status);
+    return gi_check_launch("gi_int4_move_rows");
 }
 
 extern "C" int gi_int4_gather(const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, void* k_out, void* v_out,

@@ -345,6 +345,13 @@ def decode_splits(n_runs: int, heads: int, keys: int, places: int = PLACES, unev
 # 3,000 keys, 8 heads of 128, in us against 153 with wide pages: 20 columns 51, 64 columns 82, 96 columns 137, 128 columns 154; 40 runs
 # of 1,000 keys against 163: 62, 96, 147, 185.
 FEW_COLUMNS = 96
+# Wide pages of a layer's step: up to so many bytes a step of short and long sequences is one call, beyond them two; and where more than one
+# sequence would fill them, so many at a time.  8 key/value heads of 128, groups of 4, us and MB held, as one call / split:
+#   4 x 1 behind 500, 300 new        59 (11) / 121 (3): launches            47 x 1 behind 6,000, 512 new       269 (22) / 138 (7)
+#   8 x 1 behind 2,000, 200 of 2,200 202 (1) / 112 (10)                     40 x 1 behind 8,000, 2,048 new   1,116 (1,284) / 186 (24)
+#   6 x 512 behind 30,000            1,890 (740) / 1,960 (262)              32 x 1 behind 8,000, 4,096 new   1,034 (1,056) / 300 (48)
+TOGETHER_BYTES = 32 << 20
+GATHER_BYTES = 256 << 20
 
 
 def attention_decode(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor, tok_pos: torch.Tensor,
@@ -369,12 +376,37 @@ def attention_decode(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
 
 
 def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor, runs: torch.Tensor,
-                     blocks: torch.Tensor, scale: float, window: int, status: torch.Tensor) -> torch.Tensor:
+                     blocks: torch.Tensor, scale: float, window: int, status: torch.Tensor,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of prompts, or portions of prompts, q [n, n_q, d] bfloat16, over the cache (the tokens' own keys are in it).  `runs`
     int32 [n_runs, 4] cuts the rows into runs of at most 128 consecutive tokens of one sequence: {slot, first row, rows, position
     of the first row}; rows in no run are zeros, no row is in two.  `blocks` int32 [n_blocks, 2] lists, each once, the blocks of 64
     positions that any of them sees: {slot, position / 64}.  Runs of a few tokens read the cache as single tokens do;
-    for longer ones the blocks' keys and values are rounded to bfloat16 pages for the tensor-memory kernel.  Returns [n, n_q * d]."""
+    for longer ones the blocks' keys and values are rounded to bfloat16 pages for the tensor-memory kernel.  One call has one way, by the
+    mean length of its runs: short runs beside long ones are `attention_some`'s.  Returns [n, n_q * d]; `out` (dense): written there, rows
+    in no run stay as they are (those of a run that names no slot, or what does not exist, stay or become zeros)."""
+    return _prompt(q, k_rows, v_rows, block_table, runs, blocks, scale, window, status, out)
+
+
+def attention_some(q: torch.Tensor, rows: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor, runs: torch.Tensor,
+                   blocks: torch.Tensor, scale: float, window: int, status: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """`attention_prompt` for some rows of q: `rows` int32 names them, each once, and `runs` counts in that list.  Their results go into the
+    same rows of `out` [n, n_q * d], which is returned; the others stay as they are.  A row that does not exist is reported in `status`.  A step of single tokens and long prompts is one
+    call of each: the tokens' keys are read as codes, only the prompts' are gathered."""
+    l, dev = _start()
+    if rows.dim() != 1 or q.dim() != 3 or out.shape != (q.shape[0], q.shape[1] * q.shape[2]):
+        raise KernelError(f"rows {tuple(rows.shape)} of queries {tuple(q.shape)} into {tuple(out.shape)}")
+    n, n_q, d = q.shape
+    some = q.new_empty((rows.shape[0], n_q, d))
+    move = (_check(dev, rows, "rows", torch.int32), some.shape[0], n, n_q * d * 2)
+    check(l.gi_int4_move_rows(_check(dev, q, "q", torch.bfloat16), some.data_ptr(), *move, 0, _status(dev, status), _stream(dev)), l)
+    to = _check(dev, out, "out", torch.bfloat16)
+    done = _prompt(some, k_rows, v_rows, block_table, runs, blocks, scale, window, status, None)
+    check(l.gi_int4_move_rows(to, done.data_ptr(), *move, 1, _status(dev, status), _stream(dev)), l)
+    return out
+
+
+def _prompt(q, k_rows, v_rows, block_table, runs, blocks, scale: float, window: int, status, out) -> torch.Tensor:
     l, dev = _start()
     shape, pools = _pools(dev, k_rows, v_rows)
     n_pages, heads, page_size, d = shape
@@ -386,13 +418,15 @@ def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
     table = _table(dev, block_table)
     _, n_slots, width = table
     window, n_runs, n_blocks = int(window or 0), runs.shape[0], blocks.shape[0]
+    if out is not None and (out.shape != (n, n_q * d) or _check(dev, out, "out", torch.bfloat16) % 16):
+        raise KernelError(f"out {tuple(out.shape)} for a result of {(n, n_q * d)} that starts on 16 bytes")
     if n_runs == 0 or n == 0:
-        return q.new_zeros((n, n_q * d))
+        return q.new_zeros((n, n_q * d)) if out is None else out
     columns = -(-n * (n_q // heads) // n_runs)
     if columns <= FEW_COLUMNS:
         tiles, places = (1, PLACES) if columns <= 8 else (-(-columns // 16), 444)
-        return _few(l, dev, q, at, shape, pools, table, runs_at, n_runs, None, None, scale, window, status, q.new_zeros((n, n_q * d)),
-                    decode_splits(n_runs * tiles, heads, 64 * n_blocks // n_runs, places, 2048), n_runs * heads * tiles)
+        return _few(l, dev, q, at, shape, pools, table, runs_at, n_runs, None, None, scale, window, status,
+                    q.new_zeros((n, n_q * d)) if out is None else out, decode_splits(n_runs * tiles, heads, 64 * n_blocks // n_runs, places, 2048), n_runs * heads * tiles)
     if n_blocks == 0:
         raise KernelError(f"{n_runs} runs that see no block of the cache")
     max_blocks = -(-width * page_size // 64)
@@ -402,4 +436,4 @@ def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
     check(l.gi_int4_gather(*pools, pages[0].data_ptr(), pages[1].data_ptr(), new_table.data_ptr(), blocks_at, n_blocks, runs_at,
                            kept.data_ptr(), n_runs, n, table[0], heads, d, n_slots, width, max_blocks, page_size, n_pages, window,
                            _status(dev, status), _stream(dev)), l)
-    return kernels.attention_prefill_tcgen05(q, pages[0], pages[1], new_table, kept, scale, window)
+    return kernels.attention_prefill_tcgen05(q, pages[0], pages[1], new_table, kept, scale, window, out=out)

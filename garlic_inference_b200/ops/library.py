@@ -120,6 +120,7 @@ _SIGNATURES = {
     "gi_int4_append": ([P, L, L, P, L, L, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, P], I),
     "gi_int4_read": ([P, P, P, I, P, P, P, I, I, I, I, I, I, I, P, P], I),
     "gi_int4_gather": ([P, P, P, P, P, P, P, P, I, P, P, I, I, P, I, I, I, I, I, I, I, I, P, P], I),
+    "gi_int4_move_rows": ([P, P, P, I, I, L, I, P, P], I),
     "gi_int4_qk_norm_rope_append": ([P, P, P, P, P, P, P, P, I, F, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, I, P, P], I),
     "gi_int4_linear_tcgen05": ([P, P, P, I, L, I, I, I, I, I, F, F, F, F, I, P, P], I),
     "gi_int4_attention": ([P, P, P, P, P, P, P, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, P], I),

@@ -22,7 +22,7 @@ import torch
 from ..cache import KVRequirement
 from ..ops import int4, kernels, linear
 from ..weights.loader import TensorWant
-from .base import Mixer, register_part
+from .base import Mixer, StepShape, register_part
 
 
 def query_runs(shape, rows: int) -> np.ndarray:
@@ -41,6 +41,38 @@ def key_blocks(shape, window: int) -> np.ndarray:
     rows = [(s, b) for s, n, p in zip(shape.seq_slots, shape.seq_lens, shape.seq_past) if n
             for b in range(max(0, p - window + 1) // 64 if window else 0, -(-(p + n) // 64))]
     return np.asarray(rows, dtype=np.int32).reshape(-1, 2)
+
+
+def some_sequences(shape, which, packed: bool = False) -> StepShape:
+    """The step's sequences `which`; `packed`: their rows counted as if there were no others."""
+    pick = lambda a: [a[i] for i in which]
+    lens = pick(shape.seq_lens)
+    starts = [sum(lens[:i]) for i in range(len(lens))] if packed else pick(shape.seq_starts)
+    return StepShape(pick(shape.seq_slots), starts, lens, pick(shape.seq_past), False)
+
+
+def short_and_long(shape, window: int, group: int, together: int, most_blocks: int) -> tuple:
+    """How a step goes over a cache in 4 bits: (sequences whose few tokens read codes, lists of those whose keys are gathered together).  A
+    sequence is short up to `int4.FEW_COLUMNS` columns (tokens x query heads of a key/value head); a list has at most
+    `most_blocks` blocks of 64 keys, or is one sequence.  A step that sees up to `together` blocks is one list.  Worked out once per step."""
+    key = ("short_and_long", window, group, together, most_blocks)
+    if key not in shape.notes:
+        short, lists, held, total = [], [], 0, 0
+        for i, (n, p) in enumerate(zip(shape.seq_lens, shape.seq_past)):
+            if not n:
+                continue
+            blocks = -(-(p + n) // 64) - (max(0, p - window + 1) // 64 if window else 0)
+            total += blocks
+            if n * group <= int4.FEW_COLUMNS:
+                short.append(i)
+                continue
+            if not lists or held + blocks > most_blocks:
+                lists.append([])
+                held = 0
+            lists[-1].append(i)
+            held += blocks
+        shape.notes[key] = (short, lists) if total > together else ([], [list(range(len(shape.seq_lens)))])
+    return shape.notes[key]
 
 
 def _key_tiles(shape, window: int, chunk: int, keep: int) -> tuple:
@@ -139,10 +171,30 @@ class GQAAttention(Mixer):
 
     def step_arrays(self, shape, cache):
         if self.bits and not shape.all_single:
-            w = self.window or 0
-            return {"query_runs_128": lambda: query_runs(shape, 128), f"key_blocks_{w}": lambda: key_blocks(shape, w)}
+            return self._calls(shape)[0]
         rows = 0 if shape.all_single else self._run_rows(cache.kv, shape)
         return {f"query_runs_{rows}": lambda: query_runs(shape, rows)} if rows else {}
+
+    def _calls(self, shape) -> tuple:
+        """A step with prompts over a cache in 4 bits: the arrays of its calls ({name: function}), and their names as (rows, runs, blocks), the
+        short sequences' call with its rows last.  A step of one kind is one call."""
+        w, group = self.window or 0, self.n_q // self.n_kv
+        block = 4 * 64 * self.n_kv * self.d
+        short, lists = short_and_long(shape, w, group, int4.TOGETHER_BYTES // block, max(1, int4.GATHER_BYTES // block))
+        if not lists or (not short and len(lists) == 1):
+            return {"query_runs_128": lambda: query_runs(shape, 128), f"key_blocks_{w}": lambda: key_blocks(shape, w)}, \
+                [(None, "query_runs_128", f"key_blocks_{w}")]
+        arrays, calls = {}, []
+        for i, which in enumerate(lists + ([short] if short else [])):
+            part, packed = some_sequences(shape, which, packed=i == len(lists)), i == len(lists)
+            name = f"{w}_{group}_{self.n_kv * self.d}_{i}"
+            arrays[f"some_runs_{name}"] = lambda part=part: query_runs(part, 128)
+            arrays[f"some_blocks_{name}"] = lambda part=part: key_blocks(part, w)
+            if packed:
+                arrays[f"some_rows_{name}"] = lambda: np.concatenate(
+                    [np.arange(shape.seq_starts[s], shape.seq_starts[s] + shape.seq_lens[s], dtype=np.int32) for s in short])
+            calls.append((f"some_rows_{name}" if packed else None, f"some_runs_{name}", f"some_blocks_{name}"))
+        return arrays, calls
 
     def _array(self, ctx, name: str, make) -> torch.Tensor:
         a = ctx.arrays.get(name)
@@ -161,13 +213,24 @@ class GQAAttention(Mixer):
         attention for runs of tokens, for heads of 64 too unless they see few keys; split-KV when every sequence brings
         one token and the group is at most 16).  Otherwise bfloat16 with a head size the mma.sync kernels take: the split-KV kernel for single
         tokens, the flash kernel for runs.  Everything else (float32, other head sizes, larger groups in
-        decode) goes to the exact-order kernel.  Pages in 4 bits have kernels of their own."""
+        decode) goes to the exact-order kernel.  Pages in 4 bits have kernels of their own: of a step that mixes them, short
+        sequences read codes and long ones' keys are gathered, no more at a time than `int4.GATHER_BYTES` say."""
         if self.bits:
             w = self.window or 0
             if ctx.all_single or not ctx.seq_lens:
                 return int4.attention_decode(q, kv.k_pool, kv.v_pool, kv.block_table, ctx.tok_pos, ctx.tok_slot, self.scale, w, ctx.status)
-            return int4.attention_prompt(q, kv.k_pool, kv.v_pool, kv.block_table, self._runs(ctx, 128),
-                                         self._array(ctx, f"key_blocks_{w}", lambda: key_blocks(ctx, w)), self.scale, w, ctx.status)
+            arrays, calls = self._calls(ctx)
+            o = None
+            for names in calls:
+                rows, runs, blocks = (None if n is None else self._array(ctx, n, arrays[n]) for n in names)
+                pages = (kv.k_pool, kv.v_pool, kv.block_table, runs, blocks, self.scale, w, ctx.status)
+                if rows is not None:
+                    int4.attention_some(q, rows, *pages, o)
+                elif o is not None:
+                    int4.attention_prompt(q, *pages, o)
+                else:
+                    o = int4.attention_prompt(q, *pages)
+            return o
         covered = (not ctx.all_single) and ctx.n_tokens == sum(ctx.seq_lens)
         if ctx.all_single:
             if kernels.tcgen05_decode_takes(q.dtype, self.d, kv.page_size, self.n_q // self.n_kv):

@@ -424,3 +424,106 @@ def test_wide_units_of_long_prompts_take_a_bounded_work_space(ops, m, inter, k, 
     gate, up = y.chunk(2, 1)
     want = gate * torch.sigmoid(gate) * up
     assert float(((got.double() - want).abs() / unit_bound(x, w, want, gate, up)).max()) <= 1
+
+
+# ------------------------------------------------------------------------------------------------ steps of unlike sequences
+MIXED = [
+    # heads, kv heads, d, page, (cached, new), window
+    (8, 2, 128, 64, [(300, 1), (64, 150), (900, 1), (0, 1), (10, 3)], 0),
+    (4, 1, 64, 16, [(0, 200), (333, 1), (64, 24), (100, 25)], 0),
+    (4, 2, 128, 64, [(500, 1), (200, 130), (0, 300), (90, 2)], 100),
+    (6, 6, 64, 7, [(70, 97), (70, 96), (5, 1)], 0),
+]
+
+
+@pytest.mark.parametrize("limit", [256 << 20, 1])
+@pytest.mark.parametrize("heads,kv,d,page,seqs,window", MIXED)
+def test_a_layer_over_short_and_long_sequences(ops, heads, kv, d, page, seqs, window, limit, monkeypatch):
+    """What a layer makes of such a step: rows of short sequences as exact as codes allow, those of long ones as the gathered path; all long
+    ones gathered together, and one by one."""
+    from garlic_inference_b200.cache.paged import KVView
+    from garlic_inference_b200.parts import StepContext
+    from test_int4 import _layer
+    monkeypatch.setattr(ops.int4, "GATHER_BYTES", limit)
+    monkeypatch.setattr(ops.int4, "TOGETHER_BYTES", 0)
+    g = gen(heads + d + page)
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [p + n for p, n in seqs], kv, d, page)
+    part = _layer(heads // kv, d, kv, window or None)
+    lens, past = [n for _, n in seqs], [p for p, _ in seqs]
+    starts = [sum(lens[:i]) for i in range(len(lens))]
+    n = sum(lens)
+    at = torch.zeros(n, dtype=torch.int32, device=DEV)
+    ctx = StepContext(n, at, at, at, list(range(len(seqs))), starts, lens, past, False, status=status)
+    kv_view = KVView(k_rows, v_rows, table, page, window or None)
+    q = (1.5 * randn(g, n, heads, d)).to(torch.bfloat16)
+    got = part.attend(q, kv_view, ctx)
+    spans = [(s, starts[s], lens[s], past[s]) for s in range(len(seqs))]
+    short = [t for t in spans if t[2] * (heads // kv) <= ops.int4.FEW_COLUMNS]
+    long = [t for t in spans if t not in short]
+    assert short and long and int(status) == 0
+    for part_of, oracle in ((short, plain.attention), (long, wide_attention)):
+        want, bound = oracle(q, k_rows, v_rows, table, part_of, part.scale, window)
+        for _, r, c, _ in part_of:
+            check_attention(got[r:r + c], want[r:r + c], bound[r:r + c])
+    ctx.arrays.clear()
+    assert torch.equal(got, part.attend(q, kv_view, ctx))
+
+
+def test_single_tokens_beside_a_prompt_gather_nothing_of_theirs(ops):
+    """40 single tokens behind 1,000 and a prompt of 300: what the layer holds meanwhile is the prompt's pages, not the others'."""
+    from garlic_inference_b200.cache.paged import KVView
+    from garlic_inference_b200.parts import StepContext
+    from test_int4 import _layer
+    heads, kv, d = 8, 2, 128
+    seqs = [(1000, 1)] * 20 + [(0, 300)] + [(1000, 1)] * 20
+    k_rows, v_rows, table, status, *_ = make_cache(ops, gen(3), [p + n for p, n in seqs], kv, d, 64)
+    part = _layer(heads // kv, d, kv)
+    lens, past = [n for _, n in seqs], [p for p, _ in seqs]
+    starts = [sum(lens[:i]) for i in range(len(lens))]
+    n = sum(lens)
+    at = torch.zeros(n, dtype=torch.int32, device=DEV)
+    ctx = StepContext(n, at, at, at, list(range(len(seqs))), starts, lens, past, False, status=status)
+    kv_view = KVView(k_rows, v_rows, table, 64, None)
+    q = randn(gen(4), n, heads, d).to(torch.bfloat16)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    part.attend(q, kv_view, ctx)
+    torch.cuda.synchronize()
+    pages = 5 * 2 * 64 * kv * d * 2                          # the prompt's five blocks, keys and values
+    slices = 40 * heads * 8 * (d + 2) * 4
+    assert torch.cuda.max_memory_allocated() - before <= pages + slices + 4 * n * heads * d * 2 + (1 << 20)
+    assert 40 * 16 * 2 * 64 * kv * d * 2 > pages + slices + 4 * n * heads * d * 2 + (1 << 20)
+
+
+def test_some_rows_of_a_step(ops):
+    """Rows in any order; what no row names stays; rows that do not exist are reported and put nowhere; refusals."""
+    g = gen(83)
+    heads, kv, d = 4, 2, 64
+    k_rows, v_rows, table, status, *_ = make_cache(ops, g, [50, 70, 9], kv, d, 16)
+    q = randn(g, 9, heads, d).to(torch.bfloat16)
+    rows = torch.tensor([7, 2, 0, 1], dtype=torch.int32, device=DEV)      # sequence 1 at 69, sequence 0 at 47, sequence 2 at 7 and 8
+    runs, blocks = runs_and_blocks([(1, 0, 1, 69), (0, 1, 1, 47), (2, 2, 2, 7)], 0)
+    fixed = (k_rows, v_rows, table, runs, blocks, d ** -0.5, 0, status)
+    out = torch.full((9, heads * d), 5.0, dtype=torch.bfloat16, device=DEV)
+    assert ops.int4.attention_some(q, rows, *fixed, out) is out
+    want = ops.int4.attention_prompt(q[rows.long()].contiguous(), *fixed)
+    assert int(status) == 0 and torch.equal(out[rows.long()], want) and bool((out[[3, 4, 5, 6, 8]] == 5).all())
+    for bad in (-1, 9, 2147483647):
+        some = rows.clone()
+        some[1] = bad
+        out.fill_(5.0)
+        ops.int4.attention_some(q, some, *fixed, out)
+        assert int(status) == 4 and torch.equal(out[[7, 0, 1]], want[[0, 2, 3]]) and bool((out[[2, 3, 4, 5, 6, 8]] == 5).all())
+        status.zero_()
+    for call in (lambda: ops.int4.attention_some(q, rows.long(), *fixed, out), lambda: ops.int4.attention_some(q, rows[None], *fixed, out),
+                 lambda: ops.int4.attention_some(q, rows, *fixed, out[:8]), lambda: ops.int4.attention_some(q, rows, *fixed, out.float()),
+                 lambda: ops.int4.attention_some(q, rows.cpu(), *fixed, out), lambda: ops.int4.attention_some(q[:, ::2], rows, *fixed, out[:, :heads * d // 2]),
+                 lambda: ops.int4.attention_prompt(q, *fixed, out[:8]), lambda: ops.int4.attention_prompt(q, *fixed, out.float()),
+                 lambda: ops.int4.attention_prompt(q, *fixed, out[:, ::2])):
+        with pytest.raises(ops.KernelError):
+            call()
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    out.fill_(5.0)
+    ops.int4.attention_some(q, none, k_rows, v_rows, table, runs[:0], blocks, d ** -0.5, 0, status, out)
+    assert int(status) == 0 and bool((out == 5).all())

@@ -132,3 +132,57 @@ def test_gated_units_are_made_wide_in_bounded_pieces():
             assert c == n if 4 * n * k <= INT4_GATED_BYTES // 2 else c == n or c < n and c % 128 == 0
             assert 4 * min(c, n) * k <= max(INT4_GATED_BYTES, 4 * 128 * k)
             assert -(-n // c) <= -(-4 * n * k // INT4_GATED_BYTES) * 2
+
+
+def _layer(group, d=128, kv=2, window=None):
+    cls = part_class("gqa_attention")
+    params = dict(hidden_size=64, n_heads=kv * group, n_kv_heads=kv, head_dim=d, **({} if window is None else {"window": window}))
+    return cls(params, _Load(cls.wanted(params)), Runtime(torch.bfloat16, torch.device("cpu"), cache="int4"))
+
+
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("group", [1, 4, 7])
+def test_steps_are_split_into_short_and_long_sequences(group, window, monkeypatch):
+    """Over random steps: every row is in one run of one call, short sequences in the call that names its rows, every call's blocks are those
+    that its own sequences see, and no list of long ones holds more than the limit unless it is one sequence."""
+    import random
+    rnd = random.Random(group)
+    part = _layer(group, window=window)
+    limit = 20
+    monkeypatch.setattr(int4, "GATHER_BYTES", limit * 4 * 64 * part.n_kv * part.d)
+    assert len(part._calls(StepShape([0, 1], [0, 1], [1, 300], [50, 0], False))[1]) == 1      # little to gather: one call
+    monkeypatch.setattr(int4, "TOGETHER_BYTES", 0)
+    kinds = set()
+    for _ in range(60):
+        n = rnd.randint(1, 9)
+        lens = [rnd.choice([1, 1, 2, 20, 97, 130, 300]) for _ in range(n)]
+        past = [rnd.choice([0, 5, 64, 500, 1500]) for _ in range(n)]
+        slots = rnd.sample(range(20), n)
+        starts = [sum(lens[:i]) for i in range(n)]
+        shape = StepShape(slots, starts, lens, past, all(x == 1 for x in lens))
+        if shape.all_single:
+            continue
+        arrays, calls = part._calls(shape)
+        assert set(arrays) == {a for c in calls for a in c if a} and part.step_arrays(shape, None).keys() == arrays.keys()
+        short = {i for i in range(n) if lens[i] * group <= int4.FEW_COLUMNS}
+        covered = []
+        for rows, runs, blocks in calls:
+            of = np.arange(sum(lens)) if rows is None else arrays[rows]()
+            seen, got, held = set(), arrays[runs](), arrays[blocks]()
+            assert got.dtype == held.dtype == np.int32 and of.dtype in (np.int32, np.int64)
+            who = set()
+            for s, r, c, p in got.tolist():
+                i = slots.index(s)
+                who.add(i)
+                assert 1 <= c <= 128 and [int(x) for x in of[r:r + c]] == list(range(starts[i] + p - past[i], starts[i] + p - past[i] + c))
+                covered += [int(x) for x in of[r:r + c]]
+                w = window or 1 << 30
+                seen |= {(s, j // 64) for q in range(p, p + c) for j in (max(0, q - w + 1), q)}
+                seen |= {(s, b) for b in range(max(0, p - w + 1) // 64, (p + c - 1) // 64 + 1)}
+            assert {tuple(b) for b in held.tolist()} == seen and len(held) == len(seen)
+            if len(calls) > 1:
+                assert who <= short if rows else not who & short
+                assert rows or len(who) == 1 or len(held) <= limit
+        assert sorted(covered) == list(range(sum(lens)))
+        kinds.add((len(calls) > 1, calls[-1][0] is not None))
+    assert kinds >= {(False, False), (True, True)}
