@@ -65,13 +65,16 @@ __device__ __forceinline__ float i4_up(float x) {
 }
 // Step and low value of a group with smallest number `mn` and largest `mx`: low = mn, step = (mx - mn) / 15, both rounded to bfloat16
 // so that low + 15 step reaches mx.  Halves are taken first so that the difference of two numbers near the largest float32
-// stays finite.
+// stays finite.  What the codes stand for has to be a bfloat16: numbers beyond the largest one count as that one, and a step that would
+// lead beyond it is rounded down (mx then lies an eighth of a step above code 15, still nearest to it).
 __device__ __forceinline__ void i4_step_low(float mn, float mx, bool finite, float& step, float& low) {
+    constexpr float MOST = 3.38953139e38f;                               // the largest bfloat16
+    mn = fmaxf(fminf(mn, MOST), -MOST), mx = fmaxf(fminf(mx, MOST), -MOST);
     low = i4_down(mn);
     const float exact = __fdiv_rn(__fsub_rn(mx * 0.5f, low * 0.5f), 7.5f);
     step = i4_up(exact);
-    if (fmaf(15.f, step, low) > 3.402823466e38f) step = i4_down(exact);       // 15 steps up is beyond the largest float32
-    if (!finite || !(step <= 3.4e38f) || !(fabsf(low) <= 3.4e38f)) step = low = __uint_as_float(0x7FC00000u);
+    if (fmaf(15.f, step, low) > MOST) step = i4_down(exact);
+    if (!finite) step = low = __uint_as_float(0x7FC00000u);
 }
 __device__ __forceinline__ uint32_t i4_code(float x, float step, float low) {
     if (!(step > 0.f)) return 0;                                         // all numbers alike, or not finite

@@ -527,3 +527,46 @@ def test_some_rows_of_a_step(ops):
     out.fill_(5.0)
     ops.int4.attention_some(q, none, k_rows, v_rows, table, runs[:0], blocks, d ** -0.5, 0, status, out)
     assert int(status) == 0 and bool((out == 5).all())
+
+
+# ------------------------------------------------------------------------------------------------ the largest numbers
+MOST = 2.0 ** 127 * (2 - 2.0 ** -7)                          # the largest bfloat16
+
+
+def largest_groups(dtype):
+    """Groups of 64 numbers up to the ends of bfloat16, and of float32: [groups, 64]."""
+    g = gen(89)
+    r = torch.rand(8, 64, generator=g, device=DEV, dtype=torch.float64)
+    x = torch.stack([r[0] * MOST, -r[1] * MOST, (2 * r[2] - 1) * MOST, MOST * (0.99 + 0.01 * r[3]), torch.full_like(r[4], MOST),
+                     torch.full_like(r[5], -MOST), r[6] * 0.9 * MOST, (2 * r[7] - 1) * MOST])
+    x[0, 3], x[1, 5], x[2, 7], x[2, 8], x[3, 1] = MOST, -MOST, MOST, -MOST, MOST
+    x = x.clamp(-MOST, MOST)
+    if dtype == torch.float32:
+        top = torch.finfo(torch.float32).max
+        x[7, 0], x[7, 1], x[0, 9], x[4, :] = top, -top, top, top
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_largest_numbers_come_back_finite(ops, dtype):
+    """Within half a step (2^-18 of a step for the quotient) of themselves, or of the largest bfloat16; in bfloat16 with its rounding, 2^-8."""
+    x = largest_groups(dtype)
+    want = x.double().clamp(-MOST, MOST)
+    w = ops.int4.quantize_weight(torch.cat([x, x], 1))       # groups of 128
+    codes, step, low = plain.unpack_weight(w)
+    rows = [ops.int4.Int4Rows.zeros(1, 8, 16, 64, DEV) for _ in range(2)]
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    pos, slot, status = torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.int4.append(x[None], x[None], *rows, table, pos, slot, status)
+    steps = rows[0].meta[0, :, 0, 0, 0].double()
+    for t in (torch.float32, torch.bfloat16):
+        back = ops.int4.dequantize_weight(w, t)[:, :64].double()
+        read = ops.int4.read(rows[0], table, pos, slot, status, t)[0].double()
+        for got, s in ((back, step[:, 0]), (read, steps)):
+            assert bool(torch.isfinite(got).all())
+            bound = s[:, None] * (0.5 + 2 ** -18) + (2 ** -8 if t == torch.bfloat16 else 2 ** -24) * want.abs()
+            assert float(((got - want).abs() / bound).max()) <= 1
+    y = torch.zeros(20, 128, dtype=torch.bfloat16, device=DEV)
+    y[:, 5] = 2.0 ** -100
+    for rows_of in (8, 20):                                  # a number that is finite stays one on its way to the tensor cores
+        assert bool(torch.isfinite(ops.linear(y[:rows_of], w, torch.float32)).all())
