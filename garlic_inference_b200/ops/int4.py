@@ -27,7 +27,7 @@ GROUP_ROWS = 64             # numbers of a head that share a step
 TILE_BYTES = 1088           # 16 outputs x 128 inputs: 1,024 bytes of codes, then (step, low) of the 16 outputs
 _NO_UNIT = (0, 1.0, float("inf"), float("inf"), 0.0)
 MAX_CLUSTER = 8             # slices of the keys that join themselves
-PLACES = 592                # blocks of the attention kernel for up to 8 columns that 148 SMs hold; 444 for up to 16
+PLACES, PLACES_WIDE = 592, 444      # blocks of the attention kernel that 148 SMs hold: for up to 8 columns, and for up to 16
 LINEAR_MAX_ROWS = 16        # rows of x that the kernel reading a weight's codes takes
 
 
@@ -309,14 +309,14 @@ def _queries(dev: int, q: torch.Tensor, shape: tuple) -> int:
 
 
 def _few(l, dev: int, q: torch.Tensor, at: int, shape: tuple, pools: tuple, table: tuple, runs, n_runs: int, pos, slot, scale: float,
-         window: int, status: torch.Tensor, out: torch.Tensor, n_splits: int, blocks: int) -> torch.Tensor:
-    """`blocks`: of the kernel, without slices.  Up to 8 slices are a cluster and join themselves where all blocks have a place at
+         window: int, status: torch.Tensor, out: torch.Tensor, n_splits: int, blocks: int, places: int) -> torch.Tensor:
+    """`blocks`: of the kernel, without slices; `places`: how many blocks of its kind run at once.  Up to 8 slices are a cluster and join themselves where all blocks have a place at
     once (8 runs of 2,048 keys, 6 slices: 12.7 us, 14.0 with a second kernel); where they wait for places, a cluster waits for
     as many as it has blocks (64 runs of 500 keys, 4 slices: 35.7 against 24.3)."""
     n_pages, heads, page_size, d = shape
     n, n_q, _ = q.shape
     part_o = part_ml = None
-    if n_splits > MAX_CLUSTER or n_splits > 1 and n_splits * blocks > PLACES:      # one workspace: the slices' sums, then their maxima and weights
+    if n_splits > MAX_CLUSTER or n_splits > 1 and n_splits * blocks > places:      # one workspace: the slices' sums, then their maxima and weights
         room = q.new_empty((n * n_q * n_splits * (d + 2),), dtype=torch.float32)
         part_o = room.data_ptr()
         part_ml = part_o + n * n_q * n_splits * d * 4
@@ -324,6 +324,13 @@ def _few(l, dev: int, q: torch.Tensor, at: int, shape: tuple, pools: tuple, tabl
     check(l.gi_int4_attention(at, *pools, table[0], runs, n_runs, n, pos, slot, out.data_ptr(), part_o, part_ml, n_q, heads, d, table[1],
                               table[2], page_size, n_pages, window, scale, n_splits, _status(dev, status), _stream(dev)), l)
     return out
+
+
+def _tiles(columns: int) -> tuple:
+    """(blocks of a run's columns, how many such blocks run at once): 8 columns a block up to 8, 16 beyond.  Slices by these counts, by those of 8
+    columns for all, in us: 8 runs of 2,048 keys, 8 heads of 128, groups of 16 17.5, 27.8; 20 of 2,000, 4 heads of 64, groups of 32 17.7,
+    27.5; 1 of 131,000, 8 heads of 128, groups of 16 68.8, 86.9."""
+    return (1, PLACES) if columns <= 8 else (-(-columns // 16), PLACES_WIDE)
 
 
 def decode_splits(n_runs: int, heads: int, keys: int, places: int = PLACES, uneven: int = 1024) -> int:
@@ -367,12 +374,12 @@ def attention_decode(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_
     pos, slot = _tokens(dev, n, tok_pos, tok_slot)
     table = _table(dev, block_table)
     window = int(window or 0)
+    tiles, places = _tiles(n_q // shape[1])
     if not n_splits:
         keys = table[2] * shape[2]
-        n_splits = decode_splits(n, shape[1], min(keys, window) if window else keys)
-    group = n_q // shape[1]
+        n_splits = decode_splits(n * tiles, shape[1], min(keys, window) if window else keys, places)
     return _few(l, dev, q, at, shape, pools, table, None, n, pos, slot, scale, window, status, q.new_empty((n, n_q * d)), n_splits,
-                n * shape[1] * (1 if group <= 8 else -(-group // 16)))
+                n * shape[1] * tiles, places)
 
 
 def attention_prompt(q: torch.Tensor, k_rows: Int4Rows, v_rows: Int4Rows, block_table: torch.Tensor, runs: torch.Tensor,
@@ -424,9 +431,9 @@ def _prompt(q, k_rows, v_rows, block_table, runs, blocks, scale: float, window: 
         return q.new_zeros((n, n_q * d)) if out is None else out
     columns = -(-n * (n_q // heads) // n_runs)
     if columns <= FEW_COLUMNS:
-        tiles, places = (1, PLACES) if columns <= 8 else (-(-columns // 16), 444)
+        tiles, places = _tiles(columns)
         return _few(l, dev, q, at, shape, pools, table, runs_at, n_runs, None, None, scale, window, status,
-                    q.new_zeros((n, n_q * d)) if out is None else out, decode_splits(n_runs * tiles, heads, 64 * n_blocks // n_runs, places, 2048), n_runs * heads * tiles)
+                    q.new_zeros((n, n_q * d)) if out is None else out, decode_splits(n_runs * tiles, heads, 64 * n_blocks // n_runs, places, 2048), n_runs * heads * tiles, places)
     if n_blocks == 0:
         raise KernelError(f"{n_runs} runs that see no block of the cache")
     max_blocks = -(-width * page_size // 64)

@@ -186,3 +186,15 @@ def test_steps_are_split_into_short_and_long_sequences(group, window, monkeypatc
         assert sorted(covered) == list(range(sum(lens)))
         kinds.add((len(calls) > 1, calls[-1][0] is not None))
     assert kinds >= {(False, False), (True, True)}
+
+
+def test_slices_are_counted_with_the_blocks_that_run_at_once():
+    """Groups of more than 8 have blocks of 16 columns, of which fewer run at once: whatever joins as clusters has a place, all at once."""
+    assert int4._tiles(1) == int4._tiles(8) == (1, 592) and int4._tiles(9) == int4._tiles(16) == (1, 444) and int4._tiles(17) == (2, 444)
+    for group in (1, 4, 8, 9, 12, 16, 24, 32, 48):
+        tiles, places = int4._tiles(group)
+        for n in (1, 3, 8, 20, 64, 300):
+            for heads in (1, 4, 8):
+                s = int4.decode_splits(n * tiles, heads, 2048, places)
+                assert s <= 2 or s * n * tiles * heads <= places      # (2: runs of 2,048 keys may differ in length)
+    assert int4.decode_splits(8, 8, 2048, 444) == 6
