@@ -390,6 +390,89 @@ def fivitar_config_dict(width, heads, ff, vocab, n_layers, head_dim=128, kv_rank
             "layers": [layer(i) for i in range(n_layers)]}
 
 
+def study_int4(args, pk) -> int:
+    """Decode steps of the benchmark's model with weights, cache, both or neither in 4 bits, at batches of 1 to 64 behind 500 to 30,000 cached
+    tokens in a cache that just holds them, and the kernel that norms, rotates and appends a step's keys.  One JSON line."""
+    import torch
+    from garlic_inference_b200 import LanguageModel, Qwen3Config
+    from garlic_inference_b200.ops import int4, kernels
+    from garlic_inference_b200.sampling import SamplingParams
+    K, W = min(args.steps, 32), max(min(args.warmup, 8), 3)
+    torch.cuda.set_device(0)
+    greedy, gen = SamplingParams(), torch.Generator().manual_seed(0)
+    n_layers = args.layers or QWEN3_8B["num_hidden_layers"]
+    cfg = Qwen3Config(**{**QWEN3_8B, "num_hidden_layers": n_layers})
+    out = {"study": "int4", "data": "synthetic", "steps": K, "warmup": W, "layers": n_layers, "peaks": pk, "models": {}, "kernels": {}}
+    points = ((1, 500), (8, 500), (8, 4000), (32, 1000), (64, 2000), (1, 30000))
+    for name, kept in (("bfloat16", {}), ("weights", {"weights": "int4"}), ("cache", {"cache": "int4"}), ("both", {"weights": "int4", "cache": "int4"})):
+        clocks = ClockSampler("0")
+        res = out["models"][name] = {}
+        for batch, cached in points:
+            room = batch * (-(-(cached + W + K + 8) // 64) * 64)
+            model = LanguageModel.from_random(cfg, seed=0, device=0, dtype="bfloat16", max_tokens=room, **kept)
+            eng, sampler = model.engine, model.sampler
+            res["weight_bytes"] = model.model.weight_bytes()
+            slots, toks = [], []
+            for _ in range(batch):
+                s = eng.alloc_slot()
+                ids = torch.randint(0, cfg.vocab_size, (cached,), generator=gen).tolist()
+                toks.append(sampler.sample(model.step([(s, ids, [cached - 1])]), greedy, [0], [0]))
+                slots.append(s)
+            toks = torch.cat(toks)
+            for _ in range(W):
+                toks = sampler.sample(eng.step_decode_device(slots, toks), greedy, slots, slots)
+            torch.cuda.synchronize()
+            clocks.start()
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(K):
+                toks = sampler.sample(eng.step_decode_device(slots, toks), greedy, slots, slots)
+            b.record()
+            torch.cuda.synchronize()
+            clocks.stop()
+            res[f"decode_b{batch}_ctx{cached}_ms"] = round(a.elapsed_time(b) / K, 3)
+            eng.check()
+            del model, eng, sampler
+            torch.cuda.empty_cache()
+        res["clocks"] = clocks.summary()
+
+    # a step's joined projections into the cache, 32 and 8 heads of 128: 8 single tokens, and a prompt; 16 launches a graph, each with
+    # rows and pages of its own (more than L2 holds, for the prompt)
+    H, G, d, page, dev = 32, 8, 128, 64, "cuda"
+    cos, sin = (torch.rand(4096, d // 2, device=dev) for _ in range(2))
+    w = torch.ones(d, dtype=torch.bfloat16, device=dev)
+    for n, label in ((8, "8_tokens"), (2048, "prompt_2048")):
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        pos = torch.arange(n, dtype=torch.int32, device=dev)
+        slot = torch.zeros(n, dtype=torch.int32, device=dev)
+        n_pages = -(-n // page)
+        table = torch.arange(n_pages, dtype=torch.int32, device=dev)[None].contiguous()
+        sets = []
+        for _ in range(16):
+            qkv = torch.randn(n, (H + 2 * G) * d, device=dev).to(torch.bfloat16)
+            wide = [torch.zeros(n_pages, G, page, d, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+            sets.append((qkv, wide, [int4.Int4Rows.zeros(n_pages, G, page, d, dev) for _ in range(2)]))
+        for kind, fn, which in (("bfloat16", kernels.qk_norm_rope_append, 1), ("int4", int4.qk_norm_rope_append, 2)):
+            call = lambda s: fn(s[0], H, G, d, w, w, 1e-6, cos, sin, d, pos, slot, *s[which], table, status)
+            call(sets[0])
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                for s in sets:
+                    call(s)
+            times = []
+            for _ in range(8):
+                a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                a.record(); graph.replay(); b.record()
+                torch.cuda.synchronize()
+                times.append(a.elapsed_time(b) / 16 * 1e3)
+            out["kernels"][f"qk_norm_rope_append_{label}_{kind}_us"] = round(statistics.median(times[3:]), 2)
+            del graph
+    kernels.check_bounded_waits(torch.device("cuda", 0))
+    print(json.dumps(out))
+    return 0
+
+
 def study_fivitar(args, pk) -> int:
     """Prefill (one prompt of 2,048 tokens) and decode (batches of 1, 8 and 64 with 2,048 cached tokens each)
     of Fivitar models with random weights, beside Qwen3 models of the same width, depth, heads and feed-forward
@@ -1770,9 +1853,10 @@ def main() -> int:
     ap.add_argument("--write-model", default=None, metavar="DIR",
                     help="with --impl reference: only write the model folder that arm uses (tied head, --layers of the 36) "
                          "to DIR and exit, for running baseline/_ref/bin/reference_runner by hand or under a profiler")
-    ap.add_argument("--study", default=None, choices=["prefill-clocks", "fivitar", "zogulorn", "dugopel", "kenovik", "nezolorn", "netolorn"],
+    ap.add_argument("--study", default=None, choices=["prefill-clocks", "int4", "fivitar", "zogulorn", "dugopel", "kenovik", "nezolorn", "netolorn"],
                     help="prefill-clocks: 40 prompt steps of 2,048 tokens back to back with the clock and the power "
-                         "sampled every 20 ms; prints a table and no JSON line.  fivitar: prefill and decode of the "
+                         "sampled every 20 ms; prints a table and no JSON line.  int4: decode steps of the benchmark's model with "
+                         "weights, cache, both or neither in 4 bits; one JSON line of its own.  fivitar: prefill and decode of the "
                          "Fivitar design at two sizes of real layers beside Qwen3 at equal sizes, and the mixers' "
                          "kernels alone; one JSON line of its own.  zogulorn, dugopel, kenovik, nezolorn, "
                          "netolorn: the same for those designs (dugopel beside Fivitar's latent layers and Qwen3, nezolorn "
@@ -1792,6 +1876,8 @@ def main() -> int:
         print(f"bench.py: this library runs on one GPU; --gpus {args.gpus} is not supported (nothing was run)")
         return 2
 
+    if args.study == "int4":
+        return study_int4(args, peaks())
     if args.study == "fivitar":
         return study_fivitar(args, peaks())
     if args.study == "zogulorn":
