@@ -20,12 +20,13 @@
 //  * A block is one run of tokens, one key/value head, one block of 8 NT columns (token, query head of the group) and one
 //    slice of the keys.  Its 4 warps take 32 keys each, in turn, through a queue of their own (cp.async, three chunks deep), 16 at a time, and
 //    are merged in shared memory at the end; up to 8 slices are a cluster that joins itself, others are joined by a second kernel.
-//  * The reference of the softmax is moved only when a score lies 2^8 above it, and the scale of the steps only when one outgrows it:
-//    one vote a step instead of reductions and products over all sums.
+//  * The reference of the softmax is moved only when a score lies 2^8 above it, and the scale of the steps only when one leaves its range:
+//    one vote a step instead of reductions and products over all sums.  What is rare (steps far apart, values that are not finite) has a
+//    branch of its own, which shortened the common path by 9 instructions.
 //  * What runs once a block is kept small and rolled up: such instructions come from the instruction cache's next level at about 20 cycles each.
 //
-// Measured, 8 key/value heads of 128: one sequence of 131,000 keys 43 us in 74 slices (3.5 TB/s; 344 instructions for 16 keys of a head at 2.05 a
-// cycle and SM, 80 of them unpacking, 16 warps an SM), 8 of 2,048 13.6 us, 64 of 500 16.4 us, 48 of 1 to 8,000 61 us.
+// Measured, 8 key/value heads of 128, nothing in L2: one sequence of 131,000 keys 45.5 us in 74 slices (3.3 TB/s; 335 instructions for 16 keys of a
+// head at 2.2 a cycle and SM, 80 of them unpacking, 16 warps an SM), 8 of 2,048 14.8 us, 64 of 500 18.3 us, 48 of 1 to 8,000 61 us.
 #include "int4.cuh"
 
 #include <type_traits>

@@ -310,9 +310,9 @@ def _queries(dev: int, q: torch.Tensor, shape: tuple) -> int:
 
 def _few(l, dev: int, q: torch.Tensor, at: int, shape: tuple, pools: tuple, table: tuple, runs, n_runs: int, pos, slot, scale: float,
          window: int, status: torch.Tensor, out: torch.Tensor, n_splits: int, blocks: int, places: int) -> torch.Tensor:
-    """`blocks`: of the kernel, without slices; `places`: how many blocks of its kind run at once.  Up to 8 slices are a cluster and join themselves where all blocks have a place at
-    once (8 runs of 2,048 keys, 6 slices: 12.7 us, 14.0 with a second kernel); where they wait for places, a cluster waits for
-    as many as it has blocks (64 runs of 500 keys, 4 slices: 35.7 against 24.3)."""
+    """`blocks`: of the kernel, without slices; `places`: how many blocks of its kind run at once.  Up to 8 slices are a cluster and join
+    themselves where all blocks have a place at once (8 runs of 2,048 keys, 6 slices: 12.7 us, 14.0 with a second kernel, part of the pages
+    in L2); where they wait for places, a cluster waits for as many as it has blocks (64 runs of 500 keys, 4 slices: 35.7 against 24.3)."""
     n_pages, heads, page_size, d = shape
     n, n_q, _ = q.shape
     part_o = part_ml = None
@@ -336,14 +336,14 @@ def _tiles(columns: int) -> tuple:
 def decode_splits(n_runs: int, heads: int, keys: int, places: int = PLACES, uneven: int = 1024) -> int:
     """Slices of the keys per (run, key/value head): as many as fill the 148 SMs with 4 blocks each (`places`), a run of many keys among
     others one for every `uneven` keys up to 8 (lengths may differ, and are not known here), none of fewer than 256 keys, 8
-    instead of a few more (they join themselves).  `keys`: what the table's width or the window lets a run see.  Heads of 128, in us
-    by slices:
-      8 runs of 2,048 keys, 8 heads    1: 24.3   4: 13.4   6: 12.7   8: 13.6   14: 14.2   74: 23.0      (8 taken)
-      1 run of 131,000 keys, 8 heads   37: 51.1   55: 45.8   74: 43.0   111: 51.9                       (74)
-      1 run of 4,000 keys, 8 heads     1: 40.0   4: 14.3   8: 9.7   16: 8.4                             (16)
-      48 runs of 1 .. 8,000, 8 heads   1: 93.8   4: 64.5   7: 60.9   9: 63.1   14: 69.3                 (7)
-      64 runs of 500 keys, 8 heads     1: 16.4   2: 22.3   9: 29.0                                      (1)
-      1 run of 100 keys, 8 heads       1: 4.9   4: 6.1   74: 10.0                                       (1)"""
+    instead of a few more (they join themselves).  `keys`: what the table's width or the window lets a run see, which is the cache's
+    capacity rather than a length; runs far below it pay for slices that are empty.  Heads of 128, us by slices, nothing in L2:
+      8 runs of 2,048 keys, 8 heads    1: 21.3   4: 12.8   6: 14.3   8: 14.8   14: 15.8   74: 23.5      (8 taken)
+      1 run of 131,000 keys, 8 heads   37: 47.5   55: 44.6   74: 45.7   111: 53.0                       (74)
+      1 run of 4,000 keys, 8 heads     1: 36.4   4: 14.6   8: 10.6   16: 10.3                           (16)
+      48 runs of 1 .. 8,000, 8 heads   1: 87.0   4: 64.2   7: 61.2   9: 63.1   14: 68.9                 (7)
+      64 runs of 500 keys, 8 heads     1: 18.3   2: 26.3   8: 29.8                                      (1; 8 in a table of 262,144)
+      1 run of 100 keys, 8 heads       1: 5.9   4: 7.4   74: 11.3                                       (1; 74 in a table of 131,072)"""
     n = max(1, min(max(places // max(1, n_runs * heads), min(8, keys // uneven)), -(-keys // 256), 74))
     return 8 if 8 < n < 12 else n
 
