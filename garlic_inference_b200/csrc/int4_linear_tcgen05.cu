@@ -7,7 +7,9 @@
 //                of 512 bytes W came at 1.1 us a group).  W is nobody's output: in a recorded step the ring fills before the kernel
 //                waits for the one that makes x.
 //   warps 0-7    make it wide, two groups of four warps in turn: step * q + low in bfloat16 (one rounding, by fma), a thread an output, into
-//                tensor memory: the 128-row operand never passes through shared memory again, 32 KB a group.
+//                tensor memory: the 128-row operand never passes through shared memory again, 32 KB a group.  bfloat16, since both operands
+//                are of one type and x is that: an f16 would round less, but have no room for what x and a step may be without a scale for
+//                every row of x and every output, which would have to be known before the first group.
 //   warp 9       brings the rows of x.
 //   warp 10      products, 128 x BN x 16, accumulated in float32 in tensor memory over the whole slice.
 // Then the sums go to shared memory, the blocks of the cluster add up a share of the rows each, in the order of the ranks (the same bits from

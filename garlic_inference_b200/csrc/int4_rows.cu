@@ -218,7 +218,8 @@ int4_read_kernel(Int4Pool pool, T* __restrict__ out, const int* __restrict__ tab
     i4r_unpack(out + (size_t)item * 16, bits, meta);
 }
 
-// Blocks of 64 positions of the step's sequences as bfloat16 pages of their own, [blocks, n_kv, 64, d], for the prompt kernel on
+// Blocks of 64 positions of the step's sequences, each number rounded to bfloat16 (which holds whatever a step and a low value make, next to
+// any other; the prompt kernel's operands are that), as pages of their own, [blocks, n_kv, 64, d], for the prompt kernel on
 // tensor memory, and their block table [n_slots, max_blocks]: block i holds positions 64 b .. of the slot that blocks[i] =
 // {slot, b} names.  Positions without a page are zeros, as are those behind the table's last column; one that a run sees is reported.  runs_out: the
 // runs, those that name a slot, rows or positions that do not exist as empty ones (the prompt kernel takes them as they are).
