@@ -12,8 +12,8 @@
 //
 // q goes in exactly (a scaled f16), p_j * step_j rounded to the 11 significant bits of an f16, scaled by a power of two that
 // follows the largest step so far; a probability of 2^-20 of the largest still has all of them, 2^-10 with a step 2^10 below the
-// largest.  Steps further apart go in as several products of one range each, so that no key, seen or not, takes bits from others.
-// Everything else is float32.
+// largest.  From the first 16 keys on whose steps lie further apart, every column has a scale of its own, so that no key, seen or not, takes
+// bits from others.  Everything else is float32, but for what int4.cuh says of the sums in an instruction.
 // The transposition that the second product needs of V (its 16-wide side runs along a row of the cache) is ldmatrix's, on half words of
 // four numbers; that of the probabilities is movmatrix.
 //
@@ -306,12 +306,10 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
             for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
     }
     // What scales the largest step so far (of those below 2^31) to [2^6, 2^7): 2^(6 - e), e its exponent; 0 while there is none.  A step
-    // shares this scale if it lies in [2^(e - 10), 2^(e + 1)).
+    // shares this scale if it lies in [2^(e - 10), 2^(e + 1)).  Negative once some step did not: sums of columns that see only small ones
+    // then want the scale of their own that the branch for such keys gives them, to the end of the slice.
     float vscale[G];
-    auto step_exp = [&](int gr) { return vscale[gr] == 0.f ? -113 : I4A_STEP_TOP + 127 - (int)(__float_as_uint(vscale[gr]) >> 23); };
-    auto outside = [&](int gr, uint32_t step) {
-        return step + __float_as_uint(vscale[gr]) - ((uint32_t)(I4A_STEP_TOP - I4A_STEP_RANGE + 254) << 23) >= (uint32_t)(I4A_STEP_RANGE + 1) << 23;
-    };
+    auto step_exp = [&](int gr) { return vscale[gr] == 0.f ? -113 : I4A_STEP_TOP + 127 - (int)(__float_as_uint(fabsf(vscale[gr])) >> 23); };
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) vscale[gr] = 0.f;
 
@@ -409,7 +407,7 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
             for (int gr = 0; gr < G; ++gr)
                 moved |= !(fabsf(vs[gr][0] * vscale[gr] - 64.f) <= 63.9375f) || !(fabsf(vs[gr][1] * vscale[gr] - 64.f) <= 63.9375f);      // [2^-4, 2^7)
             // ---- a new reference for the columns' sums, or a new scale for the steps
-            uint32_t apart = 0;                                                // groups with steps of several ranges
+            bool apart = false;                                                // steps of more than one range
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
@@ -417,9 +415,11 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
                     const uint32_t most = __reduce_max_sync(0xffffffffu, max(b0 < 0x7F800000u ? b0 : 0u, b1 < 0x7F800000u ? b1 : 0u));
                     const int before = step_exp(gr), e = max(max(min((int)(most >> 23) - 127, I4A_STEP_MOST), -112), before);
                     const float grow = before < -112 ? 0.f : i4a_exp2((float)(before - e));      // nothing summed up yet: 0 times 0
-                    vscale[gr] = i4_pow2(I4A_STEP_TOP - e);
-                    const bool far = (b0 != 0 && b0 < 0x7F800000u && outside(gr, b0)) || (b1 != 0 && b1 < 0x7F800000u && outside(gr, b1));
-                    apart |= __any_sync(0xffffffffu, far) ? 1u << gr : 0u;
+                    auto outside = [&](uint32_t b) { return b != 0 && b < 0x7F800000u && (b >> 23) - (uint32_t)(e - I4A_STEP_RANGE + 127) > I4A_STEP_RANGE; };
+                    const bool far = vscale[gr] < 0.f || (before >= -112 && e - before > I4A_STEP_RANGE) || outside(b0) || outside(b1);
+                    const bool any = __any_sync(0xffffffffu, far);
+                    vscale[gr] = any ? -i4_pow2(I4A_STEP_TOP - e) : i4_pow2(I4A_STEP_TOP - e);
+                    apart |= any;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -456,17 +456,13 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
                         l[nt][e] += s[nt][e] + s[nt][e + 2];
                     }
             };
-            // a half's second operand, keys of its 8 rows, with their step scaled; what a column does not see stays out of it
-            auto operand = [&](int nt, int half, float step) {
-                const float p0 = s[nt][half * 2], p1 = s[nt][half * 2 + 1];
-                return i4a_transpose(i4_f16x2(p0 == 0.f ? 0.f : p0 * step, p1 == 0.f ? 0.f : p1 * step));
-            };
             auto offsets = [&](int gr, int half, int nt) {
                 const float p0 = s[nt][half * 2], p1 = s[nt][half * 2 + 1];
                 off_sum[nt][gr][0] += p0 == 0.f ? 0.f : p0 * vo[gr][half];
                 off_sum[nt][gr][1] += p1 == 0.f ? 0.f : p1 * vo[gr][half];
             };
-            // ---- steps of several ranges: one product for each, the largest first, brought to the sums' scale afterwards
+            // ---- steps far apart, or values that are not finite: what a column does not see stays out, and every column has a scale of
+            // its own, so that its largest probability times step lies in [2^14, 2^15)
             if (apart || odd) {
                 probabilities();
 #pragma unroll
@@ -474,34 +470,39 @@ __device__ __forceinline__ void i4a_columns(const bf16* __restrict__ q, const In
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) offsets(gr, 0, nt), offsets(gr, 1, nt);
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr)
-#pragma unroll 1
-                    while (__any_sync(0xffffffffu, vs[gr][0] != 0.f || vs[gr][1] != 0.f)) {      // a step that has had its turn becomes 0
-                        const uint32_t b0 = __float_as_uint(vs[gr][0]), b1 = __float_as_uint(vs[gr][1]);
-                        const uint32_t most = __reduce_max_sync(0xffffffffu, max(b0 < 0x7F800000u ? b0 : 0u, b1 < 0x7F800000u ? b1 : 0u));
-                        const int e = max((int)(most >> 23) - 127, -112);
-                        const uint32_t from = e > -112 ? (uint32_t)(e - I4A_STEP_RANGE + 127) << 23 : 1u;
-                        const float scale = i4_pow2(I4A_STEP_TOP - e), up = i4a_exp2((float)(e - step_exp(gr)));
-                        uint32_t w[4], b[NT][2];
+                for (int gr = 0; gr < G; ++gr) {
+                    const uint32_t b0 = __float_as_uint(vs[gr][0]), b1 = __float_as_uint(vs[gr][1]);
+                    const uint32_t most = __reduce_max_sync(0xffffffffu, max(b0 < 0x7F800000u ? b0 : 0u, b1 < 0x7F800000u ? b1 : 0u));
+                    const int e = min(max((int)(most >> 23) - 127, -112), 126);
+                    const float down = i4_pow2(-e), up = i4a_exp2((float)(I4A_STEP_TOP + e - step_exp(gr)));
+                    uint32_t w[4];
+                    i4a_matrix_trans(w, sK + C::CODES + matrix[gr]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            b[nt][0] = operand(nt, 0, b0 >= from ? vs[gr][0] * scale : 0.f);      // NaN with the first
-                            b[nt][1] = operand(nt, 1, b1 >= from ? vs[gr][1] * scale : 0.f);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float x[2][2], back[2];                                // [half][column]
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float p0 = s[nt][c], p1 = s[nt][2 + c];
+                            x[0][c] = p0 == 0.f ? 0.f : p0 * (vs[gr][0] * down), x[1][c] = p1 == 0.f ? 0.f : p1 * (vs[gr][1] * down);
+                            float top = fmaxf(x[0][c], x[1][c]);               // NaN aside
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                            int ex;
+                            const float f = i4_factor(top, ex);
+                            x[0][c] *= f, x[1][c] *= f;
+                            back[c] = i4_pow2(ex - 14) * up;
                         }
-                        vs[gr][0] = b0 >= from ? 0.f : vs[gr][0], vs[gr][1] = b1 >= from ? 0.f : vs[gr][1];
-                        i4a_matrix_trans(w, sK + C::CODES + matrix[gr]);
+                        const uint32_t k0 = i4a_transpose(i4_f16x2(x[0][0], x[0][1])), k8 = i4a_transpose(i4_f16x2(x[1][0], x[1][1]));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint32_t a = w[i & 2] >> (i & 1) * 8, d = w[(i & 2) + 1] >> (i & 1) * 8;
+                            float z[4];
+                            i4_mma_first(z, a & I4_NEAR, a & I4_FAR, d & I4_NEAR, d & I4_FAR, k0, k8);
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                float z[4];
-                                i4_mma_first(z, a & I4_NEAR, a & I4_FAR, d & I4_NEAR, d & I4_FAR, b[nt][0], b[nt][1]);
-#pragma unroll
-                                for (int x = 0; x < 4; ++x) o[gr * 4 + i][nt][x] = fmaf(z[x], up, o[gr * 4 + i][nt][x]);
-                            }
+                            for (int r = 0; r < 4; ++r) o[gr * 4 + i][nt][r] = fmaf(z[r], back[r & 1], o[gr * 4 + i][nt][r]);
                         }
                     }
+                }
                 continue;
             }
             probabilities();

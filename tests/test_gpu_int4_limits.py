@@ -570,3 +570,74 @@ def test_the_largest_numbers_come_back_finite(ops, dtype):
     y[:, 5] = 2.0 ** -100
     for rows_of in (8, 20):                                  # a number that is finite stays one on its way to the tensor cores
         assert bool(torch.isfinite(ops.linear(y[:rows_of], w, torch.float32)).all())
+
+
+# ------------------------------------------------------------------------------------------------ inputs of very unlike sizes
+def lined_up(x, w):
+    """What lining products up cuts off (int4.cuh): 17 times 2^-14 of the largest |x| of the 16 inputs that an instruction takes, times the step.
+    Instruction (j, h) of a group takes inputs 32 t + 8 j + 2 h + {0, 1, 4, 5}, t = 0 .. 3."""
+    of = torch.tensor([[32 * t + 8 * j + 2 * h + e for t in range(4) for e in (0, 1, 4, 5)] for j in range(4) for h in range(2)], device=DEV)
+    groups = torch.nn.functional.pad(x.double().abs(), (0, -w.k % 128)).unflatten(1, (-1, 128))
+    return 17 * 2 ** -14 * groups[:, :, of].amax(-1).sum(-1) @ plain.unpack_weight(w)[1].t()
+
+
+@pytest.mark.parametrize("spread", [1.0, 2.0, 4.0])
+@pytest.mark.parametrize("m,n,k", [(1, 777, 65), (8, 33, 128), (7, 32, 1024), (16, 64, 4096)])
+def test_inputs_of_very_unlike_sizes(ops, m, n, k, spread):
+    """Inputs that span up to 2^30, and some 300 times as large as their neighbours."""
+    for seed in range(6):
+        g = gen(seed + k)
+        w = random_weight(ops, g, n, k)
+        x = (randn(g, m, k) * torch.exp(spread * randn(g, k))).to(torch.bfloat16)
+        if seed % 2:
+            x[:, seed % k] *= 300
+        want = x.double() @ plain.values(*plain.unpack_weight(w), 128).t()
+        got = ops.linear(x, w, torch.float32).double()
+        assert float(((got - want).abs() / (linear_bound(x, w) + lined_up(x, w) + 2 ** -24 * want.abs())).max()) <= 1
+
+
+def attention_lined_up(q, k_rows, v_rows, table, spans, scale, window):
+    """What lining products up (int4.cuh) can cut off of `plain.attention`'s results: 17 times 2^-14 of the largest |q| of every 16 numbers of a
+    head, times a key's step, in its score, which a result sees twice; and of the largest p step of every 16 keys."""
+    of = torch.tensor([[32 * h + 8 * t + 2 * i + e for t in range(4) for e in (0, 1, 4, 5)] for h in range(2) for i in range(2)], device=DEV)
+    n, n_q, d = q.shape
+    out = torch.zeros(n, n_q * d, dtype=torch.float64, device=DEV)
+    for slot, row, count, past in spans:
+        (kc, ks, kl), (vc, vs, vl) = (plain.sequence(r, table[slot], past + count) for r in (k_rows, v_rows))
+        k, v = plain.values(kc, ks, kl, 64), plain.values(vc, vs, vl, 64)
+        i, j = torch.arange(past, past + count, device=DEV)[:, None], torch.arange(past + count, device=DEV)[None]
+        hidden = (j > i) | ((j <= i - window) if window else torch.zeros_like(j > i))
+        for h in range(n_q):
+            e, x = h // (n_q // k.shape[0]), q[row:row + count, h].double()
+            p = torch.softmax((x @ k[e].t() * scale).masked_fill(hidden, -float("inf")), dim=1)
+            most = x.abs().unflatten(1, (-1, 64))[:, :, of].amax(-1).sum(-1)
+            off = (17 * 2 ** -14 * 1.4427 * scale * (most @ ks[e].t())).masked_fill(hidden, 0.0).amax(1, keepdim=True)
+            steps = torch.nn.functional.pad(p[:, :, None] * vs[e][None], (0, 0, 0, -(past + count) % 16)).unflatten(1, (-1, 16)).amax(2).sum(1)
+            out[row:row + count, h * d:(h + 1) * d] = 2 * off * (p @ v[e].abs()) + 17 * 2 ** -14 * steps.repeat_interleave(64, -1)
+    return out
+
+
+@pytest.mark.parametrize("down", [0, 14, 20])
+@pytest.mark.parametrize("at", [0, 20, 150])
+@pytest.mark.parametrize("heads,d,new", [(4, 128, 1), (2, 64, 1), (4, 64, 7), (16, 128, 1)])
+def test_one_small_value_with_nearly_all_the_weight(ops, heads, d, new, at, down):
+    """A key with nearly all the probability whose values are 2^-`down` of the others': these, far more of them and each of hardly any weight,
+    are to be as exact as the sum of all asks, in front of that key and behind it, and for tokens that do not see the largest."""
+    n = 200 + new
+    g = gen(97 + at)
+    k_rows, v_rows, table, status, k, v, pos, slot = make_cache(ops, g, [n], 1, d, 64)
+    k *= 0.05
+    k[at] = 20.0 / d ** 0.5                                  # its score lies about 20 above the others'
+    v[at] *= 2.0 ** -down
+    v[-1] *= 2.0 ** 12
+    ops.int4.append(k, v, k_rows, v_rows, table, pos, slot, status)
+    q = (1 + 0.1 * randn(g, new, heads, d)).to(torch.bfloat16)
+    spans = [(0, 0, new, n - new)]
+    args = (q, k_rows, v_rows, table, spans, d ** -0.5, 0)
+    want, bound = plain.attention(*args)
+    if new == 1:
+        got = [ops.int4.attention_decode(q, k_rows, v_rows, table, pos[-1:], slot[:1], d ** -0.5, 0, status, n_splits=s) for s in (None, 1)]
+    else:
+        got = [ops.int4.attention_prompt(q, k_rows, v_rows, table, *runs_and_blocks(spans, 0), d ** -0.5, 0, status)]
+    for t in got:
+        check_attention(t, want, bound + attention_lined_up(*args))
