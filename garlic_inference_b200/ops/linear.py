@@ -81,10 +81,10 @@ INT4_GATED_BYTES = 1 << 30
 
 def _int4(x: torch.Tensor, w: int4.Int4Weight, out_dtype: torch.dtype, unit: Optional[tuple] = None,
           out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The product with a weight in 4 bits, or (`unit`) the gated unit of its halves.  bfloat16: up to 16 rows `int4.linear_rows`
-    where it has room (17 rows of 4,096 x 4,096: 15 us in two pieces, 10 in one of the next), up to INT4_CODES_MAX_ROWS `int4.linear_wide`.  More, or float32: the weight is made wide, some outputs at a time, for the products that
-    `linear` has for that type.  Beyond `linear_rows` bfloat16 rounds each number of the weight once on the way (by half a step of
-    2^-8, a hundredth of what 4 bits leave of it)."""
+    """The product with a weight in 4 bits, or (`unit`) the gated unit of its halves.  bfloat16: up to 16 rows `int4.linear_rows` where it
+    has room (17 rows of 4,096 x 4,096: 15 us in two pieces, 10 in one of the next), up to INT4_CODES_MAX_ROWS `int4.linear_wide`.  More, or
+    float32: the weight is made wide, some outputs at a time, for the products that `linear` has for that type.  Beyond `linear_rows`
+    bfloat16 rounds each number of the weight once on the way (by half a step of 2^-8, a hundredth of what 4 bits leave of it)."""
     if x.dim() != 2 or x.shape[1] != w.k:
         raise KernelError(f"linear: x {tuple(x.shape)} does not fit a weight {w.shape} ([out, in])")
     if unit is not None and w.n % 2:
